@@ -32,15 +32,57 @@
 #include "../../include/forge_q.h"
 #include "fq_kernels.h"
 #include "fq_pack.h"
+#include "fq_scratch.h"
 
 namespace {
 
 thread_local int g_last_hip = 0;
 
+}  // namespace
+
+namespace fq {
+
 int hip_fail(hipError_t e) {
     g_last_hip = (int)e;
     return FQ_ERR_HIP;
 }
+
+DevInfo device_info(int dev) {
+    static std::mutex mu;
+    static std::map<int, DevInfo> cache;
+    std::lock_guard<std::mutex> lk(mu);
+    auto it = cache.find(dev);
+    if (it != cache.end()) return it->second;
+    DevInfo d;
+    if (hipDeviceGetAttribute(&d.cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess) d.cus = 0;
+    int lds = 0;
+    if (hipDeviceGetAttribute(&lds, hipDeviceAttributeMaxSharedMemoryPerBlock, dev) != hipSuccess) lds = 0;
+    d.lds = (size_t)lds;
+    if (d.cus <= 0) d.cus = 256;
+    if (d.lds == 0) d.lds = 64 * 1024;
+    cache[dev] = d;
+    return d;
+}
+
+std::mutex g_scratch_mu;
+std::map<std::tuple<int, hipStream_t, int>, std::unique_ptr<StreamScratch>> g_scratch;
+
+StreamScratch& stream_scratch(int dev, hipStream_t st, int slot) {
+    std::lock_guard<std::mutex> lk(g_scratch_mu);
+    auto& p = g_scratch[{dev, st, slot}];
+    if (!p) p.reset(new StreamScratch);
+    return *p;
+}
+
+}  // namespace fq
+
+using fq::device_info;
+using fq::DevInfo;
+using fq::hip_fail;
+using fq::stream_scratch;
+using fq::StreamScratch;
+
+namespace {
 
 struct Geometry {
     int be, bb, ng;
@@ -67,86 +109,6 @@ bool row_fits(const Geometry& g, int K) { return (int64_t)(K / g.be) * g.bb <= I
 
 // Formats with the aligned packed layout (fq_pack.h).
 bool packable(uint32_t dtype) { return fq::packed_row_bytes((int)dtype, 256) > 0; }
-
-struct DevInfo {
-    int cus = 0;
-    size_t lds = 0;
-};
-
-DevInfo device_info(int dev) {
-    static std::mutex mu;
-    static std::map<int, DevInfo> cache;
-    std::lock_guard<std::mutex> lk(mu);
-    auto it = cache.find(dev);
-    if (it != cache.end()) return it->second;
-    DevInfo d;
-    if (hipDeviceGetAttribute(&d.cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess) d.cus = 0;
-    int lds = 0;
-    if (hipDeviceGetAttribute(&lds, hipDeviceAttributeMaxSharedMemoryPerBlock, dev) != hipSuccess) lds = 0;
-    d.lds = (size_t)lds;
-    if (d.cus <= 0) d.cus = 256;
-    if (d.lds == 0) d.lds = 64 * 1024;
-    cache[dev] = d;
-    return d;
-}
-
-// Device scratch per (device, stream, slot) for the MFMA path (slot 0: token
-// operands, group sums, exponents and split-K partial slabs) and the GGUF
-// fused FFN / QKV (slot 1: the gate/up or per-matrix rows).
-//
-// A call holds its slot's lock (StreamScratch::Lease) from taking the pointer
-// until its launches are enqueued, so two host threads sharing a stream never
-// see a buffer change under them.  The buffer only grows, at least doubling;
-// a superseded buffer is not freed inside a compute call (queued work may
-// still read it, and waiting for it would block the host mid-stream): it is
-// kept until fq_release_workspace(), so the workspace of a stream holds less
-// than twice its largest request.  fq_reserve_workspace() sizes it up front;
-// during HIP-graph capture a call that would have to grow it fails with
-// FQ_ERR_WORKSPACE instead of allocating.
-struct StreamScratch {
-    std::mutex mu;
-    uint8_t* p = nullptr;
-    size_t n = 0;
-    std::vector<uint8_t*> retired;
-
-    class Lease {
-      public:
-        explicit Lease(StreamScratch& s) : lk_(s.mu), s_(s) {}
-        // the slot's buffer, at least `bytes` long
-        int get(size_t bytes, hipStream_t st, uint8_t** out) {
-            if (s_.n < bytes) {
-                hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
-                if (st && hipStreamIsCapturing(st, &cs) == hipSuccess &&
-                    cs != hipStreamCaptureStatusNone)
-                    return FQ_ERR_WORKSPACE;
-                const size_t want = std::max(bytes, 2 * s_.n);
-                uint8_t* np = nullptr;
-                const hipError_t e = hipMalloc(reinterpret_cast<void**>(&np), want);
-                if (e != hipSuccess) return hip_fail(e);
-                if (s_.p) s_.retired.push_back(s_.p);
-                s_.p = np;
-                s_.n = want;
-            }
-            *out = s_.p;
-            return FQ_OK;
-        }
-        size_t held() const { return s_.n; }
-
-      private:
-        std::unique_lock<std::mutex> lk_;
-        StreamScratch& s_;
-    };
-};
-
-std::mutex g_scratch_mu;
-std::map<std::tuple<int, hipStream_t, int>, std::unique_ptr<StreamScratch>> g_scratch;
-
-StreamScratch& stream_scratch(int dev, hipStream_t st, int slot) {
-    std::lock_guard<std::mutex> lk(g_scratch_mu);
-    auto& p = g_scratch[{dev, st, slot}];
-    if (!p) p.reset(new StreamScratch);
-    return *p;
-}
 
 // Workspace bytes of the MFMA path for one call (the same plan run_mmq makes).
 struct MmqPlan {
@@ -1794,7 +1756,7 @@ int fq_release_workspace(void* stream) {
     if (e != hipSuccess) return hip_fail(e);
     e = hipStreamSynchronize(st);  // queued work may still read the buffers
     if (e != hipSuccess) return hip_fail(e);
-    for (int slot = 0; slot < 2; ++slot) {
+    for (int slot = 0; slot < fq::kScratchSlots; ++slot) {
         StreamScratch& s = stream_scratch(dev, st, slot);
         std::lock_guard<std::mutex> lk(s.mu);
         for (uint8_t* r : s.retired) hipFree(r);
