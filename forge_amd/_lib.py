@@ -1,4 +1,4 @@
-"""ctypes binding of the C ABI in include/forge_q.h (libforge_q.so).
+"""ctypes binding of the C ABI in include/forge_q.h and forge_step.h (libforge_q.so).
 
 The library is loaded from this package directory only.  There is no
 fallback: if the shared library is missing the import of ``lib()`` raises,
@@ -21,11 +21,12 @@ FQ_ERR_NO_DEVICE = 5
 FQ_ERR_ALIGN = 6
 FQ_ERR_WORKSPACE = 7
 
-# Every symbol include/forge_q.h declares, with its ctypes signature.
+# Every symbol that include/forge_q.h and forge_step.h declare, with its ctypes signature.
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _U = ctypes.c_uint32
 _L = ctypes.c_int64
+_F = ctypes.c_float
 SIGNATURES = {
     "fq_block_info": (_I, [_U, ctypes.POINTER(_I), ctypes.POINTER(_I)]),
     "fq_status_str": (ctypes.c_char_p, [_I]),
@@ -48,6 +49,13 @@ SIGNATURES = {
     "fq_matmul_transB_noalloc": (_I, [_U, _P, _P, _P, _I, _L, _P, _I, _I, _I, _P]),
     "fq_reserve_workspace": (_I, [_I, _I, _I, _P]),
     "fq_release_workspace": (_I, [_P]),
+    "fq_plan_step": (_I, [_P, _P, _P, _I, _I, _I, _P, _I, _L, _P, _I, _P, _P, _P, _P, _P, _P]),
+    "fq_qk_norm_rope": (_I, [_P, _L, _I, _I, _I, _I, _I, _I, _P, _P, _P, _F, _P, _P, _P, _I, _P,
+                             _U, _P, _P, _I, _I, _L, _L, _L, _P]),
+    "fq_tree_attention": (_I, [_P, _L, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _U, _P, _P, _I, _I,
+                               _L, _L, _L, _P, _I, _L, _P, _P]),
+    "fq_token_logprobs": (_I, [_P, _U, _L, _I, _I, _P, _I, _I, _P, _P, _P, _P, _P]),
+    "fq_reserve_step": (_I, [_P]),
 }
 
 _lib = None

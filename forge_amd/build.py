@@ -23,6 +23,7 @@ ARCH = "gfx950"
 
 SOURCES = ["fq_dequant.hip", "fq_gemv1.hip", "fq_gemvp.hip", "fq_gemvt.hip", "fq_pack.hip", "fq_mmq.hip",
            "fq_mmqi.hip", "fq_mmqs.hip", "fq_mmqp.hip", "fq_mmqk.hip", "fq_mmqt.hip",
+           "fq_plan.hip", "fq_rope.hip", "fq_attn.hip", "fq_logp.hip", "fq_step_capi.cpp",
            "fq_capi.cpp"]
 
 COMMON = [
