@@ -98,103 +98,134 @@ __device__ __forceinline__ void split2(float x0, float x1, uint32_t (&p)[Parts<B
     }
 }
 
-// Where a work-group's units begin.
-struct Place {
-    int b;        // request
-    int64_t off;  // units of b before it
+// What a request brings.
+struct Request {
+    int t0, nt, len;  // its first new token, how many, its cached tokens
+    int keys, nu;     // keys and units of them
+    int rts;          // tiles of RT rows
+    int64_t units;
 };
-
 template <int RT, int KU>
-__device__ __forceinline__ void request(const AttnArgs& a, int b, int& t0, int& nt, int& len,
-                                        int& keys, int& nu, int& rts) {
-    t0 = min(max(sload(a.cu + b), 0), a.N);
-    nt = min(max(sload(a.cu + b + 1), t0), a.N) - t0;
-    len = max(sload(a.lengths + b), 0);
+__device__ __forceinline__ Request request(const AttnArgs& a, int c0, int c1, int len) {
+    Request r;
+    r.t0 = min(max(c0, 0), a.N);
+    r.nt = min(max(c1, r.t0), a.N) - r.t0;
+    r.len = max(len, 0);
     // (no key lies beyond the table's columns)
     const int64_t most = (int64_t)a.max_blocks << a.c.bs_log2;
-    keys = (int)min((int64_t)len + nt, min(most, (int64_t)INT32_MAX - 64));
-    nu = (keys + KU - 1) / KU;
-    rts = (int)(((int64_t)nt * a.G + RT - 1) / RT);
+    r.keys = (int)min((int64_t)r.len + r.nt, min(most, (int64_t)INT32_MAX - 4096));
+    r.nu = (r.keys + KU - 1) / KU;
+    r.rts = (int)(((int64_t)r.nt * a.G + RT - 1) / RT);
+    r.units = (int64_t)a.hkv * r.rts * r.nu;
+    return r;
 }
 
-template <bool BF16, int D, int NR, int WK>
+__device__ __forceinline__ int64_t uni64(int64_t v) {
+    return ((int64_t)uni((int)(v >> 32)) << 32) | (uint32_t)uni((int)v);
+}
+
+// The largest of the four lanes (l % 16 + 0, 16, 32, 48).
+__device__ __forceinline__ float max4(float x) {
+    const uint32_t u = __float_as_uint(x);
+    const u2 p = __builtin_bit_cast(u2, __builtin_amdgcn_permlane16_swap(u, u, false, false));
+    x = fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
+    const uint32_t v = __float_as_uint(x);
+    const u2 q = __builtin_bit_cast(u2, __builtin_amdgcn_permlane32_swap(v, v, false, false));
+    return fmaxf(__uint_as_float(q[0]), __uint_as_float(q[1]));
+}
+__device__ __forceinline__ float sum4(float x) {
+    const uint32_t u = __float_as_uint(x);
+    const u2 p = __builtin_bit_cast(u2, __builtin_amdgcn_permlane16_swap(u, u, false, false));
+    x = __uint_as_float(p[0]) + __uint_as_float(p[1]);
+    const uint32_t v = __float_as_uint(x);
+    const u2 q = __builtin_bit_cast(u2, __builtin_amdgcn_permlane32_swap(v, v, false, false));
+    return __uint_as_float(q[0]) + __uint_as_float(q[1]);
+}
+
+// Ones at the n lowest places (none for n <= 0, all from 32 on).
+__device__ __forceinline__ uint32_t low_bits(int n) {
+    return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1;
+}
+// The places 0 .. 31 of m moved n up (down where n < 0).
+__device__ __forceinline__ uint32_t shifted(uint64_t m, int n) {
+    return n >= 32 || n <= -64 ? 0u : n >= 0 ? (uint32_t)m << n : (uint32_t)(m >> -n);
+}
+
+// WR x WK waves: each group of WR shares tiles of 32 keys, each of its waves
+// with 16 NR rows of its own; the groups take every WK-th tile.  NS tiles of a
+// group are in LDS.
+template <bool BF16_, int D_, int NR_, int WR_, int WK_, int NS_>
 struct Shape {
+    static constexpr bool BF16 = BF16_;
+    static constexpr int D = D_, NR = NR_, WR = WR_, WK = WK_, NS = NS_;
+    static constexpr int WAVES = WR * WK;
     static constexpr int DP = D <= 64 ? 64 : D <= 128 ? 128 : 256;  // LDS row, elements
     static constexpr int PITCH = 2 * DP;
-    static constexpr int TILE = KT * PITCH;      // bytes
-    static constexpr int WAVE = 4 * TILE;        // two of keys, two of values
-    static constexpr int RT = 16 * NR;
+    static constexpr int RT = 16 * NR * WR;
     static constexpr int KU = KT * WK;
     static constexpr int ROWS = 1024 / PITCH;    // rows of one copy
     static constexpr int J = 16 / ROWS;          // copies of 16 rows
     static constexpr int NI = 2 * J;             // copies of a tile
-    static constexpr size_t LDS = (size_t)WK * WAVE;
+    static constexpr int CW = 2 * NI / WR;       // copies of a wave for a tile's keys and values
+    // Bytes from copy to copy in LDS, and which bits of a row's number change
+    // places of its 16-byte pieces (keys: of four, values: of four pairs): chosen so
+    // that the 16 lanes of a read find 16 (values: 8) places of the 256
+    // bytes that the banks span, with every place an immediate offset from few registers.
+    static constexpr int KSTEP = 1024 + (D == 256 ? 32 : 64);
+    static constexpr int VSTEP = 1024 + (D == 256 ? 64 : D == 64 ? 0 : 128);
+    static __device__ __forceinline__ int turn(int row) {
+        return D == 64 ? (row >> 1) & 3 : D == 256 ? row & 1 : row & 3;
+    }
+    static constexpr int KTILE = NI * KSTEP, VTILE = NI * VSTEP, STAGE = KTILE + VTILE;
+    static constexpr int GROUP = NS * STAGE;
+    static constexpr size_t LDS = (size_t)WK * GROUP;
     static constexpr int PART = RT * (D + 2);    // floats of a partial result
+    static_assert(2 * NI % WR == 0 && (WR == 1 ? NS == 2 : true), "copies");
+    // the waves' outputs are exchanged where the tiles were
+    static_assert((size_t)WAVES * NR * 16 * D * 4 <= LDS, "join");
+    static_assert(D / 16 % WK == 0, "join");
 };
 
 constexpr int DESC = 8;  // ints of a work-group's record
+constexpr int MAX_GRID = 2;                  // work-groups to a CU at most,
+constexpr size_t MAX_PART = 128 * (128 + 2); // and the floats of a part of each
 
-template <bool BF16, int D, int NR, int WK>
-__global__ __launch_bounds__(64 * WK, 1) void attn_kernel(AttnArgs a) {
-    using S = Shape<BF16, D, NR, WK>;
+template <class S>
+__global__ __launch_bounds__(64 * S::WAVES, 1) void attn_kernel(AttnArgs a) {
+    constexpr bool BF16 = S::BF16;
+    constexpr int D = S::D, NR = S::NR, WR = S::WR, WK = S::WK, NS = S::NS;
     constexpr int NL = Parts<BF16>::N;
-    constexpr int RT = S::RT, KU = S::KU, TILE = S::TILE, PITCH = S::PITCH, J = S::J;
+    constexpr int RT = S::RT, KU = S::KU, PITCH = S::PITCH, J = S::J, NI = S::NI, ROWS = S::ROWS;
     constexpr int STEPS = D / 32, DT = D / 16, SLOTS = S::DP / 8;
+    constexpr uint32_t EXP = BF16 ? 0x7F80u : 0x7C00u;  // the exponent of what is not finite
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
-    __shared__ int64_t s_part[64 * WK];
-    __shared__ int s_b;
-    __shared__ int64_t s_off;
     __shared__ float s_ml[2][WK][RT];
-    const int tid = threadIdx.x, lane = tid & 63, wk = uni(tid >> 6);
+    __shared__ int s_odd[WK];
+    const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6);
+    const int wr = wave % WR, wk = wave / WR;
     const int n16 = lane & 15, g = lane >> 4;
     const int wg = blockIdx.x;
 
-    // --- the work-group's units ---
-    int64_t total, span, u0;
+    // --- the work-group's units (every wave finds them for itself) ---
+    int64_t total, span, off;
+    int b;
     {
-        constexpr int T = 64 * WK;
-        const int per = (a.B + T - 1) / T;
+        const int per = (a.B + 63) / 64, first = lane * per;
         int64_t mine = 0;
-        for (int i = 0; i < per; ++i) {
-            const int b = tid * per + i;
-            if (b < a.B) {
-                const int c0 = min(max(a.cu[b], 0), a.N);
-                const int nt = min(max(a.cu[b + 1], c0), a.N) - c0;
-                const int len = max(a.lengths[b], 0);
-                const int64_t most = (int64_t)a.max_blocks << a.c.bs_log2;
-                const int keys = (int)min((int64_t)len + nt, min(most, (int64_t)INT32_MAX - 64));
-                mine += (int64_t)a.hkv * (((int64_t)nt * a.G + RT - 1) / RT) * ((keys + KU - 1) / KU);
-            }
+        for (int i = first; i < min(first + per, a.B); ++i)
+            mine += request<RT, KU>(a, a.cu[i], a.cu[i + 1], a.lengths[i]).units;
+        int64_t upto = mine;
+        for (int o = 1; o < 64; o <<= 1) {
+            const int64_t v = __shfl_up(upto, o);
+            if (lane >= o) upto += v;
         }
-        s_part[tid] = mine;
-        __syncthreads();
-        int64_t before = 0;
-        total = 0;
-        for (int i = 0; i < T; ++i) {
-            const int64_t v = s_part[i];
-            total += v;
-            if (i < tid) before += v;
-        }
+        total = uni64(__shfl(upto, 63));
         span = (total + gridDim.x - 1) / gridDim.x;
-        u0 = wg * span;
-        if (u0 >= before && u0 < before + mine) {
-            int b = tid * per;
-            int64_t off = u0 - before;
-            for (;; ++b) {
-                const int c0 = min(max(a.cu[b], 0), a.N);
-                const int nt = min(max(a.cu[b + 1], c0), a.N) - c0;
-                const int len = max(a.lengths[b], 0);
-                const int64_t most = (int64_t)a.max_blocks << a.c.bs_log2;
-                const int keys = (int)min((int64_t)len + nt, min(most, (int64_t)INT32_MAX - 64));
-                const int64_t n =
-                    (int64_t)a.hkv * (((int64_t)nt * a.G + RT - 1) / RT) * ((keys + KU - 1) / KU);
-                if (off < n) break;
-                off -= n;
-            }
-            s_b = b;
-            s_off = off;
-        }
-        __syncthreads();
+        const int64_t u0 = wg * span;
+        const uint64_t past = __ballot(upto > u0);
+        const int at = past ? __builtin_ctzll(past) : 0;
+        b = at * per;
+        off = u0 - uni64(__shfl(upto - mine, at));
     }
     int* desc = a.desc + wg * DESC;
     // padding tokens
@@ -205,281 +236,312 @@ __global__ __launch_bounds__(64 * WK, 1) void attn_kernel(AttnArgs a) {
              i += (int64_t)gridDim.x * blockDim.x)
             a.out[i] = 0.0f;
     }
-    if (u0 >= total) {
+    int64_t u = wg * span;
+    if (u >= total) {
         if (tid == 0) desc[0] = 0;
         return;
     }
-    int64_t left = min(span, total - u0);
-    int b = uni(s_b);
-    int64_t off = s_off;
-    off = ((int64_t)uni((int)(off >> 32)) << 32) | (uint32_t)uni((int)off);
-    left = ((int64_t)uni((int)(left >> 32)) << 32) | (uint32_t)uni((int)left);
-    int64_t u = u0;
+    int64_t left = min(span, total - u);
     bool cut = false;  // an item begun here goes on in the next work-group
 
+    if (tid < WK) s_odd[tid] = 0;
+    __syncthreads();
+
     // --- constants of a lane ---
-    const uint32_t wbase = lds_addr(lds) + wk * S::WAVE;  // K0 K1 V0 V1
-    uint32_t koff[J], voff[J];  // a copy's source in its rows: bytes from their first
-    #pragma unroll
-    for (int j = 0; j < J; ++j) {
-        const int row = j * S::ROWS + lane / SLOTS, slot = lane % SLOTS;
-        const int fk = D <= 64 ? (row >> 1) & 7 : row & 15;
-        const int fv = D <= 64 ? (row >> 1) & 3 : row & 7;
-        int ck = slot ^ fk, cv = slot ^ (fv << 1);
+    const uint32_t gbase = lds_addr(lds) + wk * S::GROUP;
+    // a copy's source: bytes from its first row
+    uint32_t ksrc, vsrc;
+    {
+        const int row = lane / SLOTS, slot = lane % SLOTS;
+        int ck = slot ^ S::turn(row), cv = slot ^ (S::turn(row) << 1);
         if (8 * ck >= D) ck -= 4;  // (rows of 12 pieces among 16: the rest is not read)
         if (8 * cv >= D) cv -= 4;
-        const uint32_t rb = (uint32_t)((lane / SLOTS) * a.c.st * 2);
-        koff[j] = rb + ck * 16;
-        voff[j] = rb + cv * 16;
+        ksrc = (uint32_t)(row * a.c.st * 2) + ck * 16;
+        vsrc = (uint32_t)(row * a.c.st * 2) + cv * 16;
     }
-    const int fk = D <= 64 ? (n16 >> 1) & 7 : n16;
-    const int vrow = 4 * g + (n16 >> 2);
-    const int fv = D <= 64 ? (vrow >> 1) & 3 : vrow & 7;
-    const uint32_t vlane = vrow * PITCH + (n16 & 3) * 8;
+    const uint32_t klane = gbase + n16 / ROWS * S::KSTEP + n16 % ROWS * PITCH +
+                           ((g ^ S::turn(n16)) << 4);
+    uint32_t vlane[4];
+    {
+        const int row = 4 * g + (n16 >> 2);
+#pragma unroll
+        for (int d = 0; d < 4; ++d)
+            vlane[d] = gbase + S::KTILE + row / ROWS * S::VSTEP + row % ROWS * PITCH +
+                       ((d ^ S::turn(row)) << 5) + (n16 & 3) * 8;
+    }
 
     for (; left > 0; ++b) {
-        int t0, nt, len, keys, nu, rts;
-        request<RT, KU>(a, b, t0, nt, len, keys, nu, rts);
-        const int64_t units = (int64_t)a.hkv * rts * nu;
-        while (off < units && left > 0) {
+        const Request rq = request<RT, KU>(a, sload(a.cu + b), sload(a.cu + b + 1), sload(a.lengths + b));
+        const int len = rq.len, keys = rq.keys, nu = rq.nu, t0 = rq.t0, nt = rq.nt;
+        while (off < rq.units && left > 0) {
             const int item = (int)(off / nu), first = (int)(off % nu);
-            const int h = item / rts, rt = item % rts;
+            const int h = item / rq.rts, rt = item % rq.rts;
             const int count = (int)min((int64_t)(nu - first), left);
 
             // --- queries ---
             u4 qf[NR][STEPS][NL];
             float rs[NR];
             uint64_t mask[NR];
-            int tq[NR];
-            #pragma unroll
+#pragma unroll
             for (int c = 0; c < NR; ++c) {
-                const int r = rt * RT + 16 * c + n16;
+                const int r = rt * RT + wr * 16 * NR + 16 * c + n16;
                 const int t = r / a.G, hh = h * a.G + r % a.G;
                 const bool on = t < nt;
-                tq[c] = on ? t : 0;
-                mask[c] = a.masks ? (on ? a.masks[t0 + t] : 0) : 0;
-                const float* q = a.q + (int64_t)(t0 + tq[c]) * a.ldq + (int64_t)(on ? hh : 0) * D;
+                // (a chain: how many of the new tokens the row sees)
+                mask[c] = !on ? 0 : a.masks ? a.masks[t0 + t] : (uint64_t)t + 1;
+                const float* q = a.q + (int64_t)(t0 + (on ? t : 0)) * a.ldq + (int64_t)(on ? hh : 0) * D;
                 f4 x[STEPS][2];
                 float mx = 0.0f;
-                #pragma unroll
+#pragma unroll
                 for (int s = 0; s < STEPS; ++s)
-                    #pragma unroll
+#pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         x[s][i] = on ? *(const f4u*)(q + 32 * s + 8 * g + 4 * i) : f4{0, 0, 0, 0};
-                        #pragma unroll
+#pragma unroll
                         for (int e = 0; e < 4; ++e) mx = fmaxf(mx, fabsf(x[s][i][e]));
                     }
                 float up = 1.0f, down = 1.0f;
                 if (!BF16) {  // the row's largest to [2^14, 2^15)
-                    mx = fmaxf(mx, __shfl_xor(mx, 16));
-                    mx = fmaxf(mx, __shfl_xor(mx, 32));
+                    mx = max4(mx);
                     if (mx > 0.0f && mx < __builtin_inff()) {
                         const int e = min(max(15 - __builtin_amdgcn_frexp_expf(mx), -126), 126);
                         up = ldexpf(1.0f, e);
                         down = ldexpf(1.0f, -e);
                     }
                 }
-                rs[c] = down * a.scale;
-                #pragma unroll
+                // (the scale's sign goes with the query: the largest score is
+                // that of the largest product)
+                up = copysignf(up, a.scale);
+                rs[c] = down * fabsf(a.scale);
+#pragma unroll
                 for (int s = 0; s < STEPS; ++s)
-                    #pragma unroll
+#pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         uint32_t p[NL];
                         split2<BF16>(x[s][i >> 1][2 * (i & 1)] * up,
                                      x[s][i >> 1][2 * (i & 1) + 1] * up, p);
-                        #pragma unroll
+#pragma unroll
                         for (int l = 0; l < NL; ++l) qf[c][s][l][i] = p[l];
                     }
             }
 
-            // --- this wave's tiles: wk, wk + WK, .. of the segment's ---
+            // --- this group's tiles: wk, wk + WK, .. of the segment's.  Waves that
+            // share tiles keep step: as many tiles for each group (those past
+            // the last key are masked) ---
             const int kbeg = first * KU + wk * KT;
             const int kend = min(keys, (first + count) * KU);
-            const int n = kbeg < kend ? (kend - kbeg + KU - 1) / KU : 0;
+            const int n = WR > 1 ? (kend - first * KU + KU - 1) / KU
+                                 : kbeg < kend ? (kend - kbeg + KU - 1) / KU : 0;
             const int last16 = (keys - 1) & ~15;
             const uint8_t* kb = a.k + (int64_t)h * a.c.sh * 2;
             const uint8_t* vb = a.v + (int64_t)h * a.c.sh * 2;
             const int* table = a.table + b * a.table_stride;
-            const auto copy = [&](int i, const uint8_t* base, const uint32_t (&lo)[J], uint32_t at) {
-                #pragma unroll
+            const auto seen = [&](uint64_t m, int old, int all) {  // of a tile's keys
+                // (old: of the context, all: of the request)
+                const uint32_t s = a.masks ? low_bits(old) | shifted(m, old)
+                                           : low_bits(old + (int)(uint32_t)m);
+                return s & low_bits(all);
+            };
+            const auto offset = [&](int i, int hf) {  // of 16 keys, in their cache
+                const int key = min(kbeg + i * KU + 16 * hf, last16);
+                const int page = min(max(sload(table + (key >> a.c.bs_log2)), 0), a.c.num_blocks - 1);
+                return 2 * (page * a.c.sb + (key & ((1 << a.c.bs_log2) - 1)) * a.c.st);
+            };
+            int64_t pre[2];  // of the tile whose values are copied next (WR == 1)
+            const auto copy_k = [&](int i) {
+#pragma unroll
                 for (int hf = 0; hf < 2; ++hf) {
-                    const int key = min(kbeg + i * KU + 16 * hf, last16);
-                    const int page = min(max(sload(table + (key >> a.c.bs_log2)), 0), a.c.num_blocks - 1);
-                    const uint8_t* p = base + 2 * (page * a.c.sb + (key & ((1 << a.c.bs_log2) - 1)) * a.c.st);
-                    #pragma unroll
+                    pre[hf] = offset(i, hf);
+#pragma unroll
                     for (int j = 0; j < J; ++j)
-                        dma16s(lo[j], p + 2 * j * S::ROWS * a.c.st, at + (hf * J + j) * 1024);
+                        dma16s(ksrc, kb + pre[hf] + 2 * j * ROWS * a.c.st,
+                               gbase + (i & 1) * S::STAGE + (hf * J + j) * S::KSTEP);
                 }
             };
-            const auto copy_k = [&](int i) { copy(i, kb, koff, wbase + (i & 1) * TILE); };
-            const auto copy_v = [&](int i) { copy(i, vb, voff, wbase + (2 + (i & 1)) * TILE); };
+            const auto copy_v = [&](int i) {
+#pragma unroll
+                for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+                    for (int j = 0; j < J; ++j)
+                        dma16s(vsrc, vb + pre[hf] + 2 * j * ROWS * a.c.st,
+                               gbase + (i & 1) * S::STAGE + S::KTILE + (hf * J + j) * S::VSTEP);
+            };
+            const auto copy_all = [&](int i, int stage) {
+                const int64_t o0 = offset(i, 0), o1 = offset(i, 1);
+                const uint32_t to = gbase + stage * S::STAGE;
+#pragma unroll
+                for (int x = 0; x < S::CW; ++x) {
+                    const int ci = wr + WR * x, c = ci % NI;
+                    const int64_t from = (c >= J ? o1 : o0) + 2 * (c % J) * ROWS * a.c.st;
+                    if (ci < NI) dma16s(ksrc, kb + from, to + c * S::KSTEP);
+                    else dma16s(vsrc, vb + from, to + S::KTILE + c * S::VSTEP);
+                }
+            };
+
             f4 o[DT][NR];
             float mrow[NR], lrow[NR];
             bool careful = false;
         again:
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            if (n > 0) copy_k(0), copy_v(0);
-            if (n > 1) copy_k(1), copy_v(1);
-            #pragma unroll
+            if constexpr (WR == 1) {
+                if (n > 0) copy_k(0), copy_v(0);
+                if (n > 1) copy_k(1), copy_v(1);
+            } else {
+                __syncthreads();  // (again: the others may still read)
+#pragma unroll
+                for (int i = 0; i < NS - 1; ++i)
+                    if (i < n) copy_all(i, i);
+            }
+#pragma unroll
             for (int c = 0; c < NR; ++c) {
                 mrow[c] = LOWEST;
                 lrow[c] = 0.0f;
-                #pragma unroll
+#pragma unroll
                 for (int d = 0; d < DT; ++d) o[d][c] = f4{0, 0, 0, 0};
             }
+            int stage = 0;
             for (int i = 0; i < n; ++i) {
                 const int key0 = kbeg + i * KU;
+                const uint32_t sat = stage * S::STAGE;
+                if constexpr (WR == 1) {
+                    if (i + 1 < n) wait_vm<3 * NI>();
+                    else wait_vm<NI>();
+                } else {
+                    // this tile's copies of this wave have landed, then everyone's;
+                    // and all are done with the tile before, whose place is filled anew
+                    if (i + NS - 2 < n) wait_vm<(NS - 2) * S::CW>();
+                    else wait_vm<0>();
+                    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                    if (i + NS - 1 < n) copy_all(i + NS - 1, stage ? stage - 1 : NS - 1);
+                }
                 // scores
-                if (i + 1 < n) wait_vm<3 * S::NI>();
-                else wait_vm<S::NI>();
                 f4 sc[2][NR];
-                #pragma unroll
+#pragma unroll
                 for (int sub = 0; sub < 2; ++sub) {
-                    #pragma unroll
+#pragma unroll
                     for (int c = 0; c < NR; ++c) sc[sub][c] = f4{0, 0, 0, 0};
-                    #pragma unroll
+#pragma unroll
                     for (int s = 0; s < STEPS; ++s) {
-                        const uint32_t at = wbase + (i & 1) * TILE + (16 * sub + n16) * PITCH +
-                                            (((4 * s + g) ^ fk) << 4);
-                        const u4 kf = *(lds_u4*)(uintptr_t)at;
-                        #pragma unroll
+                        const u4 kf = *(lds_u4*)(uintptr_t)(klane + sat + J * sub * S::KSTEP + 64 * s);
+#pragma unroll
                         for (int c = 0; c < NR; ++c)
-                            #pragma unroll
+#pragma unroll
                             for (int l = NL - 1; l >= 0; --l)
                                 sc[sub][c] = mfma<BF16>(kf, qf[c][s][l], sc[sub][c]);
                     }
                 }
-                wait_lds();
-                if (i + 2 < n) copy_k(i + 2);
+                if constexpr (WR == 1) {
+                    wait_lds();
+                    if (i + 2 < n) copy_k(i + 2);
+                }
 
                 // softmax
                 const bool tail = careful || key0 + KT > len;
+                float mul[NR];
+#pragma unroll
+                for (int c = 0; c < NR; ++c) mul[c] = rs[c];
+                if (tail) {
+                    const int old = len - key0, all = keys - key0;
+#pragma unroll
+                    for (int c = 0; c < NR; ++c) {
+                        mul[c] = 1.0f;
+                        const uint32_t see = seen(mask[c], old, all) >> (4 * g);
+#pragma unroll
+                        for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r)
+                                sc[sub][c][r] = see >> (16 * sub + r) & 1 ? sc[sub][c][r] * rs[c]
+                                                                          : -__builtin_inff();
+                    }
+                }
                 u4 pf[NR][NL];
                 float alpha[NR];
                 bool moved = false;
-                #pragma unroll
+#pragma unroll
                 for (int c = 0; c < NR; ++c) {
-                    float mx = LOWEST;
-                    #pragma unroll
-                    for (int sub = 0; sub < 2; ++sub)
-                        #pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            float s = sc[sub][c][r] * rs[c];
-                            if (tail) {
-                                const int key = key0 + 16 * sub + 4 * g + r, j = key - len;
-                                const bool see =
-                                    key < keys && (j < 0 || (a.masks ? j < 64 && ((mask[c] >> (j & 63)) & 1)
-                                                                     : j <= tq[c]));
-                                s = see ? s : -__builtin_inff();
-                            }
-                            sc[sub][c][r] = s;
-                            mx = fmaxf(mx, s);
-                        }
-                    mx = fmaxf(mx, __shfl_xor(mx, 16));
-                    mx = fmaxf(mx, __shfl_xor(mx, 32));
-                    const float m = fmaxf(mrow[c], mx);
+                    float mx = sc[0][c][0];
+#pragma unroll
+                    for (int r = 1; r < 8; ++r) mx = fmaxf(mx, sc[r >> 2][c][r & 3]);
+                    const float m = fmaxf(mrow[c], max4(mx) * mul[c]);
                     moved |= m > mrow[c];
                     alpha[c] = __builtin_amdgcn_exp2f(mrow[c] - m);
                     mrow[c] = m;
-                    const float ref = BF16 ? m : m - 14.0f;
-                    float p[2][4], sum = 0.0f;
-                    #pragma unroll
-                    for (int sub = 0; sub < 2; ++sub)
-                        #pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            p[sub][r] = __builtin_amdgcn_exp2f(sc[sub][c][r] - ref);
-                            sum += p[sub][r];
-                        }
+                    const float ref = BF16 ? -m : 14.0f - m;
+                    float p[8], sum = 0.0f;
+#pragma unroll
+                    for (int r = 0; r < 8; ++r) {
+                        p[r] = __builtin_amdgcn_exp2f(fmaf(sc[r >> 2][c][r & 3], mul[c], ref));
+                        sum += p[r];
+                    }
                     lrow[c] = lrow[c] * alpha[c] + sum;
-                    #pragma unroll
-                    for (int sub = 0; sub < 2; ++sub)
-                        #pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            uint32_t q2[NL];
-                            split2<BF16>(p[sub][2 * e], p[sub][2 * e + 1], q2);
-                            #pragma unroll
-                            for (int l = 0; l < NL; ++l) pf[c][l][2 * sub + e] = q2[l];
-                        }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        uint32_t q2[NL];
+                        split2<BF16>(p[2 * e], p[2 * e + 1], q2);
+#pragma unroll
+                        for (int l = 0; l < NL; ++l) pf[c][l][e] = q2[l];
+                    }
                 }
                 if (__any(moved))
-                    #pragma unroll
+#pragma unroll
                     for (int c = 0; c < NR; ++c)
-                        #pragma unroll
+#pragma unroll
                         for (int d = 0; d < DT; ++d) o[d][c] *= alpha[c];
 
                 // values
-                if (i + 2 < n) wait_vm<3 * S::NI>();
-                else if (i + 1 < n) wait_vm<2 * S::NI>();
-                else wait_vm<0>();
-                #pragma unroll
-                for (int d = 0; d < DT; ++d) {
-                    const uint32_t at = wbase + (2 + (i & 1)) * TILE + vlane + ((d ^ fv) << 5);
+                if constexpr (WR == 1) {
+                    if (i + 2 < n) wait_vm<3 * NI>();
+                    else if (i + 1 < n) wait_vm<2 * NI>();
+                    else wait_vm<0>();
+                }
+                if (tail) {
+                    // values that are not finite: zeros, and noted where they are the request's.
+                    // (Waves that share the tile all do so, to the same effect.)
+                    bool odd = false;
+#pragma unroll 2
+                    for (int x = 0; x < NI; ++x) {
+                        auto* at = (__attribute__((address_space(3))) u4*)(uintptr_t)(
+                            gbase + sat + S::KTILE + x * S::VSTEP + lane * 16);
+                        u4 v = *at;
+                        bool bad = false;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const bool lo = (v[e] & EXP) == EXP, hi = (v[e] >> 16 & EXP) == EXP;
+                            bad |= lo | hi;
+                            v[e] = (lo ? 0u : v[e] & 0xFFFFu) | (hi ? 0u : v[e] & 0xFFFF0000u);
+                        }
+                        odd |= bad && key0 + x * ROWS + lane / SLOTS < keys;
+                        *at = v;
+                    }
+                    if (odd) s_odd[wk] = 1;
+                }
+                const auto value = [&](int d) {
+                    const uint32_t at = vlane[d & 3] + sat + (d >> 2) * 128;
                     const s4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(uintptr_t)at);
                     const s4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                        (lds_s4*)(uintptr_t)(at + 16 * PITCH));
+                        (lds_s4*)(uintptr_t)(at + J * S::VSTEP));
                     const u2 w0 = __builtin_bit_cast(u2, v0), w1 = __builtin_bit_cast(u2, v1);
-                    u4 vf = {w0[0], w0[1], w1[0], w1[1]};
-                    if (tail) {
-                        constexpr uint32_t EXP = BF16 ? 0x7F80u : 0x7C00u;
-                        const u4 raw = vf;
-                        bool odd = false;
-                        #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const bool lo = (raw[e] & EXP) == EXP, hi = (raw[e] >> 16 & EXP) == EXP;
-                            odd |= lo | hi;
-                            vf[e] = (lo ? 0u : raw[e] & 0xFFFFu) | (hi ? 0u : raw[e] & 0xFFFF0000u);
-                        }
-                        if (__any(odd)) {
-                            // which rows see a NaN, an infinity: counts of ones
-                            constexpr uint32_t ONE = BF16 ? 0x3F80u : 0x3C00u;
-                            #pragma unroll
-                            for (int kind = 0; kind < 3; ++kind) {
-                                const float val = kind == 0 ? __builtin_nanf("")
-                                                            : kind == 1 ? __builtin_inff() : -__builtin_inff();
-                                u4 ind;
-                                #pragma unroll
-                                for (int e = 0; e < 4; ++e) {
-                                    uint32_t w = 0;
-                                    #pragma unroll
-                                    for (int q = 0; q < 2; ++q) {
-                                        const uint32_t x = raw[e] >> (16 * q) & 0xFFFFu;
-                                        const bool is = kind == 0 ? (x & 0x7FFFu) > EXP
-                                                                  : x == (kind == 1 ? EXP : EXP | 0x8000u);
-                                        w |= is ? ONE << (16 * q) : 0u;
-                                    }
-                                    ind[e] = w;
-                                }
-                                #pragma unroll
-                                for (int c = 0; c < NR; ++c) {
-                                    u4 seen;
-                                    #pragma unroll
-                                    for (int e = 0; e < 4; ++e) {
-                                        uint32_t w = 0;
-                                        #pragma unroll
-                                        for (int q = 0; q < 2; ++q)
-                                            w |= sc[e >> 1][c][2 * (e & 1) + q] != -__builtin_inff()
-                                                     ? ONE << (16 * q) : 0u;
-                                        seen[e] = w;
-                                    }
-                                    const f4 hits = mfma<BF16>(ind, seen, f4{0, 0, 0, 0});
-                                    #pragma unroll
-                                    for (int r = 0; r < 4; ++r)
-                                        if (hits[r] > 0.0f) o[d][c][r] += val;
-                                }
-                            }
-                        }
-                    }
-                    #pragma unroll
+                    return u4{w0[0], w0[1], w1[0], w1[1]};
+                };
+#pragma unroll
+                for (int d = 0; d < DT; ++d) {
+                    const u4 vf = value(d);
+#pragma unroll
                     for (int c = 0; c < NR; ++c)
-                        #pragma unroll
+#pragma unroll
                         for (int l = NL - 1; l >= 0; --l) o[d][c] = mfma<BF16>(vf, pf[c][l], o[d][c]);
                 }
-                wait_lds();
-                if (i + 2 < n) copy_v(i + 2);
+                if constexpr (WR == 1) {
+                    wait_lds();
+                    if (i + 2 < n) copy_v(i + 2);
+                    stage ^= 1;
+                } else {
+                    stage = stage + 1 < NS ? stage + 1 : 0;
+                }
             }
 
             // an infinite cached value times the two signs (or a zero) of a
-            // probability's parts is NaN: once more, with the values looked at
+            // probability's parts is NaN: once more, with all values looked at
             if (!careful) {
                 bool nan = false;
 #pragma unroll
@@ -488,85 +550,100 @@ __global__ __launch_bounds__(64 * WK, 1) void attn_kernel(AttnArgs a) {
                     for (int d = 0; d < DT; ++d)
 #pragma unroll
                         for (int r = 0; r < 4; ++r) nan |= o[d][c][r] != o[d][c][r];
-                if (__any(nan)) {
+                nan = WR == 1 ? __any(nan) : __syncthreads_or(nan);
+                if (nan) {
                     careful = true;
                     goto again;
                 }
             }
 
-            // --- join the waves ---
-            #pragma unroll
+            // --- join the groups: each takes D / WK of the columns ---
+            int ln = lane;  // (opaque: addresses made from it are not kept through the tiles)
+            asm volatile("" : "+v"(ln));
+#pragma unroll
             for (int c = 0; c < NR; ++c) {
-                lrow[c] += __shfl_xor(lrow[c], 16);
-                lrow[c] += __shfl_xor(lrow[c], 32);
-                if (lane < 16) {
-                    s_ml[0][wk][16 * c + n16] = mrow[c];
-                    s_ml[1][wk][16 * c + n16] = lrow[c];
+                lrow[c] = sum4(lrow[c]);
+                if (ln < 16) {
+                    s_ml[0][wk][16 * (wr * NR + c) + ln % 16] = mrow[c];
+                    s_ml[1][wk][16 * (wr * NR + c) + ln % 16] = lrow[c];
                 }
             }
             __syncthreads();
-            float lsum[NR];
-            #pragma unroll
-            for (int c = 0; c < NR; ++c) {
-                float m = LOWEST;
-                #pragma unroll
-                for (int w = 0; w < WK; ++w) m = fmaxf(m, s_ml[0][w][16 * c + n16]);
-                lsum[c] = 0.0f;
-                #pragma unroll
-                for (int w = 0; w < WK; ++w)
-                    lsum[c] += s_ml[1][w][16 * c + n16] *
-                               __builtin_amdgcn_exp2f(s_ml[0][w][16 * c + n16] - m);
-                const float f = __builtin_amdgcn_exp2f(mrow[c] - m);
-                mrow[c] = m;
-                #pragma unroll
-                for (int d = 0; d < DT; ++d) o[d][c] *= f;
-            }
-            float* buf = (float*)lds;  // the tiles are not needed any more
-            for (int half = WK / 2; half; half >>= 1) {
-                if (wk >= half && wk < 2 * half)
-                    #pragma unroll
-                    for (int c = 0; c < NR; ++c)
-                        #pragma unroll
-                        for (int d = 0; d < DT; ++d)
-                            #pragma unroll
-                            for (int r = 0; r < 4; ++r)
-                                buf[(((wk - half) * NR + c) * DT + d) * 256 + r * 64 + lane] = o[d][c][r];
-                __syncthreads();
-                if (wk < half)
-                    #pragma unroll
-                    for (int c = 0; c < NR; ++c)
-                        #pragma unroll
-                        for (int d = 0; d < DT; ++d)
-                            #pragma unroll
-                            for (int r = 0; r < 4; ++r)
-                                o[d][c][r] += buf[((wk * NR + c) * DT + d) * 256 + r * 64 + lane];
-                __syncthreads();
-            }
-            const bool whole = count == nu;
-            if (wk == 0) {
-                float* part = a.part + (int64_t)(2 * wg + (first == 0)) * S::PART;
-                #pragma unroll
-                for (int c = 0; c < NR; ++c) {
-                    const int rl = 16 * c + n16, r = rt * RT + rl;
-                    const int t = r / a.G, hh = h * a.G + r % a.G;
-                    const float inv = lsum[c] != 0.0f ? 1.0f / lsum[c] : 0.0f;
-                    if (whole) {
-                        if (t < nt)
-                            #pragma unroll
-                            for (int d = 0; d < DT; ++d) {
-                                f4 v = o[d][c] * inv;
-                                if (lsum[c] == 0.0f) v = f4{0, 0, 0, 0};
-                                *(f4*)(a.out + ((int64_t)(t0 + t) * a.hq + hh) * D + 16 * d + 4 * g) = v;
-                            }
-                    } else {
-                        #pragma unroll
-                        for (int d = 0; d < DT; ++d)
-                            *(f4*)(part + rl * D + 16 * d + 4 * g) = o[d][c];
-                        if (g == 0) {
-                            part[RT * D + rl] = mrow[c];
-                            part[RT * D + RT + rl] = lsum[c];
+            if (s_odd[wk]) {
+                // what was taken out, back into the rows that see it
+#pragma unroll 1
+                for (int key = kbeg; key < kbeg + n * KU && key < keys; ++key) {
+                    const int at = (key - kbeg) % KU, key0 = key - at;
+                    if (at >= KT || !(careful || key0 + KT > len)) continue;
+                    const int page = min(max(sload(table + (key >> a.c.bs_log2)), 0), a.c.num_blocks - 1);
+                    const uint8_t* v = vb + 2 * (page * a.c.sb + (key & ((1 << a.c.bs_log2) - 1)) * a.c.st);
+                    bool see[NR];
+#pragma unroll
+                    for (int c = 0; c < NR; ++c) see[c] = seen(mask[c], len - key0, keys - key0) >> at & 1;
+#pragma unroll
+                    for (int d = 0; d < DT; ++d) {
+                        const u2 x = *(const u2*)(v + 2 * (16 * d + 4 * (ln / 16)));
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const uint32_t w = x[r >> 1] >> (16 * (r & 1)) & 0xFFFFu;
+                            const float f = (w & EXP) != EXP ? 0.0f
+                                            : w & (EXP ^ 0x7FFFu) ? __builtin_nanf("")
+                                            : w & 0x8000u ? -__builtin_inff() : __builtin_inff();
+#pragma unroll
+                            for (int c = 0; c < NR; ++c)
+                                if (see[c] && (w & EXP) == EXP) o[d][c][r] += f;
                         }
                     }
+                }
+            }
+            float* buf = (float*)lds;  // the tiles are not needed any more
+            float lsum[NR];
+#pragma unroll
+            for (int c = 0; c < NR; ++c) {
+                const int rl = 16 * (wr * NR + c) + ln % 16;
+                float m = LOWEST;
+#pragma unroll
+                for (int w = 0; w < WK; ++w) m = fmaxf(m, s_ml[0][w][rl]);
+                lsum[c] = 0.0f;
+#pragma unroll
+                for (int w = 0; w < WK; ++w)
+                    lsum[c] += s_ml[1][w][rl] * __builtin_amdgcn_exp2f(s_ml[0][w][rl] - m);
+                const float f = __builtin_amdgcn_exp2f(mrow[c] - m);
+                mrow[c] = m;
+#pragma unroll
+                for (int d = 0; d < DT; ++d) {
+                    o[d][c] *= f;
+                    if (WK > 1) *(f4*)(buf + (((wave * NR + c) * DT + d) * 64 + ln) * 4) = o[d][c];
+                }
+            }
+            __syncthreads();
+            if (tid < WK) s_odd[tid] = 0;
+            const bool whole = count == nu;
+            float* part = a.part + (int64_t)(2 * wg + (first == 0)) * S::PART;
+#pragma unroll
+            for (int c = 0; c < NR; ++c) {
+                const int rl = 16 * (wr * NR + c) + ln % 16, r = rt * RT + rl;
+                const int t = r / a.G, hh = h * a.G + r % a.G;
+                const float inv = lsum[c] != 0.0f ? 1.0f / lsum[c] : 0.0f;
+                float* to = whole ? a.out + ((int64_t)(t0 + t) * a.hq + hh) * D : part + rl * D;
+#pragma unroll
+                for (int d0 = 0; d0 < DT / WK; ++d0) {
+                    const int d = wk * (DT / WK) + d0;
+                    f4 v;
+                    if (WK > 1) {
+                        v = f4{0, 0, 0, 0};
+#pragma unroll
+                        for (int w = 0; w < WK; ++w)
+                            v += *(const f4*)(buf + ((((w * WR + wr) * NR + c) * DT + d) * 64 + ln) * 4);
+                    } else {
+                        v = o[d0][c];
+                    }
+                    if (whole) v = lsum[c] != 0.0f ? v * inv : f4{0, 0, 0, 0};
+                    if (!whole || t < nt) *(f4*)(to + 16 * d + 4 * (ln / 16)) = v;
+                }
+                if (!whole && wk == 0 && ln < 16) {
+                    part[RT * D + rl] = mrow[c];
+                    part[RT * D + RT + rl] = lsum[c];
                 }
             }
             if (first == 0 && !whole) {
@@ -580,8 +657,9 @@ __global__ __launch_bounds__(64 * WK, 1) void attn_kernel(AttnArgs a) {
             u += count;
             off += count;
             left -= count;
+            __syncthreads();  // the exchanged outputs are read
         }
-        off -= units;
+        off -= rq.units;
     }
     if (!cut && tid == 0) desc[0] = 0;
 }
@@ -628,42 +706,47 @@ __global__ __launch_bounds__(256) void attn_join(AttnArgs a) {
         if (64 * v + lane < D) out[64 * v + lane] = l != 0.0f ? acc[v] / l : 0.0f;
 }
 
-template <bool BF16, int D, int NR, int WK>
+template <class S>
 hipError_t go(AttnArgs a, int cus, uint8_t* ws, hipStream_t st) {
-    using S = Shape<BF16, D, NR, WK>;
-    static_assert(S::LDS <= 128 * 1024, "LDS");
-    static_assert((size_t)WK / 2 * NR * 16 * D * 4 <= S::LDS, "join");
-    a.grid = cus;
+    constexpr int PER_CU = (int)(160 * 1024 / (S::LDS + 4096)) >= 2 && S::WAVES <= 4 ? 2 : 1;
+    static_assert((size_t)PER_CU * S::PART <= MAX_PART, "workspace");
+    a.grid = PER_CU * cus;
     a.desc = (int*)ws;
-    a.part = (float*)(ws + (size_t)cus * DESC * 4);
-    const auto fn = attn_kernel<BF16, D, NR, WK>;
-    hipLaunchKernelGGL(fn, dim3(a.grid), dim3(64 * WK), S::LDS, st, a);
-    hipLaunchKernelGGL((attn_join<D, S::RT>), dim3(a.grid, S::RT / 4), dim3(256), 0, st, a);
+    a.part = (float*)(ws + (size_t)MAX_GRID * cus * DESC * 4);
+    hipLaunchKernelGGL(attn_kernel<S>, dim3(a.grid), dim3(64 * S::WAVES), S::LDS, st, a);
+    hipLaunchKernelGGL((attn_join<S::D, S::RT>), dim3(a.grid, S::RT / 4), dim3(256), 0, st, a);
     return hipGetLastError();
 }
 
-template <bool BF16, int D, int WK, int MAXNR>
+template <bool BF16, int D>
 hipError_t rows(const AttnArgs& a, int max_new, int cus, uint8_t* ws, hipStream_t st) {
     const int64_t r = (int64_t)max_new * a.G;
-    if (r <= 16) return go<BF16, D, 1, WK>(a, cus, ws, st);
-    if (r <= 32 || MAXNR == 2) return go<BF16, D, 2, WK>(a, cus, ws, st);
-    return go<BF16, D, MAXNR, WK>(a, cus, ws, st);
+    if constexpr (D == 256) {
+        if (r <= 16) return go<Shape<BF16, D, 1, 1, 2, 2>>(a, cus, ws, st);
+        return go<Shape<BF16, D, 1, 4, 1, 4>>(a, cus, ws, st);
+    } else {
+        constexpr int N = D == 64 ? 4 : 2;
+        if (r <= 16) return go<Shape<BF16, D, 1, 1, N, 2>>(a, cus, ws, st);
+        if (r <= 32) return go<Shape<BF16, D, 2, 1, N, 2>>(a, cus, ws, st);
+        if (r <= 64) return go<Shape<BF16, D, 2, 2, 2, 3>>(a, cus, ws, st);
+        return go<Shape<BF16, D, 2, 4, 2, 4>>(a, cus, ws, st);
+    }
 }
 
 template <bool BF16>
 hipError_t heads(const AttnArgs& a, int D, int max_new, int cus, uint8_t* ws, hipStream_t st) {
     switch (D) {
-        case 64: return rows<BF16, 64, 4, 4>(a, max_new, cus, ws, st);
-        case 96: return rows<BF16, 96, 4, 4>(a, max_new, cus, ws, st);
-        case 128: return rows<BF16, 128, 4, 4>(a, max_new, cus, ws, st);
-        default: return rows<BF16, 256, 2, 2>(a, max_new, cus, ws, st);
+        case 64: return rows<BF16, 64>(a, max_new, cus, ws, st);
+        case 96: return rows<BF16, 96>(a, max_new, cus, ws, st);
+        case 128: return rows<BF16, 128>(a, max_new, cus, ws, st);
+        default: return rows<BF16, 256>(a, max_new, cus, ws, st);
     }
 }
 
 }  // namespace
 
 size_t attn_part_bytes(int cus) {
-    return (size_t)cus * (DESC * 4 + 2 * sizeof(float) * 64 * (128 + 2));
+    return (size_t)cus * (MAX_GRID * DESC * 4 + 2 * sizeof(float) * MAX_PART);
 }
 
 hipError_t launch_attn(const AttnArgs& a, bool bf16, int D, int max_new, int cus, uint8_t* ws,

@@ -48,22 +48,27 @@ class TokenLogprobs(NamedTuple):
     top_tokens: Optional[torch.Tensor]    # int32 [M, top]
 
 
-def _need(ok: bool, what: str) -> None:
-    if not ok:
-        raise RuntimeError(what)
+def _refuse(what: str):
+    raise RuntimeError(what)
 
 
-def _ints(name: str, t: torch.Tensor, shape, like: torch.Tensor, dtype=torch.int32):
-    _need(t.dtype == dtype and t.is_contiguous() and t.device == like.device
-          and tuple(t.shape) == tuple(shape),
-          f"{name} must be a contiguous {dtype} tensor of shape {list(shape)} on {like.device}")
+# The checks below format a message only where they refuse: they are most of what a
+# call costs the host (17 -> 9 us a call with the messages made in advance).
+def _ints(name: str, t: torch.Tensor, shape, dev: int, dtype=torch.int32) -> int:
+    """t's address, if it is a contiguous tensor of that type and shape on GPU dev."""
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != dev or not t.is_contiguous():
+        _refuse(f"{name} must be a contiguous {dtype} tensor of shape {list(shape)} on cuda:{dev}")
     return t.data_ptr()
 
 
-def _table(name: str, t: torch.Tensor, rows: int, like: torch.Tensor) -> None:
-    _need(t.dim() == 2 and t.shape[0] == rows and t.shape[1] >= 1 and t.dtype == torch.int32
-          and t.device == like.device and t.stride(1) == 1 and t.stride(0) >= t.shape[1],
-          f"{name} must be an int32 block table of {rows} rows on {like.device}")
+def _table(name: str, t: torch.Tensor, rows: int, dev: int):
+    """A block table's address, columns and distance of rows."""
+    if t.dim() == 2 and t.dtype is torch.int32 and t.get_device() == dev:
+        n, cols = t.shape
+        stride, one = t.stride()
+        if n == rows and cols >= 1 and (one == 1 or cols == 1) and (stride >= cols or n == 1):
+            return t.data_ptr(), cols, max(stride, cols)
+    _refuse(f"{name} must be an int32 block table of {rows} rows on cuda:{dev}")
 
 
 def paged_cache(num_blocks: int, block_size: int, n_kv_heads: int, head_dim: int,
@@ -75,13 +80,17 @@ def paged_cache(num_blocks: int, block_size: int, n_kv_heads: int, head_dim: int
                              device=device).transpose(1, 2) for _ in range(2))
 
 
-def _cache(name: str, k: torch.Tensor, v: torch.Tensor, like: torch.Tensor):
-    _need(k.dim() == 4 and k.shape == v.shape and k.stride() == v.stride() and k.dtype == v.dtype
-          and k.device == like.device and v.device == like.device,
-          f"{name}: caches must be 4D [blocks, block size, kv heads, D], alike, on {like.device}")
-    _need(k.dtype in (torch.float16, torch.bfloat16), f"{name}: caches must be fp16 or bf16")
-    _need(k.stride(3) == 1, f"{name}: a cached head must be contiguous")
-    return _TYPES[k.dtype], k.data_ptr(), v.data_ptr(), k.shape[0], k.shape[1], *k.stride()[:3]
+def _cache(name: str, k: torch.Tensor, v: torch.Tensor, dev: int):
+    if (k.dim() != 4 or k.shape != v.shape or k.stride() != v.stride() or k.dtype is not v.dtype
+            or k.get_device() != dev or v.get_device() != dev):
+        _refuse(f"{name}: caches must be 4D [blocks, block size, kv heads, D], alike, on cuda:{dev}")
+    if k.dtype is not torch.float16 and k.dtype is not torch.bfloat16:
+        _refuse(f"{name}: caches must be fp16 or bf16")
+    nb, bs, hkv, D = k.shape
+    sb, st, sh, one = k.stride()
+    if one != 1 and D != 1:
+        _refuse(f"{name}: a cached head must be contiguous")
+    return _TYPES[k.dtype], k.data_ptr(), v.data_ptr(), nb, bs, sb, st, sh, hkv, D
 
 
 def plan_step(lengths: torch.Tensor, new_tokens: torch.Tensor, block_table: torch.Tensor,
@@ -96,23 +105,25 @@ def plan_step(lengths: torch.Tensor, new_tokens: torch.Tensor, block_table: torc
     (-1: the context), at most 64 tokens a request; None: chains.  Rows past the
     last request's are padding (slot -1).  The call repeats itself: given the
     same lengths and free blocks it enters the same blocks."""
-    _need(lengths.is_cuda and lengths.dim() == 1, "plan_step: lengths must be a 1D device tensor")
-    B = lengths.shape[0]
-    n = _ints("plan_step: lengths", lengths, (B,), lengths)
-    t = _ints("plan_step: new_tokens", new_tokens, (B,), lengths)
-    _table("plan_step: block_table", block_table, B, lengths)
-    f = _ints("plan_step: free_blocks", free_blocks, (free_blocks.numel(),), lengths)
-    p = None if parents is None else _ints("plan_step: parents", parents, (n_tokens,), lengths)
-    # one allocation: cu, info, slots, positions
-    out = lengths.new_empty((B + 3 + 2 * n_tokens,))
-    cu, info, slots, positions = out.split((B + 1, 2, n_tokens, n_tokens))
-    masks = None if parents is None else lengths.new_empty((n_tokens,), dtype=torch.int64)
+    if not lengths.is_cuda or lengths.dim() != 1:
+        _refuse("plan_step: lengths must be a 1D device tensor")
+    B, dev, N = lengths.shape[0], lengths.get_device(), n_tokens
+    n = _ints("plan_step: lengths", lengths, (B,), dev)
+    t = _ints("plan_step: new_tokens", new_tokens, (B,), dev)
+    table, cols, stride = _table("plan_step: block_table", block_table, B, dev)
+    n_free = free_blocks.numel()
+    f = _ints("plan_step: free_blocks", free_blocks, (n_free,), dev)
+    p = masks = m = None
+    if parents is not None:
+        p = _ints("plan_step: parents", parents, (N,), dev)
+        masks = torch.empty_like(parents, dtype=torch.int64)
+        m = masks.data_ptr()
+    out = lengths.new_empty((B + 3 + 2 * N,))  # one allocation
     at = out.data_ptr()
     _lib.check(_lib.lib().fq_plan_step(
-        n, t, p, B, n_tokens, block_size, block_table.data_ptr(), block_table.shape[1],
-        block_table.stride(0), f, free_blocks.numel(), at, at + 4 * (B + 3),
-        at + 4 * (B + 3 + n_tokens), None if masks is None else masks.data_ptr(), at + 4 * (B + 1),
-        _stream_ptr(lengths)), "plan_step")
+        n, t, p, B, N, block_size, table, cols, stride, f, n_free, at, at + 4 * (B + 3),
+        at + 4 * (B + 3 + N), m, at + 4 * (B + 1), _stream_ptr(lengths)), "plan_step")
+    cu, info, slots, positions = out.split_with_sizes((B + 1, 2, N, N))
     return StepPlan(cu, slots, positions, masks, info)
 
 
@@ -124,11 +135,11 @@ def rope_table(positions: int, rot: int, base: float = 10000.0, device="cuda") -
     return torch.cat([angle.cos(), angle.sin()], 1).float()
 
 
-def _vector(name: str, t: Optional[torch.Tensor], n: int, like: torch.Tensor):
+def _vector(name: str, t: Optional[torch.Tensor], n: int, dev: int):
     if t is None:
         return None
-    _need(t.dtype == torch.float32 and t.is_contiguous() and t.numel() == n
-          and t.device == like.device, f"{name} must be {n} contiguous fp32 values on {like.device}")
+    if t.dtype is not torch.float32 or t.numel() != n or t.get_device() != dev or not t.is_contiguous():
+        _refuse(f"{name} must be {n} contiguous fp32 values on cuda:{dev}")
     return t.data_ptr()
 
 
@@ -144,25 +155,27 @@ def qk_norm_rope(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor
     added to each row first; q_weight, k_weight: fp32 [D], the heads' RMS norms
     (none: not normalized); interleaved: pairs (2i, 2i + 1) instead of (i, i + rot / 2).
     Tokens whose slot is -1 leave the caches as they are."""
-    _need(qkv.dim() == 2 and qkv.is_cuda and qkv.dtype == torch.float32
-          and (qkv.stride(1) == 1 or qkv.shape[1] == 1),
-          "qk_norm_rope: qkv must be a 2D fp32 device tensor of contiguous rows")
-    type_, k, v, nb, bs, sb, st, sh = _cache("qk_norm_rope", k_cache, v_cache, qkv)
+    if (qkv.dim() != 2 or not qkv.is_cuda or qkv.dtype is not torch.float32
+            or (qkv.stride(1) != 1 and qkv.shape[1] != 1)):
+        _refuse("qk_norm_rope: qkv must be a 2D fp32 device tensor of contiguous rows")
+    dev = qkv.get_device()
+    type_, k, v, nb, bs, sb, st, sh, hkv, D = _cache("qk_norm_rope", k_cache, v_cache, dev)
     N, width = qkv.shape
-    hkv, D = k_cache.shape[2:]
-    hq = width // D - 2 * hkv
-    _need(width % D == 0 and hq >= 1 and hq % hkv == 0,
-          f"qk_norm_rope: rows of {width} do not hold heads of {D} for {hkv} kv heads")
-    _need(table.dim() == 2 and table.dtype == torch.float32 and table.is_contiguous()
-          and table.device == qkv.device, "qk_norm_rope: table must be a contiguous fp32 [positions, rot]")
+    hq = width // D - 2 * hkv if D else 0
+    if hq < 1 or width % D or hkv < 1 or hq % hkv:
+        _refuse(f"qk_norm_rope: rows of {width} do not hold heads of {D} for {hkv} kv heads")
+    if (table.dim() != 2 or table.dtype is not torch.float32 or not table.is_contiguous()
+            or table.get_device() != dev):
+        _refuse(f"qk_norm_rope: table must be a contiguous fp32 [positions, rot] on cuda:{dev}")
+    rows, rot = table.shape
     q = qkv.new_empty((N, hq, D))
     _lib.check(_lib.lib().fq_qk_norm_rope(
-        qkv.data_ptr(), qkv.stride(0) if N > 1 else width, N, hq, hkv, D, table.shape[1],
-        1 if interleaved else 0, _vector("qk_norm_rope: bias", bias, width, qkv),
-        _vector("qk_norm_rope: q_weight", q_weight, D, qkv),
-        _vector("qk_norm_rope: k_weight", k_weight, D, qkv), eps,
-        _ints("qk_norm_rope: positions", positions, (N,), qkv),
-        _ints("qk_norm_rope: slots", slots, (N,), qkv), table.data_ptr(), table.shape[0],
+        qkv.data_ptr(), qkv.stride(0) if N > 1 else width, N, hq, hkv, D, rot,
+        1 if interleaved else 0, _vector("qk_norm_rope: bias", bias, width, dev),
+        _vector("qk_norm_rope: q_weight", q_weight, D, dev),
+        _vector("qk_norm_rope: k_weight", k_weight, D, dev), eps,
+        _ints("qk_norm_rope: positions", positions, (N,), dev),
+        _ints("qk_norm_rope: slots", slots, (N,), dev), table.data_ptr(), rows,
         q.data_ptr(), type_, k, v, nb, bs, sb, st, sh, _stream_ptr(qkv)), "qk_norm_rope")
     return q
 
@@ -179,26 +192,26 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     caches already.  A token sees all of its request's cached tokens.  max_new:
     the most new tokens of one request where the caller knows it (speed only);
     scale: D^-0.5 unless given."""
-    _need(q.dim() == 3 and q.is_cuda and q.dtype == torch.float32,
-          "tree_attention: q must be a 3D fp32 device tensor")
+    if q.dim() != 3 or not q.is_cuda or q.dtype is not torch.float32:
+        _refuse("tree_attention: q must be a 3D fp32 device tensor")
     N, hq, D = q.shape
-    _need(q.stride(2) == 1 and (hq == 1 or q.stride(1) == D),
-          "tree_attention: a token's queries must be contiguous")
-    type_, k, v, nb, bs, sb, st, sh = _cache("tree_attention", k_cache, v_cache, q)
-    hkv = k_cache.shape[2]
-    _need(k_cache.shape[3] == D and hkv >= 1 and hq % hkv == 0,
-          f"tree_attention: {hq} heads of {D} do not share {hkv} kv heads of {k_cache.shape[3]}")
-    B = lengths.shape[0] if lengths.dim() == 1 else -1
-    n = _ints("tree_attention: lengths", lengths, (B,), q)
-    c = _ints("tree_attention: cu", cu, (B + 1,), q)
-    m = None if masks is None else _ints("tree_attention: masks", masks, (N,), q, torch.int64)
-    _table("tree_attention: block_table", block_table, B, q)
+    ldq, sq, one = q.stride()
+    if one != 1 or (hq != 1 and sq != D):
+        _refuse("tree_attention: a token's queries must be contiguous")
+    dev = q.get_device()
+    type_, k, v, nb, bs, sb, st, sh, hkv, Dk = _cache("tree_attention", k_cache, v_cache, dev)
+    if Dk != D or hkv < 1 or hq % hkv:
+        _refuse(f"tree_attention: {hq} heads of {D} do not share {hkv} kv heads of {Dk}")
+    B = lengths.numel()
+    n = _ints("tree_attention: lengths", lengths, (B,), dev)
+    c = _ints("tree_attention: cu", cu, (B + 1,), dev)
+    m = None if masks is None else _ints("tree_attention: masks", masks, (N,), dev, torch.int64)
+    table, cols, stride = _table("tree_attention: block_table", block_table, B, dev)
     out = q.new_empty((N, hq, D))
     _lib.check(_lib.lib().fq_tree_attention(
-        q.data_ptr(), q.stride(0) if N > 1 else hq * D, n, c, m, B, N,
-        N if max_new is None else max_new, hq, hkv, D, D ** -0.5 if scale is None else scale,
-        type_, k, v, nb, bs, sb, st, sh, block_table.data_ptr(), block_table.shape[1],
-        block_table.stride(0), out.data_ptr(), _stream_ptr(q)), "tree_attention")
+        q.data_ptr(), ldq if N > 1 else hq * D, n, c, m, B, N, N if max_new is None else max_new, hq,
+        hkv, D, D ** -0.5 if scale is None else scale, type_, k, v, nb, bs, sb, st, sh, table, cols,
+        stride, out.data_ptr(), _stream_ptr(q)), "tree_attention")
     return out
 
 
@@ -207,26 +220,28 @@ def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None,
     """Log probabilities of targets (int32 [M] or [M, J]) under softmax(logits) (fp32,
     fp16 or bf16 [M, V], rows any distance apart), each row's entropy, and its top
     largest logits (at most 64; ties: the lowest token) with their log probabilities."""
-    _need(logits.dim() == 2 and logits.is_cuda and logits.dtype in _TYPES
-          and (logits.stride(1) == 1 or logits.shape[1] == 1),
-          "token_logprobs: logits must be a 2D fp32, fp16 or bf16 device tensor of contiguous rows")
+    if (logits.dim() != 2 or not logits.is_cuda or logits.dtype not in _TYPES
+            or (logits.stride(1) != 1 and logits.shape[1] != 1)):
+        _refuse("token_logprobs: logits must be a 2D fp32, fp16 or bf16 device tensor of contiguous rows")
     M, V = logits.shape
-    t, J, lp, tl, tt = None, 0, None, None, None
+    J, t, lp, l, tl, tt, a, b = 0, None, None, None, None, None, None, None
     if targets is not None:
-        _need(targets.dim() in (1, 2), "token_logprobs: targets must be [M] or [M, J]")
+        if targets.dim() not in (1, 2):
+            _refuse("token_logprobs: targets must be [M] or [M, J]")
         J = 1 if targets.dim() == 1 else targets.shape[1]
-        t = _ints("token_logprobs: targets", targets, (M,) if targets.dim() == 1 else (M, J), logits)
-        lp = logits.new_empty(targets.shape, dtype=torch.float32)
+        t = _ints("token_logprobs: targets", targets, (M, J)[:targets.dim()], logits.get_device())
+        lp = torch.empty_like(targets, dtype=torch.float32)
+        l = lp.data_ptr()
     entropy = logits.new_empty((M,), dtype=torch.float32)
     if top:
-        _need(0 < top <= min(64, V), f"token_logprobs: top must be at most {min(64, V)}")
+        if not 0 < top <= min(64, V):
+            _refuse(f"token_logprobs: top must be at most {min(64, V)}")
         tl = logits.new_empty((M, top), dtype=torch.float32)
         tt = logits.new_empty((M, top), dtype=torch.int32)
+        a, b = tl.data_ptr(), tt.data_ptr()
     _lib.check(_lib.lib().fq_token_logprobs(
-        logits.data_ptr(), _TYPES[logits.dtype], logits.stride(0) if M > 1 else V, M, V, t, J, top,
-        None if lp is None else lp.data_ptr(), entropy.data_ptr(),
-        None if tl is None else tl.data_ptr(), None if tt is None else tt.data_ptr(),
-        _stream_ptr(logits)), "token_logprobs")
+        logits.data_ptr(), _TYPES[logits.dtype], logits.stride(0) if M > 1 else V, M, V, t, J, top, l,
+        entropy.data_ptr(), a, b, _stream_ptr(logits)), "token_logprobs")
     return TokenLogprobs(lp, entropy, tl, tt)
 
 
