@@ -60,6 +60,10 @@ __device__ __forceinline__ int sload(const int* p) {
 }
 __device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
+// All waves' LDS accesses are done (their stores to memory may be on their way).
+__device__ __forceinline__ void lds_barrier() {
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
 __device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
 template <bool BF16>
@@ -103,9 +107,9 @@ struct Request {
     int t0, nt, len;  // its first new token, how many, its cached tokens
     int keys, nu;     // keys and units of them
     int rts;          // tiles of RT rows
-    int64_t units;
+    int64_t units;    // of all its items, OV more for each
 };
-template <int RT, int KU>
+template <int RT, int KU, int OV>
 __device__ __forceinline__ Request request(const AttnArgs& a, int c0, int c1, int len) {
     Request r;
     r.t0 = min(max(c0, 0), a.N);
@@ -116,7 +120,7 @@ __device__ __forceinline__ Request request(const AttnArgs& a, int c0, int c1, in
     r.keys = (int)min((int64_t)r.len + r.nt, min(most, (int64_t)INT32_MAX - 4096));
     r.nu = (r.keys + KU - 1) / KU;
     r.rts = (int)(((int64_t)r.nt * a.G + RT - 1) / RT);
-    r.units = (int64_t)a.hkv * r.rts * r.nu;
+    r.units = r.nu ? (int64_t)a.hkv * r.rts * (r.nu + OV) : 0;
     return r;
 }
 
@@ -151,6 +155,9 @@ __device__ __forceinline__ uint32_t shifted(uint64_t m, int n) {
     return n >= 32 || n <= -64 ? 0u : n >= 0 ? (uint32_t)m << n : (uint32_t)(m >> -n);
 }
 
+#ifndef OVERHEAD
+#define OVERHEAD 4
+#endif
 // WR x WK waves: each group of WR shares tiles of 32 keys, each of its waves
 // with 16 NR rows of its own; the groups take every WK-th tile.  NS tiles of a
 // group are in LDS.
@@ -180,6 +187,9 @@ struct Shape {
     static constexpr int GROUP = NS * STAGE;
     static constexpr size_t LDS = (size_t)WK * GROUP;
     static constexpr int PART = RT * (D + 2);    // floats of a partial result
+    // What an item costs beside its units, in units: finding its blocks, its
+    // queries, the first tiles' way, joining the groups and storing.
+    static constexpr int OV = OVERHEAD;
     static_assert(2 * NI % WR == 0 && (WR == 1 ? NS == 2 : true), "copies");
     // the waves' outputs are exchanged where the tiles were
     static_assert((size_t)WAVES * NR * 16 * D * 4 <= LDS, "join");
@@ -196,6 +206,7 @@ __global__ __launch_bounds__(64 * S::WAVES, 1) void attn_kernel(AttnArgs a) {
     constexpr int D = S::D, NR = S::NR, WR = S::WR, WK = S::WK, NS = S::NS;
     constexpr int NL = Parts<BF16>::N;
     constexpr int RT = S::RT, KU = S::KU, PITCH = S::PITCH, J = S::J, NI = S::NI, ROWS = S::ROWS;
+    constexpr int OV = S::OV;
     constexpr int STEPS = D / 32, DT = D / 16, SLOTS = S::DP / 8;
     constexpr uint32_t EXP = BF16 ? 0x7F80u : 0x7C00u;  // the exponent of what is not finite
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
@@ -213,7 +224,7 @@ __global__ __launch_bounds__(64 * S::WAVES, 1) void attn_kernel(AttnArgs a) {
         const int per = (a.B + 63) / 64, first = lane * per;
         int64_t mine = 0;
         for (int i = first; i < min(first + per, a.B); ++i)
-            mine += request<RT, KU>(a, a.cu[i], a.cu[i + 1], a.lengths[i]).units;
+            mine += request<RT, KU, OV>(a, a.cu[i], a.cu[i + 1], a.lengths[i]).units;
         int64_t upto = mine;
         for (int o = 1; o < 64; o <<= 1) {
             const int64_t v = __shfl_up(upto, o);
@@ -245,7 +256,7 @@ __global__ __launch_bounds__(64 * S::WAVES, 1) void attn_kernel(AttnArgs a) {
     bool cut = false;  // an item begun here goes on in the next work-group
 
     if (tid < WK) s_odd[tid] = 0;
-    __syncthreads();
+    lds_barrier();
 
     // --- constants of a lane ---
     const uint32_t gbase = lds_addr(lds) + wk * S::GROUP;
@@ -271,60 +282,28 @@ __global__ __launch_bounds__(64 * S::WAVES, 1) void attn_kernel(AttnArgs a) {
     }
 
     for (; left > 0; ++b) {
-        const Request rq = request<RT, KU>(a, sload(a.cu + b), sload(a.cu + b + 1), sload(a.lengths + b));
+        const Request rq = request<RT, KU, OV>(a, sload(a.cu + b), sload(a.cu + b + 1), sload(a.lengths + b));
         const int len = rq.len, keys = rq.keys, nu = rq.nu, t0 = rq.t0, nt = rq.nt;
+        if (off >= rq.units) {
+            off -= rq.units;
+            continue;
+        }
+        int item = 0, pos = 0;
+        if (off) {
+            item = (int)(off / (nu + OV));
+            pos = (int)(off % (nu + OV));
+        }
         while (off < rq.units && left > 0) {
-            const int item = (int)(off / nu), first = (int)(off % nu);
+            const int take = (int)min((int64_t)(nu + OV - pos), left);
+            const int first = max(pos - OV, 0), count = max(pos + take - OV, 0) - first;
+            const int64_t start = u - pos;  // the item's
+            u += take;
+            off += take;
+            left -= take;
+            pos = 0;
+            if (count == 0) break;  // (the item's work begins in the next work-group)
             const int h = item / rq.rts, rt = item % rq.rts;
-            const int count = (int)min((int64_t)(nu - first), left);
-
-            // --- queries ---
-            u4 qf[NR][STEPS][NL];
-            float rs[NR];
-            uint64_t mask[NR];
-#pragma unroll
-            for (int c = 0; c < NR; ++c) {
-                const int r = rt * RT + wr * 16 * NR + 16 * c + n16;
-                const int t = r / a.G, hh = h * a.G + r % a.G;
-                const bool on = t < nt;
-                // (a chain: how many of the new tokens the row sees)
-                mask[c] = !on ? 0 : a.masks ? a.masks[t0 + t] : (uint64_t)t + 1;
-                const float* q = a.q + (int64_t)(t0 + (on ? t : 0)) * a.ldq + (int64_t)(on ? hh : 0) * D;
-                f4 x[STEPS][2];
-                float mx = 0.0f;
-#pragma unroll
-                for (int s = 0; s < STEPS; ++s)
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        x[s][i] = on ? *(const f4u*)(q + 32 * s + 8 * g + 4 * i) : f4{0, 0, 0, 0};
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) mx = fmaxf(mx, fabsf(x[s][i][e]));
-                    }
-                float up = 1.0f, down = 1.0f;
-                if (!BF16) {  // the row's largest to [2^14, 2^15)
-                    mx = max4(mx);
-                    if (mx > 0.0f && mx < __builtin_inff()) {
-                        const int e = min(max(15 - __builtin_amdgcn_frexp_expf(mx), -126), 126);
-                        up = ldexpf(1.0f, e);
-                        down = ldexpf(1.0f, -e);
-                    }
-                }
-                // (the scale's sign goes with the query: the largest score is
-                // that of the largest product)
-                up = copysignf(up, a.scale);
-                rs[c] = down * fabsf(a.scale);
-#pragma unroll
-                for (int s = 0; s < STEPS; ++s)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        uint32_t p[NL];
-                        split2<BF16>(x[s][i >> 1][2 * (i & 1)] * up,
-                                     x[s][i >> 1][2 * (i & 1) + 1] * up, p);
-#pragma unroll
-                        for (int l = 0; l < NL; ++l) qf[c][s][l][i] = p[l];
-                    }
-            }
-
+            ++item;
             // --- this group's tiles: wk, wk + WK, .. of the segment's.  Waves that
             // share tiles keep step: as many tiles for each group (those past
             // the last key are masked) ---
@@ -380,18 +359,64 @@ __global__ __launch_bounds__(64 * S::WAVES, 1) void attn_kernel(AttnArgs a) {
 
             f4 o[DT][NR];
             float mrow[NR], lrow[NR];
+            u4 qf[NR][STEPS][NL];
+            float rs[NR];
+            uint64_t mask[NR];
             bool careful = false;
         again:
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             if constexpr (WR == 1) {
                 if (n > 0) copy_k(0), copy_v(0);
                 if (n > 1) copy_k(1), copy_v(1);
             } else {
-                __syncthreads();  // (again: the others may still read)
+                if (careful) lds_barrier();  // (the others may still read)
 #pragma unroll
                 for (int i = 0; i < NS - 1; ++i)
                     if (i < n) copy_all(i, i);
             }
+            // --- queries (on their way while the first tiles are) ---
+#pragma unroll
+            for (int c = 0; c < NR; ++c) {
+                const int r = rt * RT + wr * 16 * NR + 16 * c + n16;
+                const int t = r / a.G, hh = h * a.G + r % a.G;
+                const bool on = t < nt;
+                // (a chain: how many of the new tokens the row sees)
+                mask[c] = !on ? 0 : a.masks ? a.masks[t0 + t] : (uint64_t)t + 1;
+                const float* q = a.q + (int64_t)(t0 + (on ? t : 0)) * a.ldq + (int64_t)(on ? hh : 0) * D;
+                f4 x[STEPS][2];
+                float mx = 0.0f;
+#pragma unroll
+                for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        x[s][i] = on ? *(const f4u*)(q + 32 * s + 8 * g + 4 * i) : f4{0, 0, 0, 0};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) mx = fmaxf(mx, fabsf(x[s][i][e]));
+                    }
+                float up = 1.0f, down = 1.0f;
+                if (!BF16) {  // the row's largest to [2^14, 2^15)
+                    mx = max4(mx);
+                    if (mx > 0.0f && mx < __builtin_inff()) {
+                        const int e = min(max(15 - __builtin_amdgcn_frexp_expf(mx), -126), 126);
+                        up = ldexpf(1.0f, e);
+                        down = ldexpf(1.0f, -e);
+                    }
+                }
+                // (the scale's sign goes with the query: the largest score is
+                // that of the largest product)
+                up = copysignf(up, a.scale);
+                rs[c] = down * fabsf(a.scale);
+#pragma unroll
+                for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        uint32_t p[NL];
+                        split2<BF16>(x[s][i >> 1][2 * (i & 1)] * up,
+                                     x[s][i >> 1][2 * (i & 1) + 1] * up, p);
+#pragma unroll
+                        for (int l = 0; l < NL; ++l) qf[c][s][l][i] = p[l];
+                    }
+            }
+
 #pragma unroll
             for (int c = 0; c < NR; ++c) {
                 mrow[c] = LOWEST;
@@ -411,7 +436,7 @@ __global__ __launch_bounds__(64 * S::WAVES, 1) void attn_kernel(AttnArgs a) {
                     // and all are done with the tile before, whose place is filled anew
                     if (i + NS - 2 < n) wait_vm<(NS - 2) * S::CW>();
                     else wait_vm<0>();
-                    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                    lds_barrier();
                     if (i + NS - 1 < n) copy_all(i + NS - 1, stage ? stage - 1 : NS - 1);
                 }
                 // scores
@@ -568,7 +593,7 @@ __global__ __launch_bounds__(64 * S::WAVES, 1) void attn_kernel(AttnArgs a) {
                     s_ml[1][wk][16 * (wr * NR + c) + ln % 16] = lrow[c];
                 }
             }
-            __syncthreads();
+            lds_barrier();
             if (s_odd[wk]) {
                 // what was taken out, back into the rows that see it
 #pragma unroll 1
@@ -616,7 +641,7 @@ __global__ __launch_bounds__(64 * S::WAVES, 1) void attn_kernel(AttnArgs a) {
                     if (WK > 1) *(f4*)(buf + (((wave * NR + c) * DT + d) * 64 + ln) * 4) = o[d][c];
                 }
             }
-            __syncthreads();
+            lds_barrier();
             if (tid < WK) s_odd[tid] = 0;
             const bool whole = count == nu;
             float* part = a.part + (int64_t)(2 * wg + (first == 0)) * S::PART;
@@ -649,61 +674,114 @@ __global__ __launch_bounds__(64 * S::WAVES, 1) void attn_kernel(AttnArgs a) {
             if (first == 0 && !whole) {
                 cut = true;
                 if (tid == 0) {
-                    const int64_t end = u + nu - 1;  // the item's last unit
+                    const int64_t end = start + OV + nu - 1;  // the item's last unit
                     desc[0] = (int)(end / span) - wg + 1;
                     desc[1] = t0, desc[2] = nt, desc[3] = h, desc[4] = rt;
                 }
             }
-            u += count;
-            off += count;
-            left -= count;
-            __syncthreads();  // the exchanged outputs are read
+            lds_barrier();  // the exchanged outputs are read
         }
         off -= rq.units;
     }
     if (!cut && tid == 0) desc[0] = 0;
 }
 
-// The rows of an item whose parts lie in work-groups w .. w + parts - 1: one wave
-// to a row.
+// Joins the parts of the items that are cut: one row after the other, by one wave
+// or, where an item has many parts, by the four waves of a work-group.
+constexpr int JOIN_GRID = 1024;
+
 template <int D, int RT>
 __global__ __launch_bounds__(256) void attn_join(AttnArgs a) {
-    constexpr int PART = RT * (D + 2);
-    const int w = blockIdx.x, lane = threadIdx.x & 63;
-    const int* desc = a.desc + w * DESC;
-    const int parts = sload(desc);
-    if (parts == 0) return;
-    const int rl = blockIdx.y * 4 + uni(threadIdx.x >> 6);
-    const int t0 = sload(desc + 1), nt = sload(desc + 2), h = sload(desc + 3), rt = sload(desc + 4);
-    const int r = rt * RT + rl, t = r / a.G;
-    if (t >= nt) return;
-    const auto slot = [&](int p) { return a.part + (int64_t)(2 * (w + p) + (p == 0)) * PART; };
-    float m = LOWEST;
-    for (int p = lane; p < parts; p += 64) m = fmaxf(m, slot(p)[RT * D + rl]);
-    for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-    constexpr int V = (D + 63) / 64;
-    float acc[V] = {}, l = 0.0f;
-    for (int p0 = 0; p0 < parts; p0 += 64) {
-        float f = 0.0f, lp = 0.0f;
-        if (p0 + lane < parts) {
-            const float* s = slot(p0 + lane) + RT * D + rl;
-            f = __builtin_amdgcn_exp2f(s[0] - m);
-            lp = s[RT];
-        }
-        const int np = min(64, parts - p0);
-        for (int p = 0; p < np; ++p) {
-            const float fp = __shfl(f, p);
-            l += fp * __shfl(lp, p);
-            const float* s = slot(p0 + p) + rl * D;
-            #pragma unroll
-            for (int v = 0; v < V; ++v)
-                if (64 * v + lane < D) acc[v] += fp * s[64 * v + lane];
-        }
+    constexpr int PART = RT * (D + 2), E = D == 64 ? 1 : D == 256 ? 4 : 2;
+    typedef float fe __attribute__((ext_vector_type(E)));
+    __shared__ int s_list[512], s_count[8], s_most[4];
+    __shared__ float s_acc[4][D + 1];
+    const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6);
+    // the work-groups that began such an item, in their order (a.grid <= 512)
+    int parts2[2], most = 0;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const int i = k * 256 + tid;
+        parts2[k] = i < a.grid ? a.desc[i * DESC] : 0;
+        most = max(most, parts2[k]);
+        const uint64_t some = __ballot(parts2[k] > 0);
+        if (lane == 0) s_count[4 * k + wave] = __popcll(some);
     }
-    float* out = a.out + ((int64_t)(t0 + t) * a.hq + h * a.G + r % a.G) * D;
-    #pragma unroll
-    for (int v = 0; v < V; ++v)
-        if (64 * v + lane < D) out[64 * v + lane] = l != 0.0f ? acc[v] / l : 0.0f;
+    for (int o = 32; o; o >>= 1) most = max(most, __shfl_xor(most, o));
+    if (lane == 0) s_most[wave] = most;
+    __syncthreads();
+    int items = 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        const uint64_t some = __ballot(parts2[k >> 2] > 0);
+        if ((k & 3) == wave && parts2[k >> 2] > 0)
+            s_list[items + __popcll(some & ((1ull << lane) - 1))] = (k >> 2) * 256 + tid;
+        items += s_count[k];
+    }
+    most = max(max(s_most[0], s_most[1]), max(s_most[2], s_most[3]));
+    __syncthreads();
+    const bool wide = most > 8;
+    const int per = wide ? RT : RT / 4, jobs = items * per;
+    for (int job = blockIdx.x; job < jobs; job += gridDim.x) {
+        const int w = uni(s_list[job / per]);
+        const int rl = wide ? job % per : job % per * 4 + wave;
+        const int* desc = a.desc + w * DESC;
+        const int parts = sload(desc), t0 = sload(desc + 1), nt = sload(desc + 2);
+        const int h = sload(desc + 3), rt = sload(desc + 4);
+        const int r = rt * RT + rl, t = r / a.G;
+        if (t >= nt) continue;
+        const auto slot = [&](int p) { return a.part + (int64_t)(2 * (w + p) + (p == 0)) * PART; };
+        float m = LOWEST;
+        for (int p = lane; p < parts; p += 64) m = fmaxf(m, slot(p)[RT * D + rl]);
+        for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+        const int share = wide ? (parts + 3) / 4 : parts;
+        const int beg = wide ? wave * share : 0, end = min(parts, beg + share);
+        fe acc = 0.0f;
+        float l = 0.0f;
+        for (int p0 = beg; p0 < end; p0 += 64) {
+            float f = 0.0f, lp = 0.0f;
+            if (p0 + lane < end) {
+                const float* s = slot(p0 + lane) + RT * D + rl;
+                f = __builtin_amdgcn_exp2f(s[0] - m);
+                lp = s[RT] * f;
+            }
+            for (int o = 32; o; o >>= 1) lp += __shfl_xor(lp, o);
+            l += lp;
+            for (int p = p0; p < min(end, p0 + 64); p += 8) {
+                fe x[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    x[i] = 0.0f;
+                    if (p + i < end && E * lane < D) x[i] = *(const fe*)(slot(p + i) + rl * D + E * lane);
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float fp = __uint_as_float(
+                        __builtin_amdgcn_readlane(__float_as_uint(f), (p + i - p0) & 63));
+                    if (p + i < end) acc += fp * x[i];
+                }
+            }
+        }
+        if (wide) {
+            if (E * lane < D)
+                for (int e = 0; e < E; ++e) s_acc[wave][E * lane + e] = acc[e];
+            if (lane == 0) s_acc[wave][D] = l;
+            __syncthreads();
+            acc = 0.0f;
+            l = 0.0f;
+            for (int i = 0; i < 4; ++i) {
+                l += s_acc[i][D];
+                if (E * lane < D)
+                    for (int e = 0; e < E; ++e) acc[e] += s_acc[i][E * lane + e];
+            }
+            __syncthreads();
+            if (wave) continue;
+        }
+        fe v = 0.0f;
+        if (l != 0.0f) v = acc * (1.0f / l);
+        if (E * lane < D)
+            *(fe*)(a.out + ((int64_t)(t0 + t) * a.hq + h * a.G + r % a.G) * D + E * lane) = v;
+    }
 }
 
 template <class S>
@@ -714,7 +792,7 @@ hipError_t go(AttnArgs a, int cus, uint8_t* ws, hipStream_t st) {
     a.desc = (int*)ws;
     a.part = (float*)(ws + (size_t)MAX_GRID * cus * DESC * 4);
     hipLaunchKernelGGL(attn_kernel<S>, dim3(a.grid), dim3(64 * S::WAVES), S::LDS, st, a);
-    hipLaunchKernelGGL((attn_join<S::D, S::RT>), dim3(a.grid, S::RT / 4), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((attn_join<S::D, S::RT>), dim3(JOIN_GRID), dim3(256), 0, st, a);
     return hipGetLastError();
 }
 
