@@ -22,7 +22,7 @@
 // Queries are fp32 and keep their bits: against fp16 keys a query is hi + lo
 // in fp16 (22 bits, its row scaled by a power of two), against bf16 keys three
 // bf16 parts (24 bits).  The probabilities take the same two or three parts,
-// in fp16 scaled by 2^14 (so that parts down to 2^-38 of the row's largest
+// in fp16 scaled by 2^11 (so that parts down to 2^-35 of the row's largest
 // count); statistics and sums are fp32.
 //
 // Rows and keys outside the lengths cost no branch in the common tile: only
@@ -52,6 +52,9 @@ typedef __attribute__((address_space(3))) float lds_f;
 
 constexpr float LOWEST = -3.402823466e38f;
 constexpr int KT = 32;  // keys of a wave's tile
+// By how much (log2) a row's largest score may be above its sums' reference, and what
+// fp16 probabilities are raised by: together they stay below fp16's largest.
+constexpr float LAG = 4.0f, UP = 11.0f;
 
 // A uniform value in a scalar register, read through the scalar cache (memory
 // that no kernel writes while this one runs).
@@ -59,6 +62,19 @@ __device__ __forceinline__ int sload(const int* p) {
     return *(const __attribute__((address_space(4))) int*)(uintptr_t)p;
 }
 __device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// Memory straight into LDS: 16 bytes a lane, from base + off to lds + 16 lane (lds
+// in M0).  The base passes through a scalar move within the block, and four states
+// follow: a vector instruction (a spilled scalar register comes back by one)
+// may have written base or M0 just before, and a load must not read such a
+// register within five states, which the compiler sees to for its own loads only.
+__device__ __forceinline__ void copy16(uint32_t off, const uint8_t* base, uint32_t lds) {
+    uint64_t at;
+    asm volatile("s_mov_b64 %0, %2\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, %0"
+                 : "=&s"(at)
+                 : "v"(off), "s"(base), "{m0}"(lds)
+                 : "memory");
+}
 
 // All waves' LDS accesses are done (their stores to memory may be on their way).
 __device__ __forceinline__ void lds_barrier() {
@@ -155,9 +171,6 @@ __device__ __forceinline__ uint32_t shifted(uint64_t m, int n) {
     return n >= 32 || n <= -64 ? 0u : n >= 0 ? (uint32_t)m << n : (uint32_t)(m >> -n);
 }
 
-#ifndef OVERHEAD
-#define OVERHEAD 4
-#endif
 // WR x WK waves: each group of WR shares tiles of 32 keys, each of its waves
 // with 16 NR rows of its own; the groups take every WK-th tile.  NS tiles of a
 // group are in LDS.
@@ -189,8 +202,8 @@ struct Shape {
     static constexpr int PART = RT * (D + 2);    // floats of a partial result
     // What an item costs beside its units, in units: finding its blocks, its
     // queries, the first tiles' way, joining the groups and storing.
-    static constexpr int OV = OVERHEAD;
-    static_assert(2 * NI % WR == 0 && (WR == 1 ? NS == 2 : true), "copies");
+    static constexpr int OV = 256 / KU;
+    static_assert(2 * NI % WR == 0 && (WR == 1 ? NS == 2 : NS >= 3), "copies");
     // the waves' outputs are exchanged where the tiles were
     static_assert((size_t)WAVES * NR * 16 * D * 4 <= LDS, "join");
     static_assert(D / 16 % WK == 0, "join");
@@ -321,39 +334,55 @@ __global__ __launch_bounds__(64 * S::WAVES, 1) void attn_kernel(AttnArgs a) {
                                            : low_bits(old + (int)(uint32_t)m);
                 return s & low_bits(all);
             };
-            const auto offset = [&](int i, int hf) {  // of 16 keys, in their cache
-                const int key = min(kbeg + i * KU + 16 * hf, last16);
-                const int page = min(max(sload(table + (key >> a.c.bs_log2)), 0), a.c.num_blocks - 1);
-                return 2 * (page * a.c.sb + (key & ((1 << a.c.bs_log2) - 1)) * a.c.st);
+            // A tile's pages, read ahead; the places of its 16s of keys in a cache;
+            // its copies.  (Past the last key: its page again.)
+            const auto key_of = [&](int i, int hf) { return min(kbeg + i * KU + 16 * hf, last16); };
+            int page[2];
+            const auto read_pages = [&](int i) {
+#pragma unroll
+                for (int hf = 0; hf < 2; ++hf) page[hf] = sload(table + (key_of(i, hf) >> a.c.bs_log2));
             };
-            int64_t pre[2];  // of the tile whose values are copied next (WR == 1)
-            const auto copy_k = [&](int i) {
+            int64_t at_k[2], at_v[2];  // of the tiles whose keys, values are copied next
+            const auto place = [&](int i) {
 #pragma unroll
                 for (int hf = 0; hf < 2; ++hf) {
-                    pre[hf] = offset(i, hf);
-#pragma unroll
-                    for (int j = 0; j < J; ++j)
-                        dma16s(ksrc, kb + pre[hf] + 2 * j * ROWS * a.c.st,
-                               gbase + (i & 1) * S::STAGE + (hf * J + j) * S::KSTEP);
+                    const int pg = min(max(page[hf], 0), a.c.num_blocks - 1);
+                    at_v[hf] = at_k[hf];
+                    at_k[hf] = 2 * (pg * a.c.sb + (key_of(i, hf) & ((1 << a.c.bs_log2) - 1)) * a.c.st);
                 }
             };
-            const auto copy_v = [&](int i) {
+            const int64_t step = 2 * ROWS * a.c.st;  // bytes from copy to copy
+            const auto copy_k = [&](int stage) {
 #pragma unroll
-                for (int hf = 0; hf < 2; ++hf)
+                for (int hf = 0; hf < 2; ++hf) {
+                    const uint8_t* from = kb + at_k[hf];
 #pragma unroll
-                    for (int j = 0; j < J; ++j)
-                        dma16s(vsrc, vb + pre[hf] + 2 * j * ROWS * a.c.st,
-                               gbase + (i & 1) * S::STAGE + S::KTILE + (hf * J + j) * S::VSTEP);
+                    for (int j = 0; j < J; ++j, from += step)
+                        copy16(ksrc, from, gbase + stage * S::STAGE + (hf * J + j) * S::KSTEP);
+                }
             };
-            const auto copy_all = [&](int i, int stage) {
-                const int64_t o0 = offset(i, 0), o1 = offset(i, 1);
-                const uint32_t to = gbase + stage * S::STAGE;
+            const auto copy_v = [&](int stage) {
+#pragma unroll
+                for (int hf = 0; hf < 2; ++hf) {
+                    const uint8_t* from = vb + at_v[hf];
+#pragma unroll
+                    for (int j = 0; j < J; ++j, from += step)
+                        copy16(vsrc, from, gbase + stage * S::STAGE + S::KTILE + (hf * J + j) * S::VSTEP);
+                }
+            };
+            // this wave's share of a tile's keys and of the one before's values
+            const auto copy_share = [&](bool ks, int kstage, bool vs, int vstage) {
 #pragma unroll
                 for (int x = 0; x < S::CW; ++x) {
                     const int ci = wr + WR * x, c = ci % NI;
-                    const int64_t from = (c >= J ? o1 : o0) + 2 * (c % J) * ROWS * a.c.st;
-                    if (ci < NI) dma16s(ksrc, kb + from, to + c * S::KSTEP);
-                    else dma16s(vsrc, vb + from, to + S::KTILE + c * S::VSTEP);
+                    const int64_t in = (c % J) * step;
+                    if (ci < NI) {
+                        if (ks) copy16(ksrc, kb + (c >= J ? at_k[1] : at_k[0]) + in,
+                                       gbase + kstage * S::STAGE + c * S::KSTEP);
+                    } else if (vs) {
+                        copy16(vsrc, vb + (c >= J ? at_v[1] : at_v[0]) + in,
+                               gbase + vstage * S::STAGE + S::KTILE + c * S::VSTEP);
+                    }
                 }
             };
 
@@ -364,14 +393,30 @@ __global__ __launch_bounds__(64 * S::WAVES, 1) void attn_kernel(AttnArgs a) {
             uint64_t mask[NR];
             bool careful = false;
         again:
+            at_k[0] = at_k[1] = 0;
             if constexpr (WR == 1) {
-                if (n > 0) copy_k(0), copy_v(0);
-                if (n > 1) copy_k(1), copy_v(1);
+                // K0 V0 K1 V1; then K2 once K0 is used, V2 once V0 is, ..
+                read_pages(0);
+                place(0);
+                read_pages(1);
+                if (n > 0) copy_k(0);
+                place(1);
+                read_pages(2);
+                if (n > 0) copy_v(0);
+                if (n > 1) copy_k(1);
+                at_v[0] = at_k[0], at_v[1] = at_k[1];
+                if (n > 1) copy_v(1);
             } else {
+                // K0, K1 V0, K2 V1, ..: each step's batch has the keys of one tile and
+                // the values of the one before
                 if (careful) lds_barrier();  // (the others may still read)
+                read_pages(0);
 #pragma unroll
-                for (int i = 0; i < NS - 1; ++i)
-                    if (i < n) copy_all(i, i);
+                for (int i = 0; i < NS; ++i) {
+                    place(i);
+                    read_pages(i + 1);
+                    copy_share(i < n, i, i > 0 && i <= n, i - 1);
+                }
             }
             // --- queries (on their way while the first tiles are) ---
 #pragma unroll
@@ -424,43 +469,68 @@ __global__ __launch_bounds__(64 * S::WAVES, 1) void attn_kernel(AttnArgs a) {
 #pragma unroll
                 for (int d = 0; d < DT; ++d) o[d][c] = f4{0, 0, 0, 0};
             }
-            int stage = 0;
-            for (int i = 0; i < n; ++i) {
-                const int key0 = kbeg + i * KU;
-                const uint32_t sat = stage * S::STAGE;
-                if constexpr (WR == 1) {
-                    if (i + 1 < n) wait_vm<3 * NI>();
-                    else wait_vm<NI>();
-                } else {
-                    // this tile's copies of this wave have landed, then everyone's;
-                    // and all are done with the tile before, whose place is filled anew
-                    if (i + NS - 2 < n) wait_vm<(NS - 2) * S::CW>();
-                    else wait_vm<0>();
-                    lds_barrier();
-                    if (i + NS - 1 < n) copy_all(i + NS - 1, stage ? stage - 1 : NS - 1);
-                }
-                // scores
-                f4 sc[2][NR];
+            // products of the keys at `at` (limbs of one sum apart, so that no
+            // product waits for the one before)
+            const auto products = [&](uint32_t at, f4 (&sc)[2][NR]) {
 #pragma unroll
-                for (int sub = 0; sub < 2; ++sub) {
+                for (int sub = 0; sub < 2; ++sub)
 #pragma unroll
                     for (int c = 0; c < NR; ++c) sc[sub][c] = f4{0, 0, 0, 0};
 #pragma unroll
-                    for (int s = 0; s < STEPS; ++s) {
-                        const u4 kf = *(lds_u4*)(uintptr_t)(klane + sat + J * sub * S::KSTEP + 64 * s);
+                for (int s = 0; s < STEPS; ++s) {
+                    u4 kf[2];
 #pragma unroll
-                        for (int c = 0; c < NR; ++c)
+                    for (int sub = 0; sub < 2; ++sub)
+                        kf[sub] = *(lds_u4*)(uintptr_t)(klane + at + J * sub * S::KSTEP + 64 * s);
 #pragma unroll
-                            for (int l = NL - 1; l >= 0; --l)
-                                sc[sub][c] = mfma<BF16>(kf, qf[c][s][l], sc[sub][c]);
-                    }
+                    for (int l = NL - 1; l >= 0; --l)
+#pragma unroll
+                        for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+                            for (int c = 0; c < NR; ++c)
+                                sc[sub][c] = mfma<BF16>(kf[sub], qf[c][s][l], sc[sub][c]);
                 }
+            };
+            f4 sc[2][NR];
+            if constexpr (WR == 1) {
+                if (n > 1) wait_vm<3 * NI>();
+                else wait_vm<NI>();
+            } else {
+                if (n >= NS) wait_vm<(NS - 1) * S::CW>();
+                else wait_vm<0>();
+                lds_barrier();
+            }
+            products(0, sc);
+            int stage = 0;
+            for (int i = 0; i < n; ++i) {
+                const int key0 = kbeg + i * KU;
+                const int stage1 = stage + 1 < NS ? stage + 1 : 0;
+                // this tile's values and the next one's keys have landed: this wave's
+                // copies of them, then everyone's; and all are done with this one's
+                // keys and the last one's values, whose places are filled anew
                 if constexpr (WR == 1) {
                     wait_lds();
-                    if (i + 2 < n) copy_k(i + 2);
+                    if (i + 2 < n) {
+                        place(i + 2);
+                        read_pages(i + 3);
+                        copy_k(stage);
+                        wait_vm<2 * NI>();
+                    } else if (i + 1 < n) {
+                        wait_vm<NI>();
+                    } else {
+                        wait_vm<0>();
+                    }
+                } else {
+                    if (i + NS - 1 < n) wait_vm<(NS - 2) * S::CW>();
+                    else if (i + 1 < n) wait_vm<S::CW / 2>();
+                    else wait_vm<0>();
+                    lds_barrier();
+                    if (i + NS - 1 < n) {
+                        place(i + NS);
+                        read_pages(i + NS + 1);
+                        copy_share(i + NS < n, stage, true, stage ? stage - 1 : NS - 1);
+                    }
                 }
-
-                // softmax
                 const bool tail = careful || key0 + KT > len;
                 float mul[NR];
 #pragma unroll
@@ -478,7 +548,31 @@ __global__ __launch_bounds__(64 * S::WAVES, 1) void attn_kernel(AttnArgs a) {
                                 sc[sub][c][r] = see >> (16 * sub + r) & 1 ? sc[sub][c][r] * rs[c]
                                                                           : -__builtin_inff();
                     }
+                    // values that are not finite: zeros, and noted where they are the request's.
+                    // (Waves that share the tile all do so, to the same effect.)
+                    bool odd = false;
+#pragma unroll 2
+                    for (int x = 0; x < NI; ++x) {
+                        auto* at = (__attribute__((address_space(3))) u4*)(uintptr_t)(
+                            gbase + stage * S::STAGE + S::KTILE + x * S::VSTEP + lane * 16);
+                        u4 v = *at;
+                        bool bad = false;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const bool lo = (v[e] & EXP) == EXP, hi = (v[e] >> 16 & EXP) == EXP;
+                            bad |= lo | hi;
+                            v[e] = (lo ? 0u : v[e] & 0xFFFFu) | (hi ? 0u : v[e] & 0xFFFF0000u);
+                        }
+                        odd |= bad && key0 + x * ROWS + lane / SLOTS < keys;
+                        *at = v;
+                    }
+                    if (odd) s_odd[wk] = 1;
                 }
+
+                // the next tile's products (of whatever is there, after the last) beside
+                // this one's softmax
+                f4 next[2][NR];
+                products(stage1 * S::STAGE, next);
                 u4 pf[NR][NL];
                 float alpha[NR];
                 bool moved = false;
@@ -487,11 +581,14 @@ __global__ __launch_bounds__(64 * S::WAVES, 1) void attn_kernel(AttnArgs a) {
                     float mx = sc[0][c][0];
 #pragma unroll
                     for (int r = 1; r < 8; ++r) mx = fmaxf(mx, sc[r >> 2][c][r & 3]);
-                    const float m = fmaxf(mrow[c], max4(mx) * mul[c]);
+                    mx = max4(mx) * mul[c];
+                    // the sums' reference follows the maximum in steps: exponentials
+                    // of up to 2^LAG are as good as those up to 1
+                    const float m = mx > mrow[c] + LAG ? mx : mrow[c];
                     moved |= m > mrow[c];
                     alpha[c] = __builtin_amdgcn_exp2f(mrow[c] - m);
                     mrow[c] = m;
-                    const float ref = BF16 ? -m : 14.0f - m;
+                    const float ref = BF16 ? -m : UP - m;
                     float p[8], sum = 0.0f;
 #pragma unroll
                     for (int r = 0; r < 8; ++r) {
@@ -513,35 +610,8 @@ __global__ __launch_bounds__(64 * S::WAVES, 1) void attn_kernel(AttnArgs a) {
 #pragma unroll
                         for (int d = 0; d < DT; ++d) o[d][c] *= alpha[c];
 
-                // values
-                if constexpr (WR == 1) {
-                    if (i + 2 < n) wait_vm<3 * NI>();
-                    else if (i + 1 < n) wait_vm<2 * NI>();
-                    else wait_vm<0>();
-                }
-                if (tail) {
-                    // values that are not finite: zeros, and noted where they are the request's.
-                    // (Waves that share the tile all do so, to the same effect.)
-                    bool odd = false;
-#pragma unroll 2
-                    for (int x = 0; x < NI; ++x) {
-                        auto* at = (__attribute__((address_space(3))) u4*)(uintptr_t)(
-                            gbase + sat + S::KTILE + x * S::VSTEP + lane * 16);
-                        u4 v = *at;
-                        bool bad = false;
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const bool lo = (v[e] & EXP) == EXP, hi = (v[e] >> 16 & EXP) == EXP;
-                            bad |= lo | hi;
-                            v[e] = (lo ? 0u : v[e] & 0xFFFFu) | (hi ? 0u : v[e] & 0xFFFF0000u);
-                        }
-                        odd |= bad && key0 + x * ROWS + lane / SLOTS < keys;
-                        *at = v;
-                    }
-                    if (odd) s_odd[wk] = 1;
-                }
                 const auto value = [&](int d) {
-                    const uint32_t at = vlane[d & 3] + sat + (d >> 2) * 128;
+                    const uint32_t at = vlane[d & 3] + stage * S::STAGE + (d >> 2) * 128;
                     const s4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(uintptr_t)at);
                     const s4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                         (lds_s4*)(uintptr_t)(at + J * S::VSTEP));
@@ -549,20 +619,28 @@ __global__ __launch_bounds__(64 * S::WAVES, 1) void attn_kernel(AttnArgs a) {
                     return u4{w0[0], w0[1], w1[0], w1[1]};
                 };
 #pragma unroll
-                for (int d = 0; d < DT; ++d) {
-                    const u4 vf = value(d);
+                for (int d = 0; d < DT; d += 2) {
+                    const u4 vf[2] = {value(d), value(d + 1)};
 #pragma unroll
-                    for (int c = 0; c < NR; ++c)
+                    for (int l = NL - 1; l >= 0; --l)
 #pragma unroll
-                        for (int l = NL - 1; l >= 0; --l) o[d][c] = mfma<BF16>(vf, pf[c][l], o[d][c]);
+                        for (int x = 0; x < 2; ++x)
+#pragma unroll
+                            for (int c = 0; c < NR; ++c)
+                                o[d + x][c] = mfma<BF16>(vf[x], pf[c][l], o[d + x][c]);
                 }
                 if constexpr (WR == 1) {
                     wait_lds();
-                    if (i + 2 < n) copy_v(i + 2);
-                    stage ^= 1;
-                } else {
-                    stage = stage + 1 < NS ? stage + 1 : 0;
+                    if (i + 2 < n) {
+                        at_v[0] = at_k[0], at_v[1] = at_k[1];
+                        copy_v(stage);
+                    }
                 }
+#pragma unroll
+                for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+                    for (int c = 0; c < NR; ++c) sc[sub][c] = next[sub][c];
+                stage = stage1;
             }
 
             // an infinite cached value times the two signs (or a zero) of a
@@ -806,8 +884,9 @@ hipError_t rows(const AttnArgs& a, int max_new, int cus, uint8_t* ws, hipStream_
         constexpr int N = D == 64 ? 4 : 2;
         if (r <= 16) return go<Shape<BF16, D, 1, 1, N, 2>>(a, cus, ws, st);
         if (r <= 32) return go<Shape<BF16, D, 2, 1, N, 2>>(a, cus, ws, st);
-        if (r <= 64) return go<Shape<BF16, D, 2, 2, 2, 3>>(a, cus, ws, st);
-        return go<Shape<BF16, D, 2, 4, 2, 4>>(a, cus, ws, st);
+        if (r <= 64) return go<Shape<BF16, D, 2, 2, 2, 4>>(a, cus, ws, st);
+        if constexpr (BF16) return go<Shape<BF16, D, 1, 8, 1, 8>>(a, cus, ws, st);
+        else return go<Shape<BF16, D, 2, 4, 2, 4>>(a, cus, ws, st);
     }
 }
 
