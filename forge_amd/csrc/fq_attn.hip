@@ -92,15 +92,18 @@ __device__ __forceinline__ f4 mfma(u4 a, u4 b, f4 c) {
                                                       __builtin_bit_cast(h8, b), c, 0, 0, 0);
 }
 
-// x0, x1 as NL pairs of 16-bit parts that add up to them.
+// x0, x1 as pairs of 16-bit parts that add up to them.  minus1: -1 where the
+// compiler does not see it, so that an fp16 rest is one fused multiply-add from the
+// packed part (with its rounding to fp16) and not a conversion and a subtraction.
 template <bool BF16>
 struct Parts {
     static constexpr int N = BF16 ? 3 : 2;
 };
 template <bool BF16>
-__device__ __forceinline__ void split2(float x0, float x1, uint32_t (&p)[Parts<BF16>::N]) {
+__device__ __forceinline__ void split2(float x0, float x1, float minus1,
+                                       uint32_t (&p)[Parts<BF16>::N]) {
     if constexpr (BF16) {
-        #pragma unroll
+#pragma unroll
         for (int i = 0; i < 3; ++i) {  // truncated: the rest is exact
             const uint32_t a = __float_as_uint(x0), b = __float_as_uint(x1);
             p[i] = __builtin_amdgcn_perm(b, a, 0x07060302u);
@@ -111,9 +114,13 @@ __device__ __forceinline__ void split2(float x0, float x1, uint32_t (&p)[Parts<B
         }
     } else {
         typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-        const h2 hi = {(_Float16)x0, (_Float16)x1};
-        const h2 lo = {(_Float16)(x0 - (float)hi[0]), (_Float16)(x1 - (float)hi[1])};
+        typedef float f2 __attribute__((ext_vector_type(2)));
+        const h2 hi = __builtin_convertvector((f2{x0, x1}), h2);
         p[0] = __builtin_bit_cast(uint32_t, hi);
+        asm("" : "+v"(p[0]));  // (one packed conversion, not one more for each rest)
+        const h2 back = __builtin_bit_cast(h2, p[0]);
+        const h2 lo = {(_Float16)fmaf((float)back[0], minus1, x0),
+                       (_Float16)fmaf((float)back[1], minus1, x1)};
         p[1] = __builtin_bit_cast(uint32_t, lo);
     }
 }
@@ -272,6 +279,8 @@ __global__ __launch_bounds__(64 * S::WAVES, 1) void attn_kernel(AttnArgs a) {
     lds_barrier();
 
     // --- constants of a lane ---
+    float minus1 = -1.0f;
+    asm("" : "+s"(minus1));
     const uint32_t gbase = lds_addr(lds) + wk * S::GROUP;
     // a copy's source: bytes from its first row
     uint32_t ksrc, vsrc;
@@ -456,7 +465,7 @@ __global__ __launch_bounds__(64 * S::WAVES, 1) void attn_kernel(AttnArgs a) {
                     for (int i = 0; i < 4; ++i) {
                         uint32_t p[NL];
                         split2<BF16>(x[s][i >> 1][2 * (i & 1)] * up,
-                                     x[s][i >> 1][2 * (i & 1) + 1] * up, p);
+                                     x[s][i >> 1][2 * (i & 1) + 1] * up, minus1, p);
 #pragma unroll
                         for (int l = 0; l < NL; ++l) qf[c][s][l][i] = p[l];
                     }
@@ -469,26 +478,36 @@ __global__ __launch_bounds__(64 * S::WAVES, 1) void attn_kernel(AttnArgs a) {
 #pragma unroll
                 for (int d = 0; d < DT; ++d) o[d][c] = f4{0, 0, 0, 0};
             }
-            // products of the keys at `at` (limbs of one sum apart, so that no
-            // product waits for the one before)
-            const auto products = [&](uint32_t at, f4 (&sc)[2][NR]) {
+            // Products of the keys at `at`, STEPS times 2 NL NR matrix instructions with
+            // beside(s) after each.  (The parts of one sum apart, so that no product
+            // waits for the one before.)  The waves of a SIMD mostly stand at the same
+            // place: in short turns one has the matrix unit while the other has
+            // the vector unit.
+            const auto products = [&](uint32_t at, f4 (&sc)[2][NR], const auto& beside) {
+                const auto keys_of = [&](int s, u4 (&kf)[2]) {
+#pragma unroll
+                    for (int sub = 0; sub < 2; ++sub)
+                        kf[sub] = *(lds_u4*)(uintptr_t)(klane + at + J * sub * S::KSTEP + 64 * s);
+                };
+                u4 kf[2][2];
+                keys_of(0, kf[0]);
 #pragma unroll
                 for (int sub = 0; sub < 2; ++sub)
 #pragma unroll
                     for (int c = 0; c < NR; ++c) sc[sub][c] = f4{0, 0, 0, 0};
 #pragma unroll
                 for (int s = 0; s < STEPS; ++s) {
-                    u4 kf[2];
-#pragma unroll
-                    for (int sub = 0; sub < 2; ++sub)
-                        kf[sub] = *(lds_u4*)(uintptr_t)(klane + at + J * sub * S::KSTEP + 64 * s);
+                    if (s + 1 < STEPS) keys_of(s + 1, kf[(s + 1) & 1]);
 #pragma unroll
                     for (int l = NL - 1; l >= 0; --l)
 #pragma unroll
                         for (int sub = 0; sub < 2; ++sub)
 #pragma unroll
                             for (int c = 0; c < NR; ++c)
-                                sc[sub][c] = mfma<BF16>(kf[sub], qf[c][s][l], sc[sub][c]);
+                                sc[sub][c] = mfma<BF16>(kf[s & 1][sub], qf[c][s][l], sc[sub][c]);
+                    __builtin_amdgcn_sched_barrier(0);
+                    beside(s);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
             };
             f4 sc[2][NR];
@@ -500,7 +519,7 @@ __global__ __launch_bounds__(64 * S::WAVES, 1) void attn_kernel(AttnArgs a) {
                 else wait_vm<0>();
                 lds_barrier();
             }
-            products(0, sc);
+            products(0, sc, [](int) {});
             int stage = 0;
             for (int i = 0; i < n; ++i) {
                 const int key0 = kbeg + i * KU;
@@ -572,12 +591,10 @@ __global__ __launch_bounds__(64 * S::WAVES, 1) void attn_kernel(AttnArgs a) {
                 // the next tile's products (of whatever is there, after the last) beside
                 // this one's softmax
                 f4 next[2][NR];
-                products(stage1 * S::STAGE, next);
                 u4 pf[NR][NL];
-                float alpha[NR];
+                float alpha[NR], ref[NR], sum[NR];
                 bool moved = false;
-#pragma unroll
-                for (int c = 0; c < NR; ++c) {
+                const auto maximum = [&](int c) {
                     float mx = sc[0][c][0];
 #pragma unroll
                     for (int r = 1; r < 8; ++r) mx = fmaxf(mx, sc[r >> 2][c][r & 3]);
@@ -588,22 +605,35 @@ __global__ __launch_bounds__(64 * S::WAVES, 1) void attn_kernel(AttnArgs a) {
                     moved |= m > mrow[c];
                     alpha[c] = __builtin_amdgcn_exp2f(mrow[c] - m);
                     mrow[c] = m;
-                    const float ref = BF16 ? -m : UP - m;
-                    float p[8], sum = 0.0f;
+                    ref[c] = BF16 ? -m : UP - m;
+                    sum[c] = 0.0f;
+                };
+                const auto exponentials = [&](int c, int sub) {
+                    float p[4];
 #pragma unroll
-                    for (int r = 0; r < 8; ++r) {
-                        p[r] = __builtin_amdgcn_exp2f(fmaf(sc[r >> 2][c][r & 3], mul[c], ref));
-                        sum += p[r];
+                    for (int r = 0; r < 4; ++r) {
+                        p[r] = __builtin_amdgcn_exp2f(fmaf(sc[sub][c][r], mul[c], ref[c]));
+                        sum[c] += p[r];
                     }
-                    lrow[c] = lrow[c] * alpha[c] + sum;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
+                    for (int e = 0; e < 2; ++e) {
                         uint32_t q2[NL];
-                        split2<BF16>(p[2 * e], p[2 * e + 1], q2);
+                        split2<BF16>(p[2 * e], p[2 * e + 1], minus1, q2);
 #pragma unroll
-                        for (int l = 0; l < NL; ++l) pf[c][l][e] = q2[l];
+                        for (int l = 0; l < NL; ++l) pf[c][l][2 * sub + e] = q2[l];
                     }
-                }
+                    if (sub == 1) lrow[c] = lrow[c] * alpha[c] + sum[c];
+                };
+                products(stage1 * S::STAGE, next, [&](int s) {
+                    // the rows' maxima, then their two halves of exponentials, spread over
+                    // the steps
+                    constexpr int PIECES = 3 * NR;
+#pragma unroll
+                    for (int x = s * PIECES / STEPS; x < (s + 1) * PIECES / STEPS; ++x) {
+                        if (x < NR) maximum(x);
+                        else exponentials((x - NR) / 2, (x - NR) % 2);
+                    }
+                });
                 if (__any(moved))
 #pragma unroll
                     for (int c = 0; c < NR; ++c)
