@@ -72,10 +72,10 @@ struct LogpArgs {
     int J, top;
     float *logprobs, *entropy, *top_logprobs;
     int* top_tokens;
-    int splits, seg;  // a row's work-groups and the elements of each
-    uint8_t* ws;
+    int seg, splits;  // elements of a wave; work-groups of a row
+    uint8_t* ws;      // results of split rows, logp_part_bytes
 };
-size_t logp_part_bytes();  // of the largest call
-hipError_t launch_logp(LogpArgs a, int type, int cus, uint8_t* ws, hipStream_t st);
+size_t logp_part_bytes(int cus);  // of the largest call
+hipError_t launch_logp(const LogpArgs& a, int type, int cus, hipStream_t st);
 
 }  // namespace fq

@@ -45,7 +45,7 @@ int device(int* dev) {
 
 int done(hipError_t e) { return e == hipSuccess ? FQ_OK : hip_fail(e); }
 
-size_t step_bytes(int cus) { return std::max(fq::attn_part_bytes(cus), fq::logp_part_bytes()); }
+size_t step_bytes(int cus) { return std::max(fq::attn_part_bytes(cus), fq::logp_part_bytes(cus)); }
 
 }  // namespace
 
@@ -179,7 +179,7 @@ int fq_token_logprobs(const void* logits, uint32_t type, int64_t ld, int M, int 
                       const int32_t* targets, int J, int top, float* logprobs, float* entropy,
                       float* top_logprobs, int32_t* top_tokens, void* stream) {
     if (type != FQ_TYPE_F32 && type != FQ_TYPE_F16 && type != FQ_TYPE_BF16) return FQ_ERR_DTYPE;
-    // (a row's last chunk ends past V, and 256 lanes a row make up the grid: ints)
+    // (a row's last part ends past V, and 256 lanes a row make up the grid: ints)
     if (M < 0 || M > (1 << 22) || V < 1 || V > INT32_MAX / 2 || ld < V || J < 0 || top < 0 || top > 64 ||
         top > V)
         return FQ_ERR_SHAPE;
@@ -205,10 +205,9 @@ int fq_token_logprobs(const void* logits, uint32_t type, int64_t ld, int M, int 
     a.top_logprobs = top_logprobs;
     a.top_tokens = top_tokens;
     fq::StreamScratch::Lease lease(fq::stream_scratch(dev, st, 2));
-    uint8_t* ws = nullptr;
-    const int rs = lease.get(step_bytes(cus), st, &ws);
+    const int rs = lease.get(step_bytes(cus), st, &a.ws);
     if (rs != FQ_OK) return rs;
-    return done(fq::launch_logp(a, type == FQ_TYPE_F32 ? 0 : type == FQ_TYPE_F16 ? 1 : 2, cus, ws, st));
+    return done(fq::launch_logp(a, type == FQ_TYPE_F32 ? 0 : type == FQ_TYPE_F16 ? 1 : 2, cus, st));
 }
 
 int fq_reserve_step(void* stream) {

@@ -512,6 +512,19 @@ def test_logprobs_masked_rows():
         run_logprobs(x, [[0, 7]] * 6, 10)
 
 
+def test_logprobs_where_every_part_of_a_row_has_all_the_largest():
+    # the largest logits lie in the last token's neighbourhood, then spread evenly
+    g = torch.Generator().manual_seed(3)
+    for V, M in ((40000, 2), (40000, 300), (70000, 600)):
+        x = torch.randn((M, V), generator=g).cuda()
+        x[:, -64:] += 20
+        run_logprobs(x, [V - 1] * M, 64)
+        x[:, ::V // 2000] += 40
+        run_logprobs(x, [0] * M, 64)
+    steps = torch.arange(120000.0, device="cuda")  # rising by units: every chunk has larger ones
+    run_logprobs(steps[None].repeat(3, 1) / 1024, [0, 1, 119999], 64)
+
+
 def test_logprobs_targets_outside_the_vocabulary():
     x = torch.randn((2, 777), device="cuda")
     run_logprobs(x, [[0, -1, 776], [777, 2 ** 31 - 1, -2 ** 31]], 3)
