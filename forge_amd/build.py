@@ -1,6 +1,6 @@
 """Build the gfx950 shared library in-tree with hipcc.
 
-    python -m forge_amd.build          # -> forge_amd/libforge_q.so
+    python -m forge_amd.build          # -> forge_amd/libforge_q.so, forge_amd/_step.so
 
 The library is compiled for gfx950 only.  Packed-FP32 instruction selection
 is disabled (-packed-fp32-ops) for every HIP translation unit.
@@ -16,6 +16,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "libforge_q.so")
+STEP = os.path.join(HERE, "_step.so")
 OBJDIR = os.path.join(HERE, "_build")
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
@@ -50,6 +51,27 @@ def _compile(src: str) -> str:
     return obj
 
 
+def _binding() -> None:
+    """forge_amd/_step.so: the step operators' host side over torch tensors, a plain
+    CPython extension that calls the library's C ABI."""
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+    lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    tmp = STEP + ".tmp"
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *(f"-isystem{p}" for p in cpp_extension.include_paths()),
+           f"-isystem{sysconfig.get_paths()['include']}", os.path.join(CSRC, "fq_step_py.cpp"),
+           "-o", tmp, f"-L{HERE}", "-l:libforge_q.so", "-Wl,-rpath,$ORIGIN", f"-L{lib}", "-lc10",
+           "-ltorch_cpu", "-ltorch_python", f"-Wl,-rpath,{lib}"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed for fq_step_py.cpp:\n{r.stderr}")
+    os.replace(tmp, STEP)
+
+
 def build(verbose: bool = True) -> str:
     os.makedirs(OBJDIR, exist_ok=True)
     srcs = [s for s in SOURCES if os.path.exists(os.path.join(CSRC, s))]
@@ -61,6 +83,7 @@ def build(verbose: bool = True) -> str:
     if r.returncode != 0:
         raise RuntimeError(f"link failed:\n{r.stderr}")
     os.replace(tmp, OUT)
+    _binding()
     if verbose:
         print(f"built {OUT}")
     return OUT
