@@ -130,7 +130,8 @@ struct Request {
     int t0, nt, len;  // its first new token, how many, its cached tokens
     int keys, nu;     // keys and units of them
     int rts;          // tiles of RT rows
-    int64_t units;    // of all its items, OV more for each
+    int cost;         // an item's units and OV more, or 1 where items are not cut
+    int64_t units;    // that of all its items
 };
 template <int RT, int KU, int OV>
 __device__ __forceinline__ Request request(const AttnArgs& a, int c0, int c1, int len) {
@@ -143,7 +144,8 @@ __device__ __forceinline__ Request request(const AttnArgs& a, int c0, int c1, in
     r.keys = (int)min((int64_t)r.len + r.nt, min(most, (int64_t)INT32_MAX - 4096));
     r.nu = (r.keys + KU - 1) / KU;
     r.rts = (int)(((int64_t)r.nt * a.G + RT - 1) / RT);
-    r.units = r.nu ? (int64_t)a.hkv * r.rts * (r.nu + OV) : 0;
+    r.cost = a.whole ? 1 : r.nu + OV;
+    r.units = r.nu ? (int64_t)a.hkv * r.rts * r.cost : 0;
     return r;
 }
 
@@ -178,13 +180,25 @@ __device__ __forceinline__ uint32_t shifted(uint64_t m, int n) {
     return n >= 32 || n <= -64 ? 0u : n >= 0 ? (uint32_t)m << n : (uint32_t)(m >> -n);
 }
 
+// Where a token lies in a cache whose page (block) that is, in bytes.  (Strides are below
+// 2^31 elements: 32-bit factors.)
+__device__ __forceinline__ uint64_t place_of(const AttnArgs& a, int page, int key) {
+    const uint32_t pg = min((uint32_t)max(page, 0), (uint32_t)a.c.num_blocks - 1);
+    const uint32_t in = (uint32_t)key & ((1u << a.c.bs_log2) - 1);
+    return 2 * ((uint64_t)pg * (uint32_t)a.c.sb + (uint64_t)in * (uint32_t)a.c.st);
+}
+
+constexpr int DESC = 4;       // ints of a work-group's record, beside the number of parts
+constexpr int MAX_GRID = 3;   // work-groups to a CU at most,
+constexpr size_t MAX_PART = 2 * 128 * (128 + 2);  // and floats of a part of each of them
+
 // WR x WK waves: each group of WR shares tiles of 32 keys, each of its waves
 // with 16 NR rows of its own; the groups take every WK-th tile.  NS tiles of a
-// group are in LDS.
-template <bool BF16_, int D_, int NR_, int WR_, int WK_, int NS_>
+// group are in LDS.  PC work-groups to a CU.
+template <bool BF16_, int D_, int NR_, int WR_, int WK_, int NS_, int PC_>
 struct Shape {
     static constexpr bool BF16 = BF16_;
-    static constexpr int D = D_, NR = NR_, WR = WR_, WK = WK_, NS = NS_;
+    static constexpr int D = D_, NR = NR_, WR = WR_, WK = WK_, NS = NS_, PC = PC_;
     static constexpr int WAVES = WR * WK;
     static constexpr int DP = D <= 64 ? 64 : D <= 128 ? 128 : 256;  // LDS row, elements
     static constexpr int PITCH = 2 * DP;
@@ -199,7 +213,7 @@ struct Shape {
     // that the 16 lanes of a read find 16 (values: 8) places of the 256
     // bytes that the banks span, with every place an immediate offset from few registers.
     static constexpr int KSTEP = 1024 + (D == 256 ? 32 : 64);
-    static constexpr int VSTEP = 1024 + (D == 256 ? 64 : D == 64 ? 0 : 128);
+    static constexpr int VSTEP = 1024 + (D == 64 ? 0 : 64);
     static __device__ __forceinline__ int turn(int row) {
         return D == 64 ? (row >> 1) & 3 : D == 256 ? row & 1 : row & 3;
     }
@@ -214,14 +228,13 @@ struct Shape {
     // the waves' outputs are exchanged where the tiles were
     static_assert((size_t)WAVES * NR * 16 * D * 4 <= LDS, "join");
     static_assert(D / 16 % WK == 0, "join");
+    static_assert(PC * (LDS + 8 * WK * (RT + 1) + 64) <= 160 * 1024, "LDS");
+    static_assert(PC <= MAX_GRID && (size_t)PC * PART <= MAX_PART, "workspace");
 };
 
-constexpr int DESC = 8;  // ints of a work-group's record
-constexpr int MAX_GRID = 2;                  // work-groups to a CU at most,
-constexpr size_t MAX_PART = 128 * (128 + 2); // and the floats of a part of each
 
 template <class S>
-__global__ __launch_bounds__(64 * S::WAVES, 1) void attn_kernel(AttnArgs a) {
+__global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void attn_kernel(AttnArgs a) {
     constexpr bool BF16 = S::BF16;
     constexpr int D = S::D, NR = S::NR, WR = S::WR, WK = S::WK, NS = S::NS;
     constexpr int NL = Parts<BF16>::N;
@@ -258,7 +271,7 @@ __global__ __launch_bounds__(64 * S::WAVES, 1) void attn_kernel(AttnArgs a) {
         b = at * per;
         off = u0 - uni64(__shfl(upto - mine, at));
     }
-    int* desc = a.desc + wg * DESC;
+    int* desc = a.desc + a.grid + wg * DESC;
     // padding tokens
     {
         const int end = min(max(sload(a.cu + a.B), 0), a.N);
@@ -269,7 +282,7 @@ __global__ __launch_bounds__(64 * S::WAVES, 1) void attn_kernel(AttnArgs a) {
     }
     int64_t u = wg * span;
     if (u >= total) {
-        if (tid == 0) desc[0] = 0;
+        if (tid == 0) a.desc[wg] = 0;
         return;
     }
     int64_t left = min(span, total - u);
@@ -312,12 +325,13 @@ __global__ __launch_bounds__(64 * S::WAVES, 1) void attn_kernel(AttnArgs a) {
         }
         int item = 0, pos = 0;
         if (off) {
-            item = (int)(off / (nu + OV));
-            pos = (int)(off % (nu + OV));
+            item = (int)(off / rq.cost);
+            pos = (int)(off % rq.cost);
         }
         while (off < rq.units && left > 0) {
-            const int take = (int)min((int64_t)(nu + OV - pos), left);
-            const int first = max(pos - OV, 0), count = max(pos + take - OV, 0) - first;
+            const int take = (int)min((int64_t)(rq.cost - pos), left);
+            const int first = a.whole ? 0 : max(pos - OV, 0);
+            const int count = a.whole ? nu : max(pos + take - OV, 0) - first;
             const int64_t start = u - pos;  // the item's
             u += take;
             off += take;
@@ -351,13 +365,12 @@ __global__ __launch_bounds__(64 * S::WAVES, 1) void attn_kernel(AttnArgs a) {
 #pragma unroll
                 for (int hf = 0; hf < 2; ++hf) page[hf] = sload(table + (key_of(i, hf) >> a.c.bs_log2));
             };
-            int64_t at_k[2], at_v[2];  // of the tiles whose keys, values are copied next
+            uint64_t at_k[2], at_v[2];  // of the tiles whose keys, values are copied next
             const auto place = [&](int i) {
 #pragma unroll
                 for (int hf = 0; hf < 2; ++hf) {
-                    const int pg = min(max(page[hf], 0), a.c.num_blocks - 1);
                     at_v[hf] = at_k[hf];
-                    at_k[hf] = 2 * (pg * a.c.sb + (key_of(i, hf) & ((1 << a.c.bs_log2) - 1)) * a.c.st);
+                    at_k[hf] = place_of(a, page[hf], key_of(i, hf));
                 }
             };
             const int64_t step = 2 * ROWS * a.c.st;  // bytes from copy to copy
@@ -379,18 +392,25 @@ __global__ __launch_bounds__(64 * S::WAVES, 1) void attn_kernel(AttnArgs a) {
                         copy16(vsrc, from, gbase + stage * S::STAGE + S::KTILE + (hf * J + j) * S::VSTEP);
                 }
             };
-            // this wave's share of a tile's keys and of the one before's values
+            // This wave's share of a tile's keys and of the one before's values: copies wr,
+            // wr + WR, .. of the NI of keys and the NI of values, copy c being number c % J of the
+            // 16 keys c / J.  Whatever does not depend on wr is known here.
+            const uint8_t *kw = kb + (wr % J) * step, *vw = vb + (wr % J) * step;
             const auto copy_share = [&](bool ks, int kstage, bool vs, int vstage) {
+                const uint32_t kto = gbase + kstage * S::STAGE + wr * S::KSTEP;
+                const uint32_t vto = gbase + vstage * S::STAGE + S::KTILE + wr * S::VSTEP;
 #pragma unroll
                 for (int x = 0; x < S::CW; ++x) {
-                    const int ci = wr + WR * x, c = ci % NI;
-                    const int64_t in = (c % J) * step;
-                    if (ci < NI) {
-                        if (ks) copy16(ksrc, kb + (c >= J ? at_k[1] : at_k[0]) + in,
-                                       gbase + kstage * S::STAGE + c * S::KSTEP);
+                    constexpr bool LOW = WR <= J;  // (all of a copy's place but wr is known)
+                    const int c0 = WR * x % NI;
+                    const bool isv = WR <= NI ? WR * x >= NI : wr >= NI;
+                    const bool upper = LOW ? c0 >= J : (wr / J) % 2 == 1;
+                    const uint64_t in = LOW ? (uint64_t)((c0 % J) * step) : 0;
+                    const int over = WR <= NI ? c0 : isv ? -NI : 0;  // copies past wr's
+                    if (!isv) {
+                        if (ks) copy16(ksrc, kw + ((upper ? at_k[1] : at_k[0]) + in), kto + over * S::KSTEP);
                     } else if (vs) {
-                        copy16(vsrc, vb + (c >= J ? at_v[1] : at_v[0]) + in,
-                               gbase + vstage * S::STAGE + S::KTILE + c * S::VSTEP);
+                        copy16(vsrc, vw + ((upper ? at_v[1] : at_v[0]) + in), vto + over * S::VSTEP);
                     }
                 }
             };
@@ -708,8 +728,7 @@ __global__ __launch_bounds__(64 * S::WAVES, 1) void attn_kernel(AttnArgs a) {
                 for (int key = kbeg; key < kbeg + n * KU && key < keys; ++key) {
                     const int at = (key - kbeg) % KU, key0 = key - at;
                     if (at >= KT || !(careful || key0 + KT > len)) continue;
-                    const int page = min(max(sload(table + (key >> a.c.bs_log2)), 0), a.c.num_blocks - 1);
-                    const uint8_t* v = vb + 2 * (page * a.c.sb + (key & ((1 << a.c.bs_log2) - 1)) * a.c.st);
+                    const uint8_t* v = vb + place_of(a, sload(table + (key >> a.c.bs_log2)), key);
                     bool see[NR];
 #pragma unroll
                     for (int c = 0; c < NR; ++c) see[c] = seen(mask[c], len - key0, keys - key0) >> at & 1;
@@ -772,9 +791,9 @@ __global__ __launch_bounds__(64 * S::WAVES, 1) void attn_kernel(AttnArgs a) {
                         v = o[d0][c];
                     }
                     if (whole) v = lsum[c] != 0.0f ? v * inv : f4{0, 0, 0, 0};
-                    if (!whole || t < nt) *(f4*)(to + 16 * d + 4 * (ln / 16)) = v;
+                    if (t < nt) *(f4*)(to + 16 * d + 4 * (ln / 16)) = v;
                 }
-                if (!whole && wk == 0 && ln < 16) {
+                if (!whole && wk == 0 && ln < 16 && t < nt) {
                     part[RT * D + rl] = mrow[c];
                     part[RT * D + RT + rl] = lsum[c];
                 }
@@ -783,124 +802,173 @@ __global__ __launch_bounds__(64 * S::WAVES, 1) void attn_kernel(AttnArgs a) {
                 cut = true;
                 if (tid == 0) {
                     const int64_t end = start + OV + nu - 1;  // the item's last unit
-                    desc[0] = (int)(end / span) - wg + 1;
-                    desc[1] = t0, desc[2] = nt, desc[3] = h, desc[4] = rt;
+                    a.desc[wg] = (int)(end / span) - wg + 1;
+                    desc[0] = t0, desc[1] = nt, desc[2] = h, desc[3] = rt;
                 }
             }
             lds_barrier();  // the exchanged outputs are read
         }
         off -= rq.units;
     }
-    if (!cut && tid == 0) desc[0] = 0;
+    if (!cut && tid == 0) a.desc[wg] = 0;
 }
 
-// Joins the parts of the items that are cut: one row after the other, by one wave
-// or, where an item has many parts, by the four waves of a work-group.
-constexpr int JOIN_GRID = 1024;
+// Joins the parts of the items that are cut: two rows at a time by one wave or, where
+// an item has many parts, one row by the four waves of a work-group.
+constexpr int JOIN_WGS = 8;  // work-groups to a CU
+constexpr int MAX_ITEMS = 1024;
+constexpr int NARROW = 16;   // parts of an item that one wave joins
 
 template <int D, int RT>
 __global__ __launch_bounds__(256) void attn_join(AttnArgs a) {
     constexpr int PART = RT * (D + 2), E = D == 64 ? 1 : D == 256 ? 4 : 2;
     typedef float fe __attribute__((ext_vector_type(E)));
-    __shared__ int s_list[512], s_count[8], s_most[4];
+    struct Item {
+        int parts, w, t0, nt, h, rt;
+    };
+    __shared__ Item s_item[MAX_ITEMS];
+    __shared__ int s_count[4], s_most[4];
     __shared__ float s_acc[4][D + 1];
     const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6);
-    // the work-groups that began such an item, in their order (a.grid <= 512)
-    int parts2[2], most = 0;
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-        const int i = k * 256 + tid;
-        parts2[k] = i < a.grid ? a.desc[i * DESC] : 0;
-        most = max(most, parts2[k]);
-        const uint64_t some = __ballot(parts2[k] > 0);
-        if (lane == 0) s_count[4 * k + wave] = __popcll(some);
+    // the items, in the order of the work-groups that began them
+    int items = 0, most = 0;
+    for (int i0 = 0; i0 < a.grid; i0 += 256) {
+        const int i = i0 + tid;
+        Item x;
+        x.parts = i < a.grid ? a.desc[i] : 0;
+        x.w = i;
+        if (x.parts) {
+            const int* d = a.desc + a.grid + i * DESC;
+            x.t0 = d[0], x.nt = d[1], x.h = d[2], x.rt = d[3];
+        }
+        most = max(most, x.parts);
+        const uint64_t some = __ballot(x.parts > 0);
+        if (lane == 0) s_count[wave] = __popcll(some);
+        __syncthreads();
+        int at = items + __popcll(some & ((1ull << lane) - 1));
+        for (int v = 0; v < 4; ++v) {
+            at += v < wave ? s_count[v] : 0;
+            items += s_count[v];
+        }
+        if (x.parts) s_item[at] = x;
+        __syncthreads();
     }
     for (int o = 32; o; o >>= 1) most = max(most, __shfl_xor(most, o));
     if (lane == 0) s_most[wave] = most;
     __syncthreads();
-    int items = 0;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-        const uint64_t some = __ballot(parts2[k >> 2] > 0);
-        if ((k & 3) == wave && parts2[k >> 2] > 0)
-            s_list[items + __popcll(some & ((1ull << lane) - 1))] = (k >> 2) * 256 + tid;
-        items += s_count[k];
-    }
     most = max(max(s_most[0], s_most[1]), max(s_most[2], s_most[3]));
-    __syncthreads();
-    const bool wide = most > 8;
-    const int per = wide ? RT : RT / 4, jobs = items * per;
-    for (int job = blockIdx.x; job < jobs; job += gridDim.x) {
-        const int w = uni(s_list[job / per]);
-        const int rl = wide ? job % per : job % per * 4 + wave;
-        const int* desc = a.desc + w * DESC;
-        const int parts = sload(desc), t0 = sload(desc + 1), nt = sload(desc + 2);
-        const int h = sload(desc + 3), rt = sload(desc + 4);
-        const int r = rt * RT + rl, t = r / a.G;
-        if (t >= nt) continue;
-        const auto slot = [&](int p) { return a.part + (int64_t)(2 * (w + p) + (p == 0)) * PART; };
+    const auto slot = [&](const Item& x, int p) {
+        return a.part + (int64_t)(2 * (x.w + p) + (p == 0)) * PART;
+    };
+    const auto store = [&](const Item& x, int r, fe acc, float l) {
+        const int t = r / a.G;
+        fe v = 0.0f;
+        if (l != 0.0f) v = acc * (1.0f / l);
+        if (E * lane < D)
+            *(fe*)(a.out + ((int64_t)(x.t0 + t) * a.hq + x.h * a.G + r % a.G) * D + E * lane) = v;
+    };
+    if (most <= NARROW) {
+        constexpr int R = 2;
+        for (int job = blockIdx.x * 4 + wave; job < items * (RT / R); job += gridDim.x * 4) {
+            const Item x = s_item[job / (RT / R)];
+            const int rl = job % (RT / R) * R, r0 = x.rt * RT + rl;
+            if (r0 >= x.nt * a.G) continue;
+            float mp[R], lp[R];
+            fe o[R][NARROW];
+#pragma unroll
+            for (int k = 0; k < R; ++k) {
+                mp[k] = LOWEST, lp[k] = 0.0f;
+                const bool on = r0 + k < x.nt * a.G;
+                if (on && lane < x.parts) {
+                    const float* s = slot(x, lane) + RT * D + rl + k;
+                    mp[k] = s[0], lp[k] = s[RT];
+                }
+#pragma unroll
+                for (int p = 0; p < NARROW; ++p) {
+                    o[k][p] = 0.0f;
+                    if (on && p < x.parts && E * lane < D) o[k][p] = *(const fe*)(slot(x, p) + (rl + k) * D + E * lane);
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < R; ++k) {
+                float m = mp[k];
+                for (int q = NARROW / 2; q; q >>= 1) m = fmaxf(m, __shfl_xor(m, q));
+                m = __shfl(m, 0);
+                const float f = __builtin_amdgcn_exp2f(mp[k] - m);
+                float l = lp[k] * f;
+                for (int q = NARROW / 2; q; q >>= 1) l += __shfl_xor(l, q);
+                l = __shfl(l, 0);
+                fe acc = 0.0f;
+#pragma unroll
+                for (int p = 0; p < NARROW; ++p)
+                    if (p < x.parts) acc += __shfl(f, p) * o[k][p];
+                if (r0 + k < x.nt * a.G) store(x, r0 + k, acc, l);
+            }
+        }
+        return;
+    }
+    for (int job = blockIdx.x; job < items * RT; job += gridDim.x) {
+        const Item x = s_item[job / RT];
+        const int rl = job % RT, r = x.rt * RT + rl, parts = x.parts;
+        if (r >= x.nt * a.G) continue;
         float m = LOWEST;
-        for (int p = lane; p < parts; p += 64) m = fmaxf(m, slot(p)[RT * D + rl]);
+        for (int p = lane; p < parts; p += 64) m = fmaxf(m, slot(x, p)[RT * D + rl]);
         for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-        const int share = wide ? (parts + 3) / 4 : parts;
-        const int beg = wide ? wave * share : 0, end = min(parts, beg + share);
+        const int share = (parts + 3) / 4, beg = wave * share, end = min(parts, beg + share);
         fe acc = 0.0f;
         float l = 0.0f;
         for (int p0 = beg; p0 < end; p0 += 64) {
             float f = 0.0f, lp = 0.0f;
             if (p0 + lane < end) {
-                const float* s = slot(p0 + lane) + RT * D + rl;
+                const float* s = slot(x, p0 + lane) + RT * D + rl;
                 f = __builtin_amdgcn_exp2f(s[0] - m);
                 lp = s[RT] * f;
             }
             for (int o = 32; o; o >>= 1) lp += __shfl_xor(lp, o);
             l += lp;
             for (int p = p0; p < min(end, p0 + 64); p += 8) {
-                fe x[8];
+                fe o[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    x[i] = 0.0f;
-                    if (p + i < end && E * lane < D) x[i] = *(const fe*)(slot(p + i) + rl * D + E * lane);
+                    o[i] = 0.0f;
+                    if (p + i < end && E * lane < D) o[i] = *(const fe*)(slot(x, p + i) + rl * D + E * lane);
                 }
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const float fp = __uint_as_float(
-                        __builtin_amdgcn_readlane(__float_as_uint(f), (p + i - p0) & 63));
-                    if (p + i < end) acc += fp * x[i];
+                    const float fp = __shfl(f, (p + i - p0) & 63);
+                    if (p + i < end) acc += fp * o[i];
                 }
             }
         }
-        if (wide) {
-            if (E * lane < D)
-                for (int e = 0; e < E; ++e) s_acc[wave][E * lane + e] = acc[e];
-            if (lane == 0) s_acc[wave][D] = l;
-            __syncthreads();
-            acc = 0.0f;
-            l = 0.0f;
-            for (int i = 0; i < 4; ++i) {
-                l += s_acc[i][D];
-                if (E * lane < D)
-                    for (int e = 0; e < E; ++e) acc[e] += s_acc[i][E * lane + e];
-            }
-            __syncthreads();
-            if (wave) continue;
-        }
-        fe v = 0.0f;
-        if (l != 0.0f) v = acc * (1.0f / l);
         if (E * lane < D)
-            *(fe*)(a.out + ((int64_t)(t0 + t) * a.hq + h * a.G + r % a.G) * D + E * lane) = v;
+            for (int e = 0; e < E; ++e) s_acc[wave][E * lane + e] = acc[e];
+        if (lane == 0) s_acc[wave][D] = l;
+        __syncthreads();
+        acc = 0.0f;
+        l = 0.0f;
+        for (int i = 0; i < 4; ++i) {
+            l += s_acc[i][D];
+            if (E * lane < D)
+                for (int e = 0; e < E; ++e) acc[e] += s_acc[i][E * lane + e];
+        }
+        __syncthreads();
+        if (wave == 0) store(x, r, acc, l);
     }
 }
 
+size_t desc_bytes(int cus) { return ((size_t)MAX_GRID * cus * (DESC + 1) * 4 + 255) & ~(size_t)255; }
+
 template <class S>
 hipError_t go(AttnArgs a, int cus, uint8_t* ws, hipStream_t st) {
-    constexpr int PER_CU = (int)(160 * 1024 / (S::LDS + 4096)) >= 2 && S::WAVES <= 4 ? 2 : 1;
-    static_assert((size_t)PER_CU * S::PART <= MAX_PART, "workspace");
-    a.grid = PER_CU * cus;
+    a.grid = S::PC * cus;
     a.desc = (int*)ws;
-    a.part = (float*)(ws + (size_t)MAX_GRID * cus * DESC * 4);
+    a.part = (float*)(ws + desc_bytes(cus));
+    // Where a request has few keys at most (by its table's columns), its items are not
+    // cut, and there is nothing to join: six units take about as long as a second launch.
+    a.whole = (int64_t)a.max_blocks << a.c.bs_log2 <= 6 * std::max(S::KU, 64);
+    if (a.grid > MAX_ITEMS) return hipErrorInvalidConfiguration;
     hipLaunchKernelGGL(attn_kernel<S>, dim3(a.grid), dim3(64 * S::WAVES), S::LDS, st, a);
-    hipLaunchKernelGGL((attn_join<S::D, S::RT>), dim3(JOIN_GRID), dim3(256), 0, st, a);
+    if (!a.whole) hipLaunchKernelGGL((attn_join<S::D, S::RT>), dim3(JOIN_WGS * cus), dim3(256), 0, st, a);
     return hipGetLastError();
 }
 
@@ -908,15 +976,17 @@ template <bool BF16, int D>
 hipError_t rows(const AttnArgs& a, int max_new, int cus, uint8_t* ws, hipStream_t st) {
     const int64_t r = (int64_t)max_new * a.G;
     if constexpr (D == 256) {
-        if (r <= 16) return go<Shape<BF16, D, 1, 1, 2, 2>>(a, cus, ws, st);
-        return go<Shape<BF16, D, 1, 4, 1, 4>>(a, cus, ws, st);
+        if (r <= 16) return go<Shape<BF16, D, 1, 1, 2, 2, 1>>(a, cus, ws, st);
+        return go<Shape<BF16, D, 1, 4, 1, 4, 1>>(a, cus, ws, st);
     } else {
         constexpr int N = D == 64 ? 4 : 2;
-        if (r <= 16) return go<Shape<BF16, D, 1, 1, N, 2>>(a, cus, ws, st);
-        if (r <= 32) return go<Shape<BF16, D, 2, 1, N, 2>>(a, cus, ws, st);
-        if (r <= 64) return go<Shape<BF16, D, 2, 2, 2, 4>>(a, cus, ws, st);
-        if constexpr (BF16) return go<Shape<BF16, D, 1, 8, 1, 8>>(a, cus, ws, st);
-        else return go<Shape<BF16, D, 2, 4, 2, 4>>(a, cus, ws, st);
+        if (r <= 16) return go<Shape<BF16, D, 1, 1, N, 2, 2>>(a, cus, ws, st);
+        if constexpr (D == 64) {
+            if (r <= 32) return go<Shape<BF16, D, 1, 2, 2, 4, 2>>(a, cus, ws, st);
+        } else {
+            if (r <= 32) return go<Shape<BF16, D, 2, 1, 2, 2, 2>>(a, cus, ws, st);
+        }
+        return go<Shape<BF16, D, 1, 4, 1, 3, 3>>(a, cus, ws, st);
     }
 }
 
@@ -933,7 +1003,7 @@ hipError_t heads(const AttnArgs& a, int D, int max_new, int cus, uint8_t* ws, hi
 }  // namespace
 
 size_t attn_part_bytes(int cus) {
-    return (size_t)cus * (MAX_GRID * DESC * 4 + 2 * sizeof(float) * MAX_PART);
+    return desc_bytes(cus) + (size_t)cus * 2 * sizeof(float) * MAX_PART;
 }
 
 hipError_t launch_attn(const AttnArgs& a, bool bf16, int D, int max_new, int cus, uint8_t* ws,

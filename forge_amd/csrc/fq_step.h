@@ -57,8 +57,9 @@ struct AttnArgs {
     int64_t table_stride;
     float* out;
     float* part;  // partial results of split items, attn_part_bytes
-    int* desc;    // one record per work-group
+    int* desc;    // of each work-group: the parts of an item that it begins and another ends; that item
     int grid;     // work-groups
+    bool whole;   // items are not cut
 };
 size_t attn_part_bytes(int cus);  // of the largest call
 hipError_t launch_attn(const AttnArgs& a, bool bf16, int D, int max_new, int cus, uint8_t* ws,

@@ -31,8 +31,8 @@ int check_cache(uint32_t type, const void* k, const void* v, int num_blocks, int
     if (num_blocks < 1 || !block_size_ok(block_size) ||
         (int64_t)num_blocks * block_size > INT32_MAX)
         return FQ_ERR_SHAPE;
-    // a wave's copy adds up to seven tokens to a 32-bit offset
-    if (sb < 0 || st < 0 || sh < 0 || st > (1 << 26)) return FQ_ERR_SHAPE;
+    // a wave's copy adds up to seven tokens to a 32-bit offset; strides are 32-bit factors
+    if (sb < 0 || st < 0 || sh < 0 || sb > INT32_MAX || st > (1 << 26) || sh > INT32_MAX) return FQ_ERR_SHAPE;
     if (!k || !v) return FQ_ERR_NULL;
     if (!aligned16(k) || !aligned16(v) || ((sb | st | sh) & 7)) return FQ_ERR_ALIGN;
     return FQ_OK;

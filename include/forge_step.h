@@ -24,8 +24,8 @@
  * Paged cache: keys and values are arrays of num_blocks blocks of block_size
  * tokens (a power of two, 16 .. 1024), element (block, token, kv head, d) at
  * block * stride_block + token * stride_token + head * stride_head + d, in
- * elements of cache_type; strides are multiples of 8 elements and the bases 16-byte
- * aligned.  The request's token n is in block block_table[b][n / block_size],
+ * elements of cache_type; strides are multiples of 8 elements below 2^31 (2^26 from
+ * token to token) and the bases 16-byte aligned.  The request's token n is in block block_table[b][n / block_size],
  * at n % block_size; a token's slot is its block * block_size plus that.
  * Values read from device memory are held to their ranges by the kernels: no
  * length, table entry, slot or parent leads to an access out of bounds.
