@@ -189,6 +189,7 @@ __device__ __forceinline__ uint64_t place_of(const AttnArgs& a, int page, int ke
 }
 
 constexpr int DESC = 4;       // ints of a work-group's record, beside the number of parts
+constexpr int MAX_ITEMS = 1024;  // work-groups at most
 constexpr int MAX_GRID = 3;   // work-groups to a CU at most,
 constexpr size_t MAX_PART = 2 * 128 * (128 + 2);  // and floats of a part of each of them
 
@@ -271,7 +272,7 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
         b = at * per;
         off = u0 - uni64(__shfl(upto - mine, at));
     }
-    int* desc = a.desc + a.grid + wg * DESC;
+    int* desc = a.desc + MAX_ITEMS + wg * DESC;
     // padding tokens
     {
         const int end = min(max(sload(a.cu + a.B), 0), a.N);
@@ -816,7 +817,6 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
 // Joins the parts of the items that are cut: two rows at a time by one wave or, where
 // an item has many parts, one row by the four waves of a work-group.
 constexpr int JOIN_WGS = 8;  // work-groups to a CU
-constexpr int MAX_ITEMS = 1024;
 constexpr int NARROW = 16;   // parts of an item that one wave joins
 
 template <int D, int RT>
@@ -830,33 +830,38 @@ __global__ __launch_bounds__(256) void attn_join(AttnArgs a) {
     __shared__ int s_count[4], s_most[4];
     __shared__ float s_acc[4][D + 1];
     const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6);
-    // the items, in the order of the work-groups that began them
-    int items = 0, most = 0;
-    for (int i0 = 0; i0 < a.grid; i0 += 256) {
-        const int i = i0 + tid;
-        Item x;
-        x.parts = i < a.grid ? a.desc[i] : 0;
-        x.w = i;
-        if (x.parts) {
-            const int* d = a.desc + a.grid + i * DESC;
-            x.t0 = d[0], x.nt = d[1], x.h = d[2], x.rt = d[3];
-        }
-        most = max(most, x.parts);
-        const uint64_t some = __ballot(x.parts > 0);
-        if (lane == 0) s_count[wave] = __popcll(some);
-        __syncthreads();
-        int at = items + __popcll(some & ((1ull << lane) - 1));
-        for (int v = 0; v < 4; ++v) {
-            at += v < wave ? s_count[v] : 0;
-            items += s_count[v];
-        }
-        if (x.parts) s_item[at] = x;
-        __syncthreads();
+    // the items, in the order of the work-groups that began them: thread i looks at
+    // the K next to each other from K i on
+    constexpr int K = MAX_ITEMS / 256;
+    int parts[K], most = 0, mine = 0;
+    int4 rec[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const int i = tid * K + k;
+        parts[k] = i < a.grid ? a.desc[i] : 0;
+        rec[k] = i < a.grid ? ((const int4*)(a.desc + MAX_ITEMS))[i] : int4{0, 0, 0, 0};
+        most = max(most, parts[k]);
+        mine += parts[k] > 0;
     }
-    for (int o = 32; o; o >>= 1) most = max(most, __shfl_xor(most, o));
+    int upto = mine;
+    for (int o = 1; o < 64; o <<= 1) {
+        const int v = __shfl_up(upto, o);
+        if (lane >= o) upto += v;
+        most = max(most, __shfl_xor(most, o));
+    }
+    if (lane == 63) s_count[wave] = upto;
     if (lane == 0) s_most[wave] = most;
     __syncthreads();
-    most = max(max(s_most[0], s_most[1]), max(s_most[2], s_most[3]));
+    int at = upto - mine, items = 0;
+    for (int v = 0; v < 4; ++v) {
+        at += v < wave ? s_count[v] : 0;
+        items += s_count[v];
+        most = max(most, s_most[v]);
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+        if (parts[k]) s_item[at++] = {parts[k], tid * K + k, rec[k].x, rec[k].y, rec[k].z, rec[k].w};
+    __syncthreads();
     const auto slot = [&](const Item& x, int p) {
         return a.part + (int64_t)(2 * (x.w + p) + (p == 0)) * PART;
     };
@@ -956,17 +961,17 @@ __global__ __launch_bounds__(256) void attn_join(AttnArgs a) {
     }
 }
 
-size_t desc_bytes(int cus) { return ((size_t)MAX_GRID * cus * (DESC + 1) * 4 + 255) & ~(size_t)255; }
+constexpr size_t DESC_BYTES = (size_t)MAX_ITEMS * (DESC + 1) * 4;
 
 template <class S>
 hipError_t go(AttnArgs a, int cus, uint8_t* ws, hipStream_t st) {
     a.grid = S::PC * cus;
     a.desc = (int*)ws;
-    a.part = (float*)(ws + desc_bytes(cus));
+    a.part = (float*)(ws + DESC_BYTES);
     // Where a request has few keys at most (by its table's columns), its items are not
     // cut, and there is nothing to join: six units take about as long as a second launch.
     a.whole = (int64_t)a.max_blocks << a.c.bs_log2 <= 6 * std::max(S::KU, 64);
-    if (a.grid > MAX_ITEMS) return hipErrorInvalidConfiguration;
+    a.grid = std::min(a.grid, MAX_ITEMS);
     hipLaunchKernelGGL(attn_kernel<S>, dim3(a.grid), dim3(64 * S::WAVES), S::LDS, st, a);
     if (!a.whole) hipLaunchKernelGGL((attn_join<S::D, S::RT>), dim3(JOIN_WGS * cus), dim3(256), 0, st, a);
     return hipGetLastError();
@@ -1003,7 +1008,7 @@ hipError_t heads(const AttnArgs& a, int D, int max_new, int cus, uint8_t* ws, hi
 }  // namespace
 
 size_t attn_part_bytes(int cus) {
-    return desc_bytes(cus) + (size_t)cus * 2 * sizeof(float) * MAX_PART;
+    return DESC_BYTES + (size_t)cus * 2 * sizeof(float) * MAX_PART;
 }
 
 hipError_t launch_attn(const AttnArgs& a, bool bf16, int D, int max_new, int cus, uint8_t* ws,
