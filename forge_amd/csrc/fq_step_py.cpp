@@ -245,7 +245,7 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
         auto* cu = static_cast<int32_t*>(required(a[5], "tree_attention: cu", at::kInt, {B + 1}, dev));
         auto* masks = static_cast<uint64_t*>(vec(a[6], "tree_attention: masks", at::kLong, {N}, dev));
         const Table t = table(a[3], "tree_attention: block_table", B, dev);
-        const int64_t hint = a[7] == Py_None ? N : std::min(integer(a[7]), N);
+        const int64_t hint = a[7] == Py_None ? (B ? (N + B - 1) / B : 0) : std::min(integer(a[7]), N);
         const double scale = a[8] == Py_None ? 1.0 / std::sqrt((double)D) : number(a[8]);
         at::Tensor out = at::empty({N, hq, D}, q.options());
         check(fq_tree_attention(static_cast<const float*>(q.data_ptr()), N > 1 ? q.stride(0) : hq * D, ln, cu, masks,

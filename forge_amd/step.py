@@ -17,7 +17,7 @@ They stand where the reference verifies drafted tokens
 fp32 as everywhere here and caches in fp16 or bf16.  All arithmetic runs in
 libforge_q.so (include/forge_step.h, which states the operators in full);
 nothing waits for the GPU, and no length is needed on the host but the sum of
-the new tokens.
+the new tokens.  examples/verify_step.py runs a small model through them.
 """
 from __future__ import annotations
 
@@ -27,6 +27,7 @@ import torch
 
 from . import _lib
 from .ops import _stream_ptr
+
 
 class StepPlan(NamedTuple):
     """What plan_step makes of a step (N tokens of B requests)."""
@@ -125,8 +126,8 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     before this step; cu, masks: plan_step's (masks None: chains, a token sees
     the ones before it and itself); the new tokens' keys and values are in the
     caches already.  A token sees all of its request's cached tokens.  max_new:
-    the most new tokens of one request where the caller knows it (speed only);
-    scale: D^-0.5 unless given."""
+    the most new tokens of one request where the caller knows it (it chooses how many
+    rows a tile has; without it their average is taken); scale: D^-0.5 unless given."""
     return _native().attention(q, k_cache, v_cache, block_table, lengths, cu, masks, max_new, scale,
                                _stream(q))
 
