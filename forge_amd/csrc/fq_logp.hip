@@ -15,9 +15,18 @@
 // all that is below it is out.  Past KEEP kept keys the top-th largest of a wave's
 // becomes its threshold.  At the end the waves' keys are ranked by counting.  Few
 // rows are split over several work-groups, whose results a second kernel joins.
+//
+// Bound: the bytes of the logits once where there are many rows of many tokens (501 x
+// 152064 fp32, top 20: 60 us, 5.0 TB/s; 48 us with top 0; a large copy runs at 5.2
+// TB/s), the vector units' work on 16-bit logits (1000 x 32000 bf16: 40 us, where
+// the bytes take 12), latency for few (5 x 32000 fp32: 11 us, one work-group a row).
+// No barrier lies between a wave's chunks, and a chunk's elements cost no test
+// against the row's end except in its last one: the loop is bound by instructions
+// where the logits come fast.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "fq_step.h"
 
@@ -29,10 +38,13 @@ constexpr int CHUNK = 64 * E;
 constexpr int MAXTOP = 64;
 constexpr int KEEP = 128;      // kept keys from which a wave prunes them
 constexpr int CAP = 2 * KEEP;  // and at most
-constexpr int MAX_SPLITS = 16;
+constexpr int MAX_SPLITS = 32;
+constexpr int MAX_KEYS = 256;  // of a row's splits together
 constexpr float LOWEST = -3.402823466e38f;
 constexpr float LOG2E = 1.44269504088896341f;
 
+typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+typedef uint64_t k2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u4a __attribute__((ext_vector_type(4), aligned(2)));
 typedef uint32_t u4b __attribute__((ext_vector_type(4), aligned(4)));
 
@@ -57,14 +69,37 @@ __device__ __forceinline__ float below_value(uint32_t order) {
 struct Stat {
     float m, s, t;
 };
-// (the differences are held finite: a lane that has seen nothing has m = LOWEST)
-__device__ __forceinline__ Stat join(Stat a, Stat b) {
+constexpr Stat NOTHING = {LOWEST, 0.0f, 0.0f};
+
+// f over all lanes, in every lane: by turns within the rows of 16, then swaps of rows.
+template <class T, class F>
+__device__ __forceinline__ T over_wave(T x, F f) {
+    const auto turned = [&](auto n) {
+        return __builtin_bit_cast(
+            T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x120 + n.value, 0xF, 0xF, false));
+    };
+    x = f(x, turned(std::integral_constant<int, 8>()));
+    x = f(x, turned(std::integral_constant<int, 4>()));
+    x = f(x, turned(std::integral_constant<int, 2>()));
+    x = f(x, turned(std::integral_constant<int, 1>()));
+    const uint32_t u = __builtin_bit_cast(uint32_t, x);
+    const u2 p = __builtin_bit_cast(u2, __builtin_amdgcn_permlane16_swap(u, u, false, false));
+    const uint32_t p0 = p[0], p1 = p[1];  // (a bit cast of an element would take element 0)
+    x = f(__builtin_bit_cast(T, p0), __builtin_bit_cast(T, p1));
+    const uint32_t v = __builtin_bit_cast(uint32_t, x);
+    const u2 q = __builtin_bit_cast(u2, __builtin_amdgcn_permlane32_swap(v, v, false, false));
+    const uint32_t q0 = q[0], q1 = q[1];
+    return f(__builtin_bit_cast(T, q0), __builtin_bit_cast(T, q1));
+}
+// The lanes' statistics as one.  (The differences are held finite: a lane that has seen
+// nothing has m = LOWEST.)
+__device__ __forceinline__ Stat join(Stat a) {
+    const auto add = [](float x, float y) { return x + y; };
     Stat r;
-    r.m = fmaxf(a.m, b.m);
-    const float da = fmaxf(a.m - r.m, -1e30f), db = fmaxf(b.m - r.m, -1e30f);
-    const float ea = exp2f(da * LOG2E), eb = exp2f(db * LOG2E);
-    r.s = ea * a.s + eb * b.s;
-    r.t = ea * (a.t + da * a.s) + eb * (b.t + db * b.s);
+    r.m = over_wave(a.m, [](float x, float y) { return fmaxf(x, y); });
+    const float d = fmaxf(a.m - r.m, -1e30f), e = exp2f(d * LOG2E);
+    r.s = over_wave(e * a.s, add);
+    r.t = over_wave(e * (a.t + d * a.s), add);
     return r;
 }
 
@@ -81,13 +116,12 @@ struct Lds {
     int n[WAVES];
     uint32_t first[WAVES];         // the waves' thresholds after their first elements
     uint64_t buf[WAVES][CAP];      // the waves' kept keys
-    uint64_t key[WAVES * MAXTOP + 4];  // those to rank, one wave's after the other's, then 0
+    alignas(16) uint64_t key[WAVES * MAXTOP + 4];  // those to rank, one wave's after the other's, then 0
 };
 
-// Of one split: its statistics and its largest keys, in falling order.
+// Of one split: its statistics and its largest keys, in falling order, then 0.
 struct Part {
     Stat st;
-    int n;
     uint64_t key[MAXTOP];
 };
 
@@ -95,9 +129,10 @@ struct Part {
 __device__ __forceinline__ int above(const uint64_t* key, int n, uint64_t mine) {
     int r = 0;
 #pragma unroll 4
-    for (int i = 0; i < n; i += 4)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) r += key[i + j] > mine;
+    for (int i = 0; i < n; i += 4) {
+        const k2 a = *(const k2*)(key + i), b = *(const k2*)(key + i + 2);
+        r += (a[0] > mine) + (a[1] > mine) + (b[0] > mine) + (b[1] > mine);
+    }
     return r;
 }
 
@@ -190,23 +225,24 @@ __device__ __forceinline__ int index_of(int at, int i) {
 
 template <int TYPE>
 __device__ __forceinline__ void load(const LogpArgs& a, int64_t row, int at, int end, Run<TYPE>& r) {
-    if (at + CHUNK <= end) {
+    constexpr int RN = Run<TYPE>::N;
 #pragma unroll
-        for (int i = 0; i < E / Run<TYPE>::N; ++i) {
-            const int64_t x = row + index_of<TYPE>(at, i * Run<TYPE>::N);
-            if (TYPE == 0) r.v[i] = *(const u4b*)((const float*)a.x + x);
-            else r.v[i] = *(const u4a*)((const uint16_t*)a.x + x);
+    for (int i = 0; i < E / RN; ++i) {
+        const int x = index_of<TYPE>(at, i * RN);
+        if (x + RN <= end) {
+            if (TYPE == 0) r.v[i] = *(const u4b*)((const float*)a.x + row + x);
+            else r.v[i] = *(const u4a*)((const uint16_t*)a.x + row + x);
+            continue;
         }
-        return;
-    }
+        // the row's last run, and -inf behind it
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-        const int x = index_of<TYPE>(at, i);
-        if (TYPE == 0) {
-            r.v[i / 4][i % 4] = x < end ? ((const uint32_t*)a.x)[row + x] : 0xFF800000u;
-        } else {
-            const uint32_t h = x < end ? ((const uint16_t*)a.x)[row + x] : TYPE == 1 ? 0xFC00u : 0xFF80u;
-            r.v[i / 8][i % 8 / 2] = i & 1 ? r.v[i / 8][i % 8 / 2] | h << 16 : h;
+        for (int j = 0; j < RN; ++j) {
+            if (TYPE == 0) {
+                r.v[i][j % 4] = x + j < end ? ((const uint32_t*)a.x)[row + x + j] : 0xFF800000u;
+            } else {
+                const uint32_t h = x + j < end ? ((const uint16_t*)a.x)[row + x + j] : TYPE == 1 ? 0xFC00u : 0xFF80u;
+                r.v[i][j / 2] = j & 1 ? r.v[i][j / 2] | h << 16 : h;
+            }
         }
     }
 }
@@ -231,7 +267,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 16 ? 4 : 16 / WAVES) void logp
     float logit;  // (on their way early)
     if (a.splits == 1) read_target<TYPE, T>(a, m, target, logit);
     int n = 0;
-    Stat st = {LOWEST, 0.0f, 0.0f};
+    Stat st = NOTHING;
     float tau = __builtin_nanf("");  // (nothing is <= NaN: all is kept)
     Run<TYPE> next;
     if (beg < end) load<TYPE>(a, row, beg, end, next);
@@ -248,8 +284,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 16 ? 4 : 16 / WAVES) void logp
             const int q = (a.top + active - 1) / active;
             int r = 0;
             if (q == 1) {
-#pragma unroll
-                for (int o = 32; o; o >>= 1) mx = max(mx, (uint32_t)__shfl_xor((int)mx, o));
+                mx = over_wave(mx, [](uint32_t x, uint32_t y) { return max(x, y); });
                 r = lane;
             } else {
 #pragma unroll 8
@@ -286,14 +321,18 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 16 ? 4 : 16 / WAVES) void logp
             uint64_t in[E];
             int hits = 0;
 #pragma unroll
-            for (int i = 0; i < E; ++i) {
-                in[i] = __ballot(!(element<TYPE>(x, i) <= tau) && index_of<TYPE>(at, i) < end);
-                hits += __popcll(in[i]);
+            for (int i = 0; i < E; ++i) in[i] = __ballot(!(element<TYPE>(x, i) <= tau));
+            if (at + CHUNK > end) {
+#pragma unroll
+                for (int i = 0; i < E; ++i) in[i] &= __ballot(index_of<TYPE>(at, i) < end);
             }
+#pragma unroll
+            for (int i = 0; i < E; ++i) hits += __popcll(in[i]);
             const bool fits = n + hits <= CAP;
             if (fits && hits) {
 #pragma unroll
                 for (int i = 0; i < E; ++i) {
+                    if (!in[i]) continue;  // (uniform: most have none)
                     if (in[i] >> lane & 1)
                         buf[n + __popcll(in[i] & below(lane))] = key_of(element<TYPE>(x, i), index_of<TYPE>(at, i));
                     n += __popcll(in[i]);
@@ -324,10 +363,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 16 ? 4 : 16 / WAVES) void logp
         }
     }
     // --- the waves together ---
-    for (int o = 32; o; o >>= 1) {
-        const Stat b = {__shfl_xor(st.m, o), __shfl_xor(st.s, o), __shfl_xor(st.t, o)};
-        st = join(st, b);
-    }
+    st = join(st);
     if (TOP) {
         uint64_t last;
         if (n > MAXTOP / 2 && n > a.top) n = prune(buf, n, a.top, last);
@@ -347,16 +383,10 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 16 ? 4 : 16 / WAVES) void logp
         __syncthreads();
     }
     if (w > 0 && 64 * w >= max(total, a.J)) return;  // nothing to write for this wave
-    st = lane < WAVES ? l.st[lane] : Stat{LOWEST, 0.0f, 0.0f};
-#pragma unroll
-    for (int o = WAVES / 2; o; o >>= 1) {
-        const Stat b = {__shfl_xor(st.m, o), __shfl_xor(st.s, o), __shfl_xor(st.t, o)};
-        st = join(st, b);
-    }
-    st = {__shfl(st.m, 0), __shfl(st.s, 0), __shfl(st.t, 0)};
+    st = join(lane < WAVES ? l.st[lane] : NOTHING);
     Part* p = (Part*)a.ws + (int64_t)m * a.splits + sp;
     if (a.splits == 1) emit<TYPE, T>(a, m, st, target, logit);
-    else if (tid == 0) p->st = st, p->n = min(total, a.top);
+    else if (tid == 0) p->st = st;
     if (TOP && tid < total) {
         const uint64_t mine = l.key[tid];
         const int r = above(l.key, (total + 3) & ~3, mine);
@@ -365,29 +395,28 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 16 ? 4 : 16 / WAVES) void logp
             else p->key[r] = mine;
         }
     }
+    if (TOP && a.splits > 1 && tid >= total && tid < a.top) p->key[tid] = 0;
 }
 
 // The splits' statistics and keys.
 template <int TYPE>
 __global__ __launch_bounds__(256) void logp_join(LogpArgs a) {
-    __shared__ Stat s_st[MAX_SPLITS];
-    __shared__ uint64_t s_key[MAX_SPLITS * MAXTOP];
-    const int m = blockIdx.x, tid = threadIdx.x;
+    __shared__ alignas(16) uint64_t s_key[MAX_KEYS + 4];
+    const int m = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
     const Part* p = (const Part*)a.ws + (int64_t)m * a.splits;
     int target;
     float logit;
     read_target<TYPE, 256>(a, m, target, logit);
-    if (tid < a.splits) s_st[tid] = p[tid].st;
+    Stat st = lane < a.splits ? p[lane].st : NOTHING;
     const int n = a.splits * a.top;
-    for (int i = tid; i < (n + 3) / 4 * 4; i += 256) s_key[i] = i < n && i % a.top < p[i / a.top].n ? p[i / a.top].key[i % a.top] : 0;
+    for (int i = tid; i < n + 3; i += 256) s_key[i] = i < n ? p[i / a.top].key[i % a.top] : 0;
     __syncthreads();
-    Stat st = s_st[0];
-    for (int i = 1; i < a.splits; ++i) st = join(st, s_st[i]);
+    st = join(st);
     emit<TYPE, 256>(a, m, st, target, logit);
     for (int i = tid; i < n; i += 256) {
         const uint64_t mine = s_key[i];
         if (!mine) continue;
-        const int r = above(s_key, (n + 3) / 4 * 4, mine);
+        const int r = above(s_key, (n + 3) & ~3, mine);
         if (r < a.top) emit_top(a, m, st, mine, r);
     }
 }
@@ -404,12 +433,19 @@ hipError_t go(LogpArgs a, hipStream_t st) {
     return hipGetLastError();
 }
 
-// 16 waves to a CU, in as few work-groups as there are rows for; a row on several CUs
-// where its waves would take more than three chunks each.
+// 16 waves to a CU, in as few work-groups as there are rows for (us, 152064 fp32
+// logits, top 20, on 4 / 8 / 16 waves a row: 256 rows 66 / 47 / 47, 300 rows 74 / 66 /
+// 82, 600 rows 95 / 94 / 129; 1000 rows of 32000 bf16: 42 / 50 / 61).  Few rows take
+// several work-groups of 8 waves each where these would have more than six chunks
+// each otherwise (1 x 60000: 9.6 us for both kernels, unsplit 17; 64 x 152064: 23.4,
+// unsplit 42; 1 x 32000: 8.1 and the second launch, unsplit 10.0), as many as bring one
+// key to a thread of the join (1 x 152064, top 20: 15.6 with 256 keys, 19.2 with 512).
 template <int TYPE>
 hipError_t waves(LogpArgs a, int cus, hipStream_t st) {
-    const int chunks = (a.V + 16 * CHUNK - 1) / (16 * CHUNK);  // of one of 16 waves
-    a.splits = chunks > 3 ? std::max(1, std::min({cus / a.M, chunks, MAX_SPLITS})) : 1;
+    const int chunks = (a.V + 8 * CHUNK - 1) / (8 * CHUNK);  // of one of 8 waves
+    a.splits = std::min({cus / a.M, MAX_KEYS / std::max(a.top, 1), chunks, MAX_SPLITS});
+    if (chunks > 6 && a.splits > 1) return go<TYPE, 8>(a, st);
+    a.splits = 1;
     if (a.M <= cus) return go<TYPE, 16>(a, st);
     if (a.M <= 2 * cus) return go<TYPE, 8>(a, st);
     return go<TYPE, 4>(a, st);
