@@ -41,7 +41,7 @@ struct RopeArgs {
     uint16_t *k, *v;
     CacheView c;
 };
-hipError_t launch_rope(const RopeArgs& a, bool bf16, bool interleaved, int cus, hipStream_t st);
+hipError_t launch_rope(const RopeArgs& a, bool bf16, bool interleaved, hipStream_t st);
 
 struct AttnArgs {
     const float* q;

@@ -100,9 +100,6 @@ int fq_qk_norm_rope(const float* qkv, int64_t ld, int N, int hq, int hkv, int D,
     if (heads * D > INT32_MAX || ld < heads * D || N * heads >= (1 << 26)) return FQ_ERR_SHAPE;
     if (N == 0) return FQ_OK;
     if (!qkv || !positions || !slots || !q || (rot && table_rows && !table)) return FQ_ERR_NULL;
-    int dev = 0;
-    const int rd = device(&dev);
-    if (rd != FQ_OK) return rd;
     fq::RopeArgs a{};
     a.qkv = qkv;
     a.ld = ld;
@@ -124,7 +121,7 @@ int fq_qk_norm_rope(const float* qkv, int64_t ld, int N, int hq, int hkv, int D,
     a.v = static_cast<uint16_t*>(v_cache);
     a.c = {num_blocks, log2_of(block_size), stride_block, stride_token, stride_head};
     return done(fq::launch_rope(a, cache_type == FQ_TYPE_BF16, interleaved != 0,
-                                fq::device_info(dev).cus, static_cast<hipStream_t>(stream)));
+                                static_cast<hipStream_t>(stream)));
 }
 
 int fq_tree_attention(const float* q, int64_t ldq, const int32_t* lengths, const int32_t* cu,
