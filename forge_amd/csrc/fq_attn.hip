@@ -1,34 +1,47 @@
 // fq_attn.hip -- attention of drafted tokens over a paged cache and over their
 // ancestors in the draft.
 //
-// An item is one request, one kv head and up to 16 NR rows (a row: one token
+// An item is one request, one kv head and up to RT = 16 NR WR rows (a row: one token
 // with one of the G query heads that share the kv head).  The keys of all items,
-// in units of 32 WK, are shared out evenly over the work-groups, whatever the
-// requests' lengths: work-group w takes units [w span, (w + 1) span) and walks
-// the items that they belong to.  Every work-group finds its place from the
-// lengths alone (no plan, no length on the host).  An item cut by such a border
+// in units of 32 WK, and a fixed cost of each item are shared out evenly over the
+// work-groups, whatever the requests' lengths: work-group w takes units [w span, (w + 1)
+// span) and walks the items that they belong to.  Every work-group finds its place from
+// the lengths alone (no plan, no length on the host).  An item cut by such a border
 // leaves partial results (maximum, sum, unnormalised output), which a second
 // kernel joins, in the order of the keys, so that results repeat.
 //
-// A wave takes 32 keys at a time, its own in LDS, copied there straight from
-// the cache's pages two tiles ahead; the keys' buffer is refilled while the
-// values are used and the other way round.  Scores are S^T = K Q^T: keys along
-// the MFMA result's rows (four to a lane and tile of 16), queries along its
+// A tile is 32 keys and their values.  WR waves share one, each with 16 NR rows of
+// its own; the WK groups of a work-group take every WK-th.  Tiles are copied straight
+// from the cache's pages to LDS, one to three ahead, keys and values in rings of their
+// own: a tile's keys go while its values are still used.  Scores are S^T = K Q^T: keys
+// along the MFMA result's rows (four to a lane and tile of 16), queries along its
 // columns (one to a lane), so that a row's statistics are its lanes' own and
 // the exponentials are, in place, the second product's B operand: O^T = V^T P^T
 // with the contraction's keys in the order in which the lanes hold them.  V^T is read
 // from LDS by transposing reads (each 16 lanes take a 4 key x 16 element block).
+// The next tile's score products stand between the pieces of this one's softmax,
+// and the reference that the exponentials are taken against moves only where a
+// row's largest score leaves it by more than 2^LAG: the outputs are seldom rescaled.
 //
 // Queries are fp32 and keep their bits: against fp16 keys a query is hi + lo
 // in fp16 (22 bits, its row scaled by a power of two), against bf16 keys three
 // bf16 parts (24 bits).  The probabilities take the same two or three parts,
 // in fp16 scaled by 2^11 (so that parts down to 2^-35 of the row's largest
-// count); statistics and sums are fp32.
+// count); statistics and sums are fp32.  So the matrix work is two or three times
+// that of 16-bit queries.
 //
 // Rows and keys outside the lengths cost no branch in the common tile: only
 // tiles that reach past the cached tokens mask their scores, and there values that
 // are not finite are taken out of the product (a masked key's 0 times NaN
 // would reach rows that do not see it) and put back into the rows that see them.
+//
+// Bound: the caches' bytes where a tile has few rows, the waves' instructions (the
+// products in parts, exponentials and splits) where it has many.  Kernel + join, us, keys
+// and values of D = 128, a large copy at 5.2 TB/s: 32 requests of 8190 keys, 8 kv heads
+// x 4, fp16 (1.07 GB, 206 us at that rate, 164 at what reads alone reach): 1 new token
+// 150 + 7, 8 155 + 9, 16 169 + 13, 32 233 + 17, 64 341 + 23 (matrix work in
+// parts: 180); 48 of 2001 keys, 4 x 7, bf16, one token 34 + 7; one of 131000, 13 tokens,
+// 4 x 7, bf16 103 + 11 (matrix work 60); one of 333 keys 12.2, uncut.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -188,9 +201,9 @@ __device__ __forceinline__ uint64_t place_of(const AttnArgs& a, int page, int ke
     return 2 * ((uint64_t)pg * (uint32_t)a.c.sb + (uint64_t)in * (uint32_t)a.c.st);
 }
 
-constexpr int DESC = 4;       // ints of a work-group's record, beside the number of parts
+constexpr int DESC = 4;          // ints of a work-group's record, beside the number of parts
 constexpr int MAX_ITEMS = 1024;  // work-groups at most
-constexpr int MAX_GRID = 3;   // work-groups to a CU at most,
+constexpr int MAX_GRID = 3;      // work-groups to a CU at most,
 constexpr size_t MAX_PART = 2 * 128 * (128 + 2);  // and floats of a part of each of them
 
 // WR x WK waves: each group of WR shares tiles of 32 keys, each of its waves
@@ -232,7 +245,6 @@ struct Shape {
     static_assert(PC * (LDS + 8 * WK * (RT + 1) + 64) <= 160 * 1024, "LDS");
     static_assert(PC <= MAX_GRID && (size_t)PC * PART <= MAX_PART, "workspace");
 };
-
 
 template <class S>
 __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void attn_kernel(AttnArgs a) {
@@ -815,7 +827,8 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
 }
 
 // Joins the parts of the items that are cut: two rows at a time by one wave or, where
-// an item has many parts, one row by the four waves of a work-group.
+// an item has more than NARROW parts, one row by the four waves of a work-group (768
+// items of 4 parts: 17 us, 55 the second way; 8 of 96 parts: 11 us, 43 the first way).
 constexpr int JOIN_WGS = 8;  // work-groups to a CU
 constexpr int NARROW = 16;   // parts of an item that one wave joins
 
@@ -969,7 +982,9 @@ hipError_t go(AttnArgs a, int cus, uint8_t* ws, hipStream_t st) {
     a.desc = (int*)ws;
     a.part = (float*)(ws + DESC_BYTES);
     // Where a request has few keys at most (by its table's columns), its items are not
-    // cut, and there is nothing to join: six units take about as long as a second launch.
+    // cut, and there is nothing to join: six units take about as long as a second launch
+    // (one of 333 keys, D = 64: 12.2 us, cut 10.1 + 5.6; 64 of 370, one token: 23.1, cut
+    // 25.8 + 6.6; 8 of 340, 8 tokens: 21.1, cut 15.3 + 6.2).
     a.whole = (int64_t)a.max_blocks << a.c.bs_log2 <= 6 * std::max(S::KU, 64);
     a.grid = std::min(a.grid, MAX_ITEMS);
     hipLaunchKernelGGL(attn_kernel<S>, dim3(a.grid), dim3(64 * S::WAVES), S::LDS, st, a);
@@ -979,13 +994,29 @@ hipError_t go(AttnArgs a, int cus, uint8_t* ws, hipStream_t st) {
 
 template <bool BF16, int D>
 hipError_t rows(const AttnArgs& a, int max_new, int cus, uint8_t* ws, hipStream_t st) {
+    // By the rows of an item: few rows take waves with keys of their own, which wait for
+    // nobody, more rows waves that share a tile's copies.  Small work-groups, several to a
+    // CU, each keeping step by itself, hide each other's waits.  Kernel and join, us,
+    // 16 requests of 4090 keys, 8 kv heads x 4, fp16:
+    //                 16 rows                        32 rows
+    //   D = 64    29.0, <1, 4, 1, 3, 3> 36.7    32.4, <1, 4, 1, 3, 3> 37.3
+    //   D = 96    38.4, 43.4                    41.0, 43.9
+    //   D = 128   44.6, 51.6 (<2, 1, 2, 2, 2>   49.3, 51.8
+    //             47.0)
+    //   D = 256   90.3, <1, 4, 1, 4, 1> 102     -
+    //   D = 128, 36 to 64 rows: 53 to 56, <2, 4, 1, 4, 2> 76.
+    // The kernel alone, 32 requests of 8190 keys, D = 128: 64 rows 169, <2, 2, 2, 4, 1>
+    // 207; 128 rows, fp16 233, <1, 4, 1, 4, 2> 227, <2, 4, 1, 4, 2> 219 (but 65 against
+    // 63 at 16 requests of 4090), <1, 8, 1, 8, 1> 286, <2, 4, 2, 4, 1> 265; bf16 233 to
+    // 245, <1, 4, 1, 4, 2> 245 to 278, <2, 4, 1, 4, 2> 283, <1, 8, 1, 8, 1> 345.
+    // D = 64, 32 rows, one request of 333 keys: <1, 2, 2, 4, 2> 13.7, <2, 1, 2, 2, 2>
+    // 19.5, <2, 1, 4, 2, 1> 15.0.
     const int64_t r = (int64_t)max_new * a.G;
     if constexpr (D == 256) {
         if (r <= 16) return go<Shape<BF16, D, 1, 1, 2, 2, 1>>(a, cus, ws, st);
         return go<Shape<BF16, D, 1, 4, 1, 4, 1>>(a, cus, ws, st);
     } else {
-        constexpr int N = D == 64 ? 4 : 2;
-        if (r <= 16) return go<Shape<BF16, D, 1, 1, N, 2, 2>>(a, cus, ws, st);
+        if (r <= 16) return go<Shape<BF16, D, 1, 1, 2, 2, 2>>(a, cus, ws, st);
         if constexpr (D == 64) {
             if (r <= 32) return go<Shape<BF16, D, 1, 2, 2, 4, 2>>(a, cus, ws, st);
         } else {
