@@ -39,9 +39,9 @@
 // products in parts, exponentials and splits) where it has many.  Kernel + join, us, keys
 // and values of D = 128, a large copy at 5.2 TB/s: 32 requests of 8190 keys, 8 kv heads
 // x 4, fp16 (1.07 GB, 206 us at that rate, 164 at what reads alone reach): 1 new token
-// 150 + 7, 8 155 + 9, 16 169 + 13, 32 233 + 17, 64 341 + 23 (matrix work in
-// parts: 180); 48 of 2001 keys, 4 x 7, bf16, one token 34 + 7; one of 131000, 13 tokens,
-// 4 x 7, bf16 103 + 11 (matrix work 60); one of 333 keys 12.2, uncut.
+// 153 + 8, 8 151 + 9, 16 166 + 13, 32 228 + 15, 64 332 + 22 (matrix work in
+// parts: 180); 48 of 2001 keys, 4 x 7, bf16, one token 33 + 7; one of 131000, 13 tokens,
+// 4 x 7, bf16 99 + 10 (matrix work 60); one of 333 keys 12.5, uncut.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -1009,8 +1009,8 @@ hipError_t rows(const AttnArgs& a, int max_new, int cus, uint8_t* ws, hipStream_
     //             47.0)
     //   D = 256   90.3, <1, 4, 1, 4, 1> 102     -
     //   D = 128, 36 to 64 rows: 53 to 56, <2, 4, 1, 4, 2> 76.
-    // The kernel alone, 32 requests of 8190 keys, D = 128: 64 rows 169, <2, 2, 2, 4, 1>
-    // 207; 128 rows, fp16 233, <1, 4, 1, 4, 2> 227, <2, 4, 1, 4, 2> 219 (but 65 against
+    // The kernel alone, 32 requests of 8190 keys, D = 128: 64 rows 166, <2, 2, 2, 4, 1>
+    // 207; 128 rows, fp16 228 to 233, <1, 4, 1, 4, 2> 227, <2, 4, 1, 4, 2> 219 (but 65 against
     // 63 at 16 requests of 4090), <1, 8, 1, 8, 1> 286, <2, 4, 2, 4, 1> 265; bf16 233 to
     // 245, <1, 4, 1, 4, 2> 245 to 278, <2, 4, 1, 4, 2> 283, <1, 8, 1, 8, 1> 345.
     // D = 64, 32 rows, one request of 333 keys: <1, 2, 2, 4, 2> 13.7, <2, 1, 2, 2, 2>
