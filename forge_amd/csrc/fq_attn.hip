@@ -193,10 +193,14 @@ __device__ __forceinline__ uint32_t shifted(uint64_t m, int n) {
     return n >= 32 || n <= -64 ? 0u : n >= 0 ? (uint32_t)m << n : (uint32_t)(m >> -n);
 }
 
-// Where a token lies in a cache whose page (block) that is, in bytes.  (Strides are below
-// 2^31 elements: 32-bit factors.)
+// Whether a page is none of the cache's blocks: its keys are seen by nobody.
+__device__ __forceinline__ bool no_block(const AttnArgs& a, int page) {
+    return (uint32_t)page >= (uint32_t)a.c.num_blocks;
+}
+// Where a token lies in a cache whose page (block) that is, in bytes (where it is none, in
+// the last: copied and masked).  (Strides are below 2^31 elements: 32-bit factors.)
 __device__ __forceinline__ uint64_t place_of(const AttnArgs& a, int page, int key) {
-    const uint32_t pg = min((uint32_t)max(page, 0), (uint32_t)a.c.num_blocks - 1);
+    const uint32_t pg = min((uint32_t)page, (uint32_t)a.c.num_blocks - 1);
     const uint32_t in = (uint32_t)key & ((1u << a.c.bs_log2) - 1);
     return 2 * ((uint64_t)pg * (uint32_t)a.c.sb + (uint64_t)in * (uint32_t)a.c.st);
 }
@@ -379,12 +383,22 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
                 for (int hf = 0; hf < 2; ++hf) page[hf] = sload(table + (key_of(i, hf) >> a.c.bs_log2));
             };
             uint64_t at_k[2], at_v[2];  // of the tiles whose keys, values are copied next
+            uint32_t highest = 0;       // of the pages placed so far (unsigned: -1 is above all blocks)
             const auto place = [&](int i) {
 #pragma unroll
                 for (int hf = 0; hf < 2; ++hf) {
                     at_v[hf] = at_k[hf];
                     at_k[hf] = place_of(a, page[hf], key_of(i, hf));
+                    highest = max(highest, (uint32_t)page[hf]);
                 }
+            };
+            // The keys of a tile that lie in a block.
+            const auto there = [&](int i) {
+                uint32_t m = ~0u;
+#pragma unroll
+                for (int hf = 0; hf < 2; ++hf)
+                    if (no_block(a, sload(table + (key_of(i, hf) >> a.c.bs_log2)))) m &= ~(0xFFFFu << (16 * hf));
+                return m;
             };
             const int64_t step = 2 * ROWS * a.c.st;  // bytes from copy to copy
             const auto copy_k = [&](int stage) {
@@ -583,16 +597,18 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
                         copy_share(i + NS < n, stage, true, stage ? stage - 1 : NS - 1);
                     }
                 }
-                const bool tail = careful || key0 + KT > len;
+                const bool holes = no_block(a, (int)highest);
+                const bool tail = careful || holes || key0 + KT > len;
                 float mul[NR];
 #pragma unroll
                 for (int c = 0; c < NR; ++c) mul[c] = rs[c];
                 if (tail) {
                     const int old = len - key0, all = keys - key0;
+                    const uint32_t in = holes ? there(i) : ~0u;
 #pragma unroll
                     for (int c = 0; c < NR; ++c) {
                         mul[c] = 1.0f;
-                        const uint32_t see = seen(mask[c], old, all) >> (4 * g);
+                        const uint32_t see = (seen(mask[c], old, all) & in) >> (4 * g);
 #pragma unroll
                         for (int sub = 0; sub < 2; ++sub)
 #pragma unroll
@@ -744,8 +760,10 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
 #pragma unroll 1
                 for (int key = kbeg; key < kbeg + n * KU && key < keys; ++key) {
                     const int at = (key - kbeg) % KU, key0 = key - at;
-                    if (at >= KT || !(careful || key0 + KT > len)) continue;
-                    const uint8_t* v = vb + place_of(a, sload(table + (key >> a.c.bs_log2)), key);
+                    if (at >= KT) continue;
+                    const int pg = sload(table + (key >> a.c.bs_log2));
+                    if (no_block(a, pg) || !(careful || no_block(a, (int)highest) || key0 + KT > len)) continue;
+                    const uint8_t* v = vb + place_of(a, pg, key);
                     bool see[NR];
 #pragma unroll
                     for (int c = 0; c < NR; ++c) see[c] = seen(mask[c], len - key0, keys - key0) >> at & 1;

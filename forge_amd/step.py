@@ -125,7 +125,9 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     q: fp32 [N, hq, D], tokens any distance apart; lengths: int32 [B], the cached tokens
     before this step; cu, masks: plan_step's (masks None: chains, a token sees
     the ones before it and itself); the new tokens' keys and values are in the
-    caches already.  A token sees all of its request's cached tokens.  max_new:
+    caches already.  A token sees all of its request's cached tokens; what a table entry
+    that is no block of the caches (-1: plan_step had none left) would hold is not
+    there, so that info[1] of the plan, where it is not 0, says that answers lack it.  max_new:
     the most new tokens of one request where the caller knows it (it chooses how many
     rows a tile has; without it their average is taken); scale: D^-0.5 unless given."""
     return _native().attention(q, k_cache, v_cache, block_table, lengths, cu, masks, max_new, scale,

@@ -28,7 +28,9 @@
  * token to token) and the bases 16-byte aligned.  The request's token n is in block block_table[b][n / block_size],
  * at n % block_size; a token's slot is its block * block_size plus that.
  * Values read from device memory are held to their ranges by the kernels: no
- * length, table entry, slot or parent leads to an access out of bounds.
+ * length, table entry, slot or parent leads to an access out of bounds.  A table entry
+ * outside 0 .. num_blocks-1 (fq_plan_step enters -1 where blocks ran out) is no block: no
+ * token has a slot in it, and fq_tree_attention's tokens see no key of it.
  *
  * fq_tree_attention and fq_token_logprobs keep partial results in the
  * library's per-stream workspace; fq_reserve_step sizes it for calls under
@@ -93,8 +95,8 @@ int fq_qk_norm_rope(const float* qkv, int64_t ld, int N, int hq, int hkv, int D,
 /* out[n][h] = softmax(scale q[n][h] . k) v over the keys that token n sees, query
  * head h reading kv head h / (hq / hkv): all cached tokens of its request, and
  * of its new tokens (in the cache too) those of its mask's bits or, with masks
- * NULL, those up to itself.  Zeros for a token that sees nothing, or whose keys
- * all score -inf, and for padding.  Keys that a token does not see have no part
+ * NULL, those up to itself, where the table has a block for them.  Zeros for a token that sees
+ * nothing, or whose keys all score -inf, and for padding.  Keys that a token does not see have no part
  * in its result, whatever they hold.  q rows (tokens) are ldq floats apart, out is
  * [N][hq][D]; D is 64, 96, 128 or 256.  max_new: the most new tokens of a
  * request, as far as known (the tiles' size goes by it, results do not). */

@@ -1,0 +1,113 @@
+"""Step operators at the edges of what device memory may hold: block tables with
+entries that are no block."""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from forge_amd import step
+from test_gpu_step import U, Case, ints
+
+pytestmark = pytest.mark.gpu
+
+NONE = [-1, -2 ** 31, 2 ** 31 - 1, 2 ** 30]  # (and the number of blocks) are no blocks
+
+
+def plain(c, scale=None):
+    """fp64 [N, hq, D]: token by token over the keys that it sees and that lie in a block;
+    a key that scores -inf has no weight, and where none has any the row is zeros."""
+    scale = c.D ** -0.5 if scale is None else scale
+    nb, bs, hkv = c.k.shape[:3]
+    hq = c.q.shape[1]
+    out = torch.zeros((c.N, hq, c.D), dtype=torch.float64)
+    for b, ln in enumerate(c.lengths):
+        t0, n = c.cu[b], c.cu[b + 1] - c.cu[b]
+        keys = min(ln + n, c.table.shape[1] * bs)
+        pages = c.table[b, :-(-keys // bs)].long()
+        fine = (pages >= 0) & (pages < nb)
+        there = fine.repeat_interleave(bs)[:keys]
+        k, v = (x[torch.where(fine, pages, 0)].flatten(0, 1)[:keys].double() for x in (c.k, c.v))
+        j = torch.arange(keys) - ln  # a key's number among the new tokens
+        for i in range(n):
+            if c.masks is None:
+                see = j <= i
+            else:
+                m = int(c.masks[t0 + i])
+                see = (j < 0) | torch.tensor([0 <= x < 64 and m >> x & 1 == 1 for x in j.tolist()], dtype=torch.bool)
+            see = see & there
+            if not see.any():
+                continue
+            kk, vv = (x[see].repeat_interleave(hq // hkv, 1) for x in (k, v))
+            s = (c.q[t0 + i].double()[None] * kk).sum(-1) * scale
+            top = s.amax(0)
+            w = torch.where(s == -math.inf, torch.zeros_like(s), torch.exp(s - top))
+            total = w.sum(0)
+            o = (w[..., None] * vv).sum(0) / torch.where(total == 0, 1.0, total)[:, None]
+            out[t0 + i] = torch.where(torch.isnan(s).any(0) | (top == math.inf), math.nan, o.T).T
+    return out
+
+
+def near(c, out, want, scale=None):
+    # as Case.check: scores off by at most 2^-20 of |q| |k|, probabilities by twice
+    # that and the roundings of the exponential, of the parts and of the keys' sums
+    def fine(x):
+        return torch.nan_to_num(x.float(), 0.0, 0.0, 0.0)
+    ds = 2.0 ** -20 * (scale or c.D ** -0.5) * float(c.q.norm(dim=-1).max()) * float(fine(c.k).norm(dim=-1).max())
+    most = max(a + b for a, b in zip(c.lengths, c.new))
+    tol = float(fine(c.v).abs().max()) * (2 * ds + (32 + most / 16) * U)
+    out = out.double().cpu()
+    assert bool((torch.isnan(out) == torch.isnan(want)).all())
+    err = float(torch.nan_to_num(out - want, 0.0, 0.0, 0.0).abs().max())
+    assert err <= tol, (err, tol)
+
+
+# (up to 16, 32 and 64 rows to a tile; whole and cut items)
+SHAPES = [(64, 2, 1), (64, 2, 5), (64, 2, 20), (128, 2, 3), (128, 2, 7), (128, 2, 24), (96, 1, 9), (256, 2, 3), (256, 2, 11)]
+
+
+@pytest.mark.parametrize("D, hkv, new", SHAPES)
+@pytest.mark.parametrize("cache, tree", [(torch.float16, True), (torch.bfloat16, False)])
+@pytest.mark.parametrize("what", [5.0, math.nan])
+def test_keys_without_a_block_are_not_seen(D, hkv, new, cache, tree, what):
+    for lengths, bs, holes in (([70, 33], 16, [(0, 1), (1, 0)]),           # one in the context, one the first
+                               ([160, 9], 32, [(0, 0), (0, 3), (0, 5)]),   # the last: the new tokens'
+                               ([3000, 700], 16, [(0, 0), (0, 100), (0, 101), (0, 150), (1, 43)]),
+                               ([130, 0], 16, [(1, x) for x in range(2)])):
+        c = Case(lengths, [new, max(1, new - 2)], 4 * hkv, hkv, D, cache=cache, bs=bs, tree=tree, seed=new)
+        nb = c.k.shape[0]
+        free = [int(c.table[b, x]) for b, x in holes]
+        for i, (b, x) in enumerate(holes):
+            c.table[b, x] = (NONE + [nb])[i % 5]
+        # what a clamp to the cache would read (blocks of nobody, or of the other request)
+        for p in (0, nb - 1):
+            if p in free or p not in c.table:
+                c.k[p], c.v[p] = what, what
+        near(c, c.run(max_new=new), plain(c))
+
+
+def test_a_request_whose_every_block_is_missing_gets_zeros():
+    c = Case([40, 50], [3, 2], 8, 2, 64, seed=2)
+    c.table[0] = -1
+    out = c.run()
+    assert not out[:3].any() and bool(out[3:].any())
+    near(c, out, plain(c))
+
+
+def test_tokens_that_found_no_block_take_no_part():
+    # the free blocks run out within the second request: its further tokens have no
+    # slot, and the first block, another request's, stays out of their attention
+    bs, hkv, hq, D, lengths, new = 16, 2, 8, 64, [16, 14], [4, 20]
+    g = torch.Generator().manual_seed(3)
+    k, v = step.paged_cache(4, bs, hkv, D)
+    k[:3], v[:3] = (torch.randn((3, bs, hkv, D), generator=g).cuda().half() for _ in range(2))
+    table = ints([[0, 9, 9], [2, 9, 9]])
+    plan = step.plan_step(ints(lengths), ints(new), table, ints([1]), bs, 24)
+    assert plan.info.tolist() == [1, 2] and table.tolist() == [[0, 1, 9], [2, -1, -1]]
+    assert plan.slots.tolist() == [16, 17, 18, 19] + [46, 47] + [-1] * 18
+    x = torch.randn((24, (hq + 2 * hkv) * D), generator=g).cuda()
+    q = step.qk_norm_rope(x, plan.positions, plan.slots, step.rope_table(64, D), k, v)
+    c = Case(lengths, new, hq, hkv, D)
+    c.q, c.k, c.v, c.table = q.cpu(), k.cpu(), v.cpu(), table.cpu()
+    near(c, step.tree_attention(q, k, v, table, ints(lengths), plan.cu), plain(c))
