@@ -151,10 +151,10 @@ __device__ __forceinline__ Request request(const AttnArgs& a, int c0, int c1, in
     Request r;
     r.t0 = min(max(c0, 0), a.N);
     r.nt = min(max(c1, r.t0), a.N) - r.t0;
-    r.len = max(len, 0);
-    // (no key lies beyond the table's columns)
+    // (no key, cached or new, lies beyond the table's columns)
     const int64_t most = (int64_t)a.max_blocks << a.c.bs_log2;
-    r.keys = (int)min((int64_t)r.len + r.nt, min(most, (int64_t)INT32_MAX - 4096));
+    r.keys = (int)min((int64_t)max(len, 0) + r.nt, min(most, (int64_t)INT32_MAX - 4096));
+    r.len = min(max(len, 0), r.keys);
     r.nu = (r.keys + KU - 1) / KU;
     r.rts = (int)(((int64_t)r.nt * a.G + RT - 1) / RT);
     r.cost = a.whole ? 1 : r.nu + OV;

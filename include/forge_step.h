@@ -30,7 +30,8 @@
  * Values read from device memory are held to their ranges by the kernels: no
  * length, table entry, slot or parent leads to an access out of bounds.  A table entry
  * outside 0 .. num_blocks-1 (fq_plan_step enters -1 where blocks ran out) is no block: no
- * token has a slot in it, and fq_tree_attention's tokens see no key of it.
+ * token has a slot in it, and fq_tree_attention's tokens see no key of it.  Nor are there
+ * slots or keys past the table's max_blocks columns, whatever the length.
  *
  * fq_tree_attention and fq_token_logprobs keep partial results in the
  * library's per-stream workspace; fq_reserve_step sizes it for calls under

@@ -1,5 +1,5 @@
 """Step operators at the edges of what device memory may hold: block tables with
-entries that are no block."""
+entries that are no block, lengths beyond a table."""
 from __future__ import annotations
 
 import math
@@ -111,3 +111,19 @@ def test_tokens_that_found_no_block_take_no_part():
     c = Case(lengths, new, hq, hkv, D)
     c.q, c.k, c.v, c.table = q.cpu(), k.cpu(), v.cpu(), table.cpu()
     near(c, step.tree_attention(q, k, v, table, ints(lengths), plan.cu), plain(c))
+
+
+@pytest.mark.parametrize("D, hkv, new", SHAPES)
+@pytest.mark.parametrize("tree", [False, True])
+def test_lengths_beyond_the_table_end_with_it(D, hkv, new, tree):
+    for cols, bs, lengths in ((3, 16, [200, 20]), (5, 16, [81, 10 ** 6]), (1, 16, [2 ** 31 - 1, 17]), (67, 16, [1071, 5000]),
+                              (3, 64, [191, 300])):
+        c = Case([min(n, cols * bs - 64) if cols * bs > 64 else 0 for n in lengths], [new, 2], 4 * hkv, hkv, D, bs=bs, tree=tree, seed=new)
+        g = torch.Generator().manual_seed(new)
+        nb = 2 * cols + 1
+        c.k, c.v = (torch.randn((nb, hkv, bs, D), generator=g).to(c.k.dtype).transpose(1, 2) for _ in range(2))
+        c.table = torch.randperm(nb, generator=g)[:2 * cols].view(2, cols).int()
+        c.lengths = lengths
+        out, want = c.run(max_new=new), plain(c)
+        c.lengths = [cols * bs - n for n in c.new]  # (the keys that there are)
+        near(c, out, want)
