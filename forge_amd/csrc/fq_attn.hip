@@ -138,6 +138,41 @@ __device__ __forceinline__ void split2(float x0, float x1, float minus1,
     }
 }
 
+// Makes split2's parts of a number all of one sign and none zero (where the first is not), so
+// that an infinite key's products with them add up to an infinity and not to NaN.  fp16: the
+// first part, a rounded one, gives a last place to the second.  bf16: the others, zero
+// where the number ends before them, become 2^-126 at least.  Of a first part that is
+// infinite (or NaN), all are it.
+template <bool BF16>
+__device__ __forceinline__ void one_sign(uint32_t (&p)[Parts<BF16>::N]) {
+    typedef uint16_t w2 __attribute__((ext_vector_type(2)));
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    const w2 first = __builtin_bit_cast(w2, p[0]), sign = first & (uint16_t)0x8000, mag = first & (uint16_t)0x7FFF;
+    const auto infinite = [&](w2 of) {
+        w2 r;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) r[i] = mag[i] >= (BF16 ? 0x7F80 : 0x7C00) ? first[i] : of[i];
+        return __builtin_bit_cast(uint32_t, r);
+    };
+    if constexpr (BF16) {
+#pragma unroll
+        for (int l = 1; l < Parts<BF16>::N; ++l) {
+            const w2 m = __builtin_bit_cast(w2, p[l]) & (uint16_t)0x7FFF;
+            w2 r;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) r[i] = mag[i] ? max(m[i], (uint16_t)0x0080) | sign[i] : 0;
+            p[l] = infinite(r);
+        }
+    } else {
+        w2 less;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) less[i] = (mag[i] - min(mag[i], (uint16_t)1)) | sign[i];
+        const h2 rest = __builtin_bit_cast(h2, p[1]) + (__builtin_bit_cast(h2, first) - __builtin_bit_cast(h2, less));
+        p[0] = infinite(less);
+        p[1] = infinite(__builtin_bit_cast(w2, rest));
+    }
+}
+
 // What a request brings.
 struct Request {
     int t0, nt, len;  // its first new token, how many, its cached tokens
@@ -516,6 +551,19 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
 #pragma unroll
                         for (int l = 0; l < NL; ++l) qf[c][s][l][i] = p[l];
                     }
+                if (!careful) continue;
+#pragma unroll
+                for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        uint32_t p[NL];
+#pragma unroll
+                        for (int l = 0; l < NL; ++l) p[l] = qf[c][s][l][i];
+                        one_sign<BF16>(p);
+#pragma unroll
+                        for (int l = 0; l < NL; ++l) qf[c][s][l][i] = p[l];
+                        __builtin_amdgcn_sched_barrier(0);  // (one after the other: few registers)
+                    }
             }
 
 #pragma unroll
@@ -726,8 +774,9 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
                 stage = stage1;
             }
 
-            // an infinite cached value times the two signs (or a zero) of a
-            // probability's parts is NaN: once more, with all values looked at
+            // an infinite cached key or value times the two signs (or a zero) of a query's
+            // or probability's parts is NaN: once more, with the queries' parts of one sign
+            // and all values looked at
             if (!careful) {
                 bool nan = false;
 #pragma unroll

@@ -1,5 +1,5 @@
 """Step operators at the edges of what device memory may hold: block tables with
-entries that are no block, lengths beyond a table."""
+entries that are no block, lengths beyond a table, keys that are infinite."""
 from __future__ import annotations
 
 import math
@@ -127,3 +127,27 @@ def test_lengths_beyond_the_table_end_with_it(D, hkv, new, tree):
         out, want = c.run(max_new=new), plain(c)
         c.lengths = [cols * bs - n for n in c.new]  # (the keys that there are)
         near(c, out, want)
+
+
+@pytest.mark.parametrize("D, hkv, new", SHAPES)
+@pytest.mark.parametrize("cache", [torch.float16, torch.bfloat16])
+def test_infinite_keys_score_as_they_do(D, hkv, new, cache):
+    # a key with an infinite element scores -inf, and has no weight, or +inf, whose
+    # softmax is NaN, by the sign of the query's element
+    for lengths in ([40, 3], [2000, 0]):
+        for at in (0, 17, lengths[0] - 1, lengths[0]):
+            c = Case(lengths, [new, 2], 4 * hkv, hkv, D, cache=cache, tree=True, seed=new)
+            p = int(c.table[0, at // 16])
+            c.k[p, at % 16, 0, 5] = math.inf
+            c.q[:, 0, 5] = c.q[:, 0, 5].abs()
+            c.q[:, 1, 5] = -c.q[:, 1, 5].abs()
+            want = plain(c)
+            assert bool(torch.isnan(want[:, 0]).any()) and bool(torch.isfinite(want[:, 1]).all())
+            near(c, c.run(max_new=new), want)
+
+
+def test_keys_that_all_score_minus_infinity_give_zeros():
+    c = Case([37], [3], 4, 2, 64, seed=4)
+    c.q = c.q.abs() + 0.1
+    c.k[torch.isfinite(c.k)] = -math.inf
+    assert not c.run().any()
