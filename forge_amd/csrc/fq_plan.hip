@@ -95,7 +95,8 @@ __global__ __launch_bounds__(WAVES * 64) void plan_kernel(PlanArgs a) {
                 const int64_t f = blk + (c - own.held);
                 e = f < a.n_free ? a.free_blocks[f] : -1;
             }
-            return e < 0 ? -1 : (int)(((unsigned)e << a.bs_log2) + (unsigned)(at & bs1));
+            // (of a block past what an int of slots reaches there is none)
+            return e < 0 || e > INT32_MAX >> a.bs_log2 ? -1 : (e << a.bs_log2) + (int)(at & bs1);
         };
         const auto put = [&](int i, int pos, int s) {
             if (tok + i < a.N) {

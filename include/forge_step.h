@@ -59,8 +59,9 @@ extern "C" {
  *                    missing blocks, up to its ceil((length + new) / block_size),
  *                    are taken from free_blocks [n_free] front to back in request
  *                    order and entered
- *   slots [N]        each token's slot; -1 for padding and where blocks or
- *                    columns of the table ran out
+ *   slots [N]        each token's slot; -1 for padding, where blocks or
+ *                    columns of the table ran out and where a block's slots pass
+ *                    the largest int
  *   positions [N]    length + depth in the draft (0 for padding)
  *   masks [N]        (with parents only) bit j: the token is, or descends from,
  *                    token j of its request

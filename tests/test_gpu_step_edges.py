@@ -151,3 +151,12 @@ def test_keys_that_all_score_minus_infinity_give_zeros():
     c.q = c.q.abs() + 0.1
     c.k[torch.isfinite(c.k)] = -math.inf
     assert not c.run().any()
+
+
+def test_slots_past_the_largest_int_are_none():
+    # (a block's number times the block's size does not fit: another block's slot)
+    table = ints([[2 ** 27, 3], [2 ** 31 - 1, 2 ** 27 - 1]])
+    plan = step.plan_step(ints([14, 3]), ints([4, 2]), table, ints([2 ** 28 + 1]), 16, 6)
+    assert plan.slots.tolist() == [-1, -1, -1, -1, -1, -1]
+    plan = step.plan_step(ints([14, 17]), ints([1, 2]), table, ints([]), 16, 3)
+    assert plan.slots.tolist() == [-1, (2 ** 27 - 1) * 16 + 1, (2 ** 27 - 1) * 16 + 2]
