@@ -160,3 +160,16 @@ def test_slots_past_the_largest_int_are_none():
     assert plan.slots.tolist() == [-1, -1, -1, -1, -1, -1]
     plan = step.plan_step(ints([14, 17]), ints([1, 2]), table, ints([]), 16, 3)
     assert plan.slots.tolist() == [-1, (2 ** 27 - 1) * 16 + 1, (2 ** 27 - 1) * 16 + 2]
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two devices")
+def test_calls_go_to_the_tensors_device():
+    from test_gpu_step import state_of, step_of
+    want = step_of(state_of(5))
+    there = [x.to("cuda:1") for x in state_of(5)]
+    there[7], there[8] = (x.transpose(1, 2).contiguous().transpose(1, 2) for x in there[7:9])
+    assert torch.cuda.current_device() == 0
+    got = step_of(there)
+    assert torch.cuda.current_device() == 0
+    torch.cuda.synchronize(1)
+    assert all(x.device.index == 1 and torch.equal(x.cpu(), y.cpu()) for x, y in zip(got, want))
