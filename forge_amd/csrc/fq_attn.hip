@@ -76,19 +76,6 @@ __device__ __forceinline__ int sload(const int* p) {
 }
 __device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
-// Memory straight into LDS: 16 bytes a lane, from base + off to lds + 16 lane (lds
-// in M0).  The base passes through a scalar move within the block, and four states
-// follow: a vector instruction (a spilled scalar register comes back by one)
-// may have written base or M0 just before, and a load must not read such a
-// register within five states, which the compiler sees to for its own loads only.
-__device__ __forceinline__ void copy16(uint32_t off, const uint8_t* base, uint32_t lds) {
-    uint64_t at;
-    asm volatile("s_mov_b64 %0, %2\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, %0"
-                 : "=&s"(at)
-                 : "v"(off), "s"(base), "{m0}"(lds)
-                 : "memory");
-}
-
 // All waves' LDS accesses are done (their stores to memory may be on their way).
 __device__ __forceinline__ void lds_barrier() {
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -442,7 +429,7 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
                     const uint8_t* from = kb + at_k[hf];
 #pragma unroll
                     for (int j = 0; j < J; ++j, from += step)
-                        copy16(ksrc, from, gbase + stage * S::STAGE + (hf * J + j) * S::KSTEP);
+                        dma16s(ksrc, from, gbase + stage * S::STAGE + (hf * J + j) * S::KSTEP);
                 }
             };
             const auto copy_v = [&](int stage) {
@@ -451,7 +438,7 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
                     const uint8_t* from = vb + at_v[hf];
 #pragma unroll
                     for (int j = 0; j < J; ++j, from += step)
-                        copy16(vsrc, from, gbase + stage * S::STAGE + S::KTILE + (hf * J + j) * S::VSTEP);
+                        dma16s(vsrc, from, gbase + stage * S::STAGE + S::KTILE + (hf * J + j) * S::VSTEP);
                 }
             };
             // This wave's share of a tile's keys and of the one before's values: copies wr,
@@ -470,9 +457,9 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
                     const uint64_t in = LOW ? (uint64_t)((c0 % J) * step) : 0;
                     const int over = WR <= NI ? c0 : isv ? -NI : 0;  // copies past wr's
                     if (!isv) {
-                        if (ks) copy16(ksrc, kw + ((upper ? at_k[1] : at_k[0]) + in), kto + over * S::KSTEP);
+                        if (ks) dma16s(ksrc, kw + ((upper ? at_k[1] : at_k[0]) + in), kto + over * S::KSTEP);
                     } else if (vs) {
-                        copy16(vsrc, vw + ((upper ? at_v[1] : at_v[0]) + in), vto + over * S::VSTEP);
+                        dma16s(vsrc, vw + ((upper ? at_v[1] : at_v[0]) + in), vto + over * S::VSTEP);
                     }
                 }
             };

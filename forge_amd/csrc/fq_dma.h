@@ -21,11 +21,17 @@ __device__ __forceinline__ void dma16(const uint8_t* g, uint32_t lds) {
 // The same copy from base + off: base wave-uniform (a scalar register pair),
 // off a 32-bit per-lane byte offset, so a loop that moves base keeps the
 // per-lane part in one register and its address arithmetic on the scalar
-// unit.
+// unit.  Base and M0 pass through scalar moves within the block: a vector
+// instruction may have written either just before (as a spilled scalar register's
+// return does), and a load must not read such a register within five states, which
+// the compiler sees to for its own loads only.  A scalar move waits for it, what
+// the move wrote may be read at once, and M0 after one state, the second move.
 __device__ __forceinline__ void dma16s(uint32_t off, const uint8_t* base, uint32_t lds) {
-    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
-                 :
-                 : "v"(off), "s"(base), "{m0}"(lds)
+    uint64_t at;
+    uint32_t m0;
+    asm volatile("s_mov_b32 m0, %4\n\ts_mov_b64 %0, %3\n\tglobal_load_lds_dwordx4 %2, %0"
+                 : "=&s"(at), "=&{m0}"(m0)
+                 : "v"(off), "s"(base), "s"(lds)
                  : "memory");
 }
 
