@@ -8,6 +8,7 @@ is disabled (-packed-fp32-ops) for every HIP translation unit.
 from __future__ import annotations
 
 import os
+import shutil
 import subprocess
 import sys
 from concurrent.futures import ThreadPoolExecutor
@@ -53,17 +54,30 @@ def _compile(src: str) -> str:
 
 def _binding() -> None:
     """forge_amd/_step.so: the step operators' host side over torch tensors, a plain
-    CPython extension that calls the library's C ABI."""
+    CPython extension that calls the library's C ABI.  Without torch, its or Python's
+    headers or g++ it is left out (and one of an earlier library removed):
+    forge_amd.step is not there then, the library is."""
     import sysconfig
 
-    import torch
-    from torch.utils import cpp_extension
+    try:
+        import torch
+        from torch.utils import cpp_extension
+        include = [*cpp_extension.include_paths(), sysconfig.get_paths()["include"]]
+        missing = next((h for h in ("torch/csrc/autograd/python_variable.h", "Python.h")
+                        if not any(os.path.exists(os.path.join(p, h)) for p in include)),
+                       None if shutil.which("g++") else "g++")
+    except ImportError:
+        missing = "torch"
+    if missing:
+        if os.path.exists(STEP):
+            os.remove(STEP)
+        print(f"no {missing}: {os.path.basename(STEP)} (forge_amd.step) is not built")
+        return
     lib = os.path.join(os.path.dirname(torch.__file__), "lib")
     tmp = STEP + ".tmp"
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-           *(f"-isystem{p}" for p in cpp_extension.include_paths()),
-           f"-isystem{sysconfig.get_paths()['include']}", os.path.join(CSRC, "fq_step_py.cpp"),
+           *(f"-isystem{p}" for p in include), os.path.join(CSRC, "fq_step_py.cpp"),
            "-o", tmp, f"-L{HERE}", "-l:libforge_q.so", "-Wl,-rpath,$ORIGIN", f"-L{lib}", "-lc10",
            "-ltorch_cpu", "-ltorch_python", f"-Wl,-rpath,{lib}"]
     r = subprocess.run(cmd, capture_output=True, text=True)
