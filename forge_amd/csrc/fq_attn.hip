@@ -230,7 +230,7 @@ __device__ __forceinline__ uint64_t place_of(const AttnArgs& a, int page, int ke
 constexpr int DESC = 4;          // ints of a work-group's record, beside the number of parts
 constexpr int MAX_ITEMS = 1024;  // work-groups at most
 constexpr int MAX_GRID = 3;      // work-groups to a CU at most,
-constexpr size_t MAX_PART = 2 * 128 * (128 + 2);  // and floats of a part of each of them
+constexpr size_t MAX_PART = 3 * 64 * (128 + 2);  // and floats of a part of all of them
 
 // WR x WK waves: each group of WR shares tiles of 32 keys, each of its waves
 // with 16 NR rows of its own; the groups take every WK-th tile.  NS tiles of a
@@ -264,7 +264,7 @@ struct Shape {
     // What an item costs beside its units, in units: finding its blocks, its
     // queries, the first tiles' way, joining the groups and storing.
     static constexpr int OV = 256 / KU;
-    static_assert(2 * NI % WR == 0 && (WR == 1 ? NS == 2 : NS >= 3), "copies");
+    static_assert(NI % WR == 0 && (WR <= J || WR == 2 * J) && (WR == 1 ? NS == 2 : NS >= 3), "copies");
     // the waves' outputs are exchanged where the tiles were
     static_assert((size_t)WAVES * NR * 16 * D * 4 <= LDS, "join");
     static_assert(D / 16 % WK == 0, "join");
@@ -452,14 +452,12 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
                 for (int x = 0; x < S::CW; ++x) {
                     constexpr bool LOW = WR <= J;  // (all of a copy's place but wr is known)
                     const int c0 = WR * x % NI;
-                    const bool isv = WR <= NI ? WR * x >= NI : wr >= NI;
-                    const bool upper = LOW ? c0 >= J : (wr / J) % 2 == 1;
+                    const bool upper = LOW ? c0 >= J : wr >= J;
                     const uint64_t in = LOW ? (uint64_t)((c0 % J) * step) : 0;
-                    const int over = WR <= NI ? c0 : isv ? -NI : 0;  // copies past wr's
-                    if (!isv) {
-                        if (ks) dma16s(ksrc, kw + ((upper ? at_k[1] : at_k[0]) + in), kto + over * S::KSTEP);
+                    if (WR * x < NI) {
+                        if (ks) dma16s(ksrc, kw + ((upper ? at_k[1] : at_k[0]) + in), kto + c0 * S::KSTEP);
                     } else if (vs) {
-                        dma16s(vsrc, vw + ((upper ? at_v[1] : at_v[0]) + in), vto + over * S::VSTEP);
+                        dma16s(vsrc, vw + ((upper ? at_v[1] : at_v[0]) + in), vto + c0 * S::VSTEP);
                     }
                 }
             };
