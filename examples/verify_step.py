@@ -13,7 +13,10 @@ model itself finds most likely:
     python examples/verify_step.py
 
 runs it on random Q4_0 / Q8_0 weights and checks that a tree gives each token
-what its own branch, decoded token by token, gives it.
+what its own branch, decoded token by token, gives it.  It ends with what is
+accepted: before the next step a program moves the accepted branch's keys and
+values to the slots right behind the context (a branch that is not the draft's first
+tokens lies apart in the cache), or runs its tokens once more as a chain.
 """
 from __future__ import annotations
 

@@ -31,17 +31,22 @@
 // that of 16-bit queries.
 //
 // Rows and keys outside the lengths cost no branch in the common tile: only
-// tiles that reach past the cached tokens mask their scores, and there values that
-// are not finite are taken out of the product (a masked key's 0 times NaN
-// would reach rows that do not see it) and put back into the rows that see them.
+// tiles that reach past the cached tokens (or past the first table entry that is no
+// block) mask their scores, and there values that are not finite are taken out
+// of the product (a masked key's 0 times NaN would reach rows that do not see
+// it) and put back into the rows that see them.
 //
-// Bound: the caches' bytes where a tile has few rows, the waves' instructions (the
-// products in parts, exponentials and splits) where it has many.  Kernel + join, us, keys
-// and values of D = 128, a large copy at 5.2 TB/s: 32 requests of 8190 keys, 8 kv heads
-// x 4, fp16 (1.07 GB, 206 us at that rate, 164 at what reads alone reach): 1 new token
-// 153 + 8, 8 151 + 9, 16 166 + 13, 32 228 + 15, 64 332 + 22 (matrix work in
-// parts: 180); 48 of 2001 keys, 4 x 7, bf16, one token 33 + 7; one of 131000, 13 tokens,
-// 4 x 7, bf16 99 + 10 (matrix work 60); one of 333 keys 12.5, uncut.
+// Bound: the bytes of keys and values, read once for each tile of RT rows: the tiles
+// of one kv head are mostly on other dies, and 98 % of what they ask of the L2s is not
+// there.  Kernel + join, us, D = 128, a large copy at 5.2 TB/s: 32 requests of 8190
+// keys, 8 kv heads x 4, fp16 (1.07 GB, 207 us at that rate): 1 new token 209 + 7,
+// 8 215 + 9, 16 235 + 14, 32 (two tiles of rows) 452 + 22, 64 (four) 884 + 31; the same of
+// 4095 to 8190 keys and 1 to 32 tokens (0.80 GB, 1.27 asked of the
+// L2s: 5.4 TB/s): 236 + 17; 48 of 1001 to 2001 keys, 4 x 7, bf16, one token 34 + 7; one of
+// 131000, 13 tokens, 4 x 7, bf16 (two tiles of rows, 0.27 GB, matrix work 60): 100 + 10;
+// one of 333 keys 12.4, uncut.  A chain's tiles of rows all walk the keys of its last
+// token, with masks from its first new one on: 2048 tokens of a prompt, 8 x 4, fp16,
+// take 344 + 18, where half the products would do.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -1039,8 +1044,9 @@ hipError_t go(AttnArgs a, int cus, uint8_t* ws, hipStream_t st) {
     a.part = (float*)(ws + DESC_BYTES);
     // Where a request has few keys at most (by its table's columns), its items are not
     // cut, and there is nothing to join: six units take about as long as a second launch
-    // (one of 333 keys, D = 64: 12.2 us, cut 10.1 + 5.6; 64 of 370, one token: 23.1, cut
-    // 25.8 + 6.6; 8 of 340, 8 tokens: 21.1, cut 15.3 + 6.2).
+    // (one of 333 keys, D = 64: 12.4 us, cut 10.0 + 6.1; 64 of 370, one token: 23.1, cut
+    // 25.8 + 6.6; 8 of 340, 8 tokens: 21.1, cut 15.3 + 6.2).  In a wider table the same
+    // requests are cut: nothing on the host knows the lengths.
     a.whole = (int64_t)a.max_blocks << a.c.bs_log2 <= 6 * std::max(S::KU, 64);
     a.grid = std::min(a.grid, MAX_ITEMS);
     hipLaunchKernelGGL(attn_kernel<S>, dim3(a.grid), dim3(64 * S::WAVES), S::LDS, st, a);
@@ -1053,7 +1059,7 @@ hipError_t rows(const AttnArgs& a, int max_new, int cus, uint8_t* ws, hipStream_
     // By the rows of an item: few rows take waves with keys of their own, which wait for
     // nobody, more rows waves that share a tile's copies.  Small work-groups, several to a
     // CU, each keeping step by itself, hide each other's waits.  Kernel and join, us,
-    // 16 requests of 4090 keys, 8 kv heads x 4, fp16:
+    // 16 requests of 2045 to 4090 keys, 8 kv heads x 4, fp16:
     //                 16 rows                        32 rows
     //   D = 64    29.0, <1, 4, 1, 3, 3> 36.7    32.4, <1, 4, 1, 3, 3> 37.3
     //   D = 96    38.4, 43.4                    41.0, 43.9
@@ -1061,7 +1067,7 @@ hipError_t rows(const AttnArgs& a, int max_new, int cus, uint8_t* ws, hipStream_
     //             47.0)
     //   D = 256   90.3, <1, 4, 1, 4, 1> 102     -
     //   D = 128, 36 to 64 rows: 53 to 56, <2, 4, 1, 4, 2> 76.
-    // The kernel alone, 32 requests of 8190 keys, D = 128: 64 rows 166, <2, 2, 2, 4, 1>
+    // The kernel alone, 32 requests of up to 8190 keys, D = 128: 64 rows 166, <2, 2, 2, 4, 1>
     // 207; 128 rows, fp16 228 to 233, <1, 4, 1, 4, 2> 227, <2, 4, 1, 4, 2> 219 (but 65 against
     // 63 at 16 requests of 4090), <1, 8, 1, 8, 1> 286, <2, 4, 2, 4, 1> 265; bf16 233 to
     // 245, <1, 4, 1, 4, 2> 245 to 278, <2, 4, 1, 4, 2> 283, <1, 8, 1, 8, 1> 345.

@@ -17,9 +17,12 @@
 // rows are split over several work-groups, whose results a second kernel joins.
 //
 // Bound: the bytes of the logits once where there are many rows of many tokens (501 x
-// 152064 fp32, top 20: 60 us, 5.0 TB/s; 48 us with top 0; a large copy runs at 5.2
-// TB/s), the vector units' work on 16-bit logits (1000 x 32000 bf16: 40 us, where
-// the bytes take 12), latency for few (5 x 32000 fp32: 11 us, one work-group a row).
+// 152064 fp32, top 20: 60 to 62 us, 5.0 TB/s; 50 us with top 0; a large copy runs at 5.2
+// TB/s), what a row costs for its largest on rows of few chunks (1000 x 32000 bf16: 36 us
+// with top 20, 26 with top 1, 14 with top 0, where the bytes take 12), latency for few
+// (5 x 32000 fp32: 11 us, one work-group a row).  NaN logits rank above all and have no
+// threshold: rows of nothing else keep and prune every key (501 x 152064: 1500 us; 64 x
+// 32000 52 us with 1 % of NaN, 21 without).
 // No barrier lies between a wave's chunks, and a chunk's elements cost no test
 // against the row's end except in its last one: the loop is bound by instructions
 // where the logits come fast.

@@ -1,7 +1,7 @@
 // fq_step_py.cpp -- forge_amd._step: the host side of forge_amd/step.py, from tensors
 // to the C ABI of include/forge_step.h.  Checks of arguments, outputs' allocation and the call
 // in one native function each: of small calls' time the host's part is the
-// larger (rotation of one token: 9.7 us a call through Python checks and ctypes, kernel 2.4).
+// larger (rotation of one token: 9.9 us a call through Python checks and ctypes, kernel 2.4).
 //
 // step.py documents the functions; the last argument of each is the stream.  The C ABI's
 // calls go to the current device, which is the tensors' while one runs.
