@@ -55,6 +55,15 @@ SIGNATURES = {
     "fq_tree_attention": (_I, [_P, _L, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _U, _P, _P, _I, _I,
                                _L, _L, _L, _P, _I, _L, _P, _P]),
     "fq_token_logprobs": (_I, [_P, _U, _L, _I, _I, _P, _I, _I, _P, _P, _P, _P, _P]),
+    "fq_qk_norm_rope8": (_I, [_P, _L, _I, _I, _I, _I, _I, _I, _P, _P, _P, _F, _P, _P, _P, _I, _P,
+                              _P, _P, _P, _P, _I, _I, _L, _L, _L, _P]),
+    "fq_read_cache8": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _L, _L, _L, _P, _I, _L, _P, _P, _I, _I, _U,
+                            _P, _P, _P]),
+    "fq_window_attention": (_I, [_P, _L, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _I, _I, _U, _P, _P,
+                                 _P, _P, _I, _I, _L, _L, _L, _P, _I, _L, _P, _P]),
+    "fq_verify_draft": (_I, [_P, _U, _L, _I, _P, _P, _I, _I, _P, _P, _P, _L, _P, _P, _P, _P, _P]),
+    "fq_keep_accepted": (_I, [_U, _P, _P, _P, _P, _I, _I, _I, _I, _L, _L, _L, _P, _I, _L, _P, _P, _P, _P,
+                              _I, _I, _P]),
     "fq_reserve_step": (_I, [_P]),
 }
 

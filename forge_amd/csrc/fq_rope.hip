@@ -10,13 +10,11 @@
 // lane and the norm one reduction within the group.
 #include <hip/hip_runtime.h>
 
-#include "fq_step.h"
+#include "fq_rope.h"
 
 namespace fq {
 namespace {
 
-typedef float f4 __attribute__((ext_vector_type(4)));
-typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint16_t u16x4 __attribute__((ext_vector_type(4)));
 
 template <bool BF16>
@@ -35,59 +33,8 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a) {
     if (item >= (int64_t)a.N * heads) return;
     const int n = (int)(item / heads), h = (int)(item % heads);
     const int p = threadIdx.x % GS;
-    const bool on = 8 * p < a.D, turned = 8 * p < a.rot, isv = h >= a.hq + a.hkv;
-    const int d0 = !INTER && turned ? 4 * p : 8 * p;
-    const int d1 = !INTER && turned ? a.rot / 2 + 4 * p : 8 * p + 4;
-    f4 x0 = 0.0f, x1 = 0.0f;
-    if (on) {
-        const float* x = a.qkv + n * a.ld + (int64_t)h * a.D;
-        x0 = *(const f4u*)(x + d0);
-        x1 = *(const f4u*)(x + d1);
-        if (a.bias) {
-            const float* bi = a.bias + (int64_t)h * a.D;
-            x0 += *(const f4u*)(bi + d0);
-            x1 += *(const f4u*)(bi + d1);
-        }
-    }
-    const float* wt = isv ? nullptr : h < a.hq ? a.qw : a.kw;
-    if (wt) {
-        float ss = 0.0f;
-        for (int i = 0; i < 4; ++i) ss = fmaf(x0[i], x0[i], fmaf(x1[i], x1[i], ss));
-        for (int o = 1; o < GS; o <<= 1) ss += __shfl_xor(ss, o, GS);
-        const float r = 1.0f / sqrtf(ss / (float)a.D + a.eps);
-        if (on) {
-            const f4 w0 = *(const f4u*)(wt + d0), w1 = *(const f4u*)(wt + d1);
-            for (int i = 0; i < 4; ++i) {
-                x0[i] = x0[i] * r * w0[i];
-                x1[i] = x1[i] * r * w1[i];
-            }
-        }
-    }
-    if (!isv) {
-        const int pos = a.positions[n];
-        const bool known = (unsigned)pos < (unsigned)a.table_rows;
-        if (turned) {
-            const float* cs = a.table + (int64_t)(known ? pos : 0) * a.rot + 4 * p;
-            const f4 c = *(const f4u*)cs, s = *(const f4u*)(cs + a.rot / 2);
-            const f4 y0 = x0, y1 = x1;
-            for (int i = 0; i < 4; ++i) {
-                if (INTER) {  // pairs (0, 1) (2, 3) of y0, then of y1
-                    const f4 y = i < 2 ? y0 : y1;
-                    const float u = y[2 * (i & 1)], v = y[2 * (i & 1) + 1];
-                    const float t0 = u * c[i] - v * s[i], t1 = v * c[i] + u * s[i];
-                    if (i < 2) {
-                        x0[2 * i] = t0, x0[2 * i + 1] = t1;
-                    } else {
-                        x1[2 * i - 4] = t0, x1[2 * i - 3] = t1;
-                    }
-                } else {
-                    x0[i] = y0[i] * c[i] - y1[i] * s[i];
-                    x1[i] = y1[i] * c[i] + y0[i] * s[i];
-                }
-            }
-        }
-        if (!known) x0 = x1 = __builtin_nanf("");
-    }
+    const bool on = 8 * p < a.D, isv = h >= a.hq + a.hkv;
+    const auto [x0, x1, d0, d1] = head_runs<GS, INTER>(a, n, h, p, on);
     if (!on) return;
     if (h < a.hq) {
         float* q = a.q + ((int64_t)n * a.hq + h) * a.D;

@@ -60,10 +60,80 @@ struct AttnArgs {
     int* desc;    // of each work-group: the parts of an item that it begins and another ends; that item
     int grid;     // work-groups
     bool whole;   // items are not cut
+    int window, sinks;  // window 0: none
+    const float *ks, *vs;  // of caches of 8 bits
 };
 size_t attn_part_bytes(int cus);  // of the largest call
 hipError_t launch_attn(const AttnArgs& a, bool bf16, int D, int max_new, int cus, uint8_t* ws,
                        hipStream_t st);
+// With a window, or over a cache of 8 bits (type 0: fp16, 1: bf16, 2: 8 bits).
+hipError_t launch_attn_window(const AttnArgs& a, int type, int D, int max_new, int cus, uint8_t* ws,
+                              hipStream_t st);
+
+// A cache of 8 bits: codes at a CacheView's places (elements of one byte) and scales
+// [block][kv head][16 tokens].
+constexpr int GROUP = 16;  // tokens that share a scale
+
+struct Cache8 {
+    int8_t *k, *v;
+    float *ks, *vs;
+    CacheView c;
+    int hkv, D;
+    __host__ __device__ int groups() const { return (1 << c.bs_log2) / GROUP; }  // of a block
+};
+// Where a token of a request lies: block * block size + its place there; -1: nowhere.
+struct TableView {
+    const int* p;
+    int cols;
+    int64_t stride;
+    __device__ __forceinline__ int slot(int b, int64_t number, const CacheView& c) const {
+        const int64_t col = number >> c.bs_log2;
+        if (number < 0 || col >= cols) return -1;
+        const int page = p[b * stride + col];
+        if ((uint32_t)page >= (uint32_t)c.num_blocks) return -1;
+        return (page << c.bs_log2) + (int)(number & ((1 << c.bs_log2) - 1));
+    }
+};
+
+hipError_t launch_rope8(const RopeArgs& a, const Cache8& c, bool interleaved, hipStream_t st);
+
+struct ReadArgs {
+    Cache8 c;
+    TableView table;
+    const int *starts, *first;
+    int B, N;
+    void *k, *v;
+};
+hipError_t launch_read8(const ReadArgs& a, int type, hipStream_t st);
+
+struct KeepArgs {
+    void *k, *v;
+    float *ks, *vs;
+    CacheView c;
+    int hkv, D;
+    TableView table;
+    const int *lengths, *cu, *path, *accepted;
+    int B, N;
+};
+hipError_t launch_keep(const KeepArgs& a, bool codes, hipStream_t st);
+
+struct VerifyArgs {
+    const void* x;
+    int64_t ld;
+    int V;
+    const int *tokens, *cu;
+    int B, N;
+    const int* parents;
+    const float* u;
+    const float* q;
+    int64_t ldq;
+    const float* temperature;
+    int *accepted, *path, *next;
+    int seg, parts;  // elements of a row's part, parts of a row
+    uint8_t* ws;
+};
+size_t verify_part_bytes(int cus);  // of the largest call
+hipError_t launch_verify(const VerifyArgs& a, int type, int cus, hipStream_t st);
 
 struct LogpArgs {
     const void* x;

@@ -1,0 +1,549 @@
+// fq_verify.hip -- drafted tokens against the target's probabilities.
+//
+// Three or four launches.  Statistics: every row's largest logit m and s = sum e^((x - m) / T)
+// (at temperatures of 0 or below its first largest), one pass over the logits in 32 bits, rows cut into parts
+// where there are few.  Walk: what is accepted.  Whether a token is, were it tried, depends on
+// its earlier siblings alone: u (1 - sum of their p) < p, so that all tests are made at
+// once, a lane a token, and the walk goes over bits.  The same launch sums e^((x - m) / T) of
+// each request's last accepted row, without the refused tokens, over chunks in 64 bits (a random number within
+// 1e-7 of a border of the cumulated sum would find another token in 32: at 150000
+// tokens one number in a hundred).  With draft probabilities, whose subtraction needs the
+// whole sum first, another launch sums what is left.  Pick: the chunk in which the sum passes the random number, then
+// the token in it.
+//
+// Bound: the bytes of the logits, read once; a row of each request is read again.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "fq_step.h"
+
+namespace fq {
+namespace {
+
+typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t u4a __attribute__((ext_vector_type(4), aligned(2)));
+
+constexpr float LOWEST = -3.402823466e38f;
+constexpr float LOG2E = 1.44269504088896341f;
+constexpr int E = 16;             // elements of a lane at a time
+constexpr int STEP = 256 * E;     // of a work-group
+constexpr int MAX_STATS = 1 << 20;
+constexpr int MAX_SUMS = 1 << 18;  // chunks of all requests
+constexpr int LANES = 64;          // tokens of a request whose parents count
+
+struct Stat {
+    float m, s;  // s: NaN for a row with NaN or +inf, 0 for one of -inf alone; > 0 otherwise
+    int first;   // the first largest, at temperatures of 0 and below
+    int pad;
+};
+// What the walk leaves of a request.
+struct Left {
+    int row;      // the last accepted token's row; -1: no next token
+    int q;        // the row of draft probabilities to take off; -1: none
+    int refused;  // how many tokens are taken out
+    int best;     // the next token where it is known already; -1
+    float m;      // the row's largest
+    int token[LANES];
+};
+struct Space {
+    Stat* stats;
+    Left* left;
+    double *whole, *rest;  // [B][chunks]
+    int chunks, chunk;
+};
+
+__device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+template <int TYPE>
+__device__ __forceinline__ float load1(const void* x, int64_t at) {
+    if (TYPE == 0) return ((const float*)x)[at];
+    if (TYPE == 1) return (float)((const _Float16*)x)[at];
+    return __uint_as_float((uint32_t)((const uint16_t*)x)[at] << 16);
+}
+
+// 16 elements of a lane: those of a work-group's step lie in runs of 16 bytes a lane.
+template <int TYPE>
+__device__ __forceinline__ int64_t place16(int i) {  // of element i of this lane in the step
+    constexpr int R = TYPE == 0 ? 4 : 8;
+    return (int64_t)(i / R) * 256 * R + threadIdx.x * R + i % R;
+}
+template <int TYPE>
+__device__ __forceinline__ void load16(const void* x, int64_t at, int64_t end, float (&v)[E]) {
+    if (at + STEP <= end) {
+        if constexpr (TYPE == 0) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const f4u w = *(const f4u*)((const float*)x + at + place16<TYPE>(4 * k));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[4 * k + e] = w[e];
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const u4a w = *(const u4a*)((const uint16_t*)x + at + place16<TYPE>(8 * k));
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const uint16_t b = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
+                    v[8 * k + e] = TYPE == 1 ? (float)__builtin_bit_cast(_Float16, b) : __uint_as_float((uint32_t)b << 16);
+                }
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            const int64_t j = at + place16<TYPE>(i);
+            v[i] = j < end ? load1<TYPE>(x, j) : -__builtin_inff();
+        }
+    }
+}
+
+// The request that row n belongs to; cu rises.  (A row before cu[0] or past cu[B]: any.)
+__device__ __forceinline__ int request_of(const int* cu, int B, int n) {
+    int lo = 0, hi = B;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        (cu[mid] <= n ? lo : hi) = mid;
+    }
+    return lo;
+}
+
+template <int TYPE, bool TEMP>
+__global__ __launch_bounds__(256) void stats_kernel(VerifyArgs a, Space w) {
+    const int n = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
+    const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6);
+    __shared__ float s_m[4], s_s[4];
+    __shared__ int s_i[4];
+    float T = 1.0f;
+    if (TEMP) T = a.temperature[uni(request_of(a.cu, a.B, n))];
+    const int64_t row = (int64_t)n * a.ld, from = (int64_t)part * a.seg, to = std::min<int64_t>(from + a.seg, a.V);
+    float m = LOWEST, s = 0.0f;
+    int first = 0x7FFFFFFF;
+    if (!TEMP || T > 0.0f) {
+        const float k = TEMP ? fminf(LOG2E / T, 3e38f) : LOG2E;
+        for (int64_t at = from; at < to; at += STEP) {
+            float v[E];
+            load16<TYPE>(a.x, row + at, row + to, v);
+            float mx = v[0];
+#pragma unroll
+            for (int i = 1; i < E; ++i) mx = fmaxf(mx, v[i]);
+            mx = fmaxf(mx, m);
+            float sum[2] = {s * exp2f((m - mx) * k), 0.0f};
+            m = mx;
+#pragma unroll
+            for (int i = 0; i < E; ++i) sum[i & 1] += __builtin_amdgcn_exp2f((v[i] - m) * k);
+            s = sum[0] + sum[1];
+        }
+        float mx = m;
+        for (int o = 1; o < 64; o <<= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
+        if (lane == 0) s_m[wave] = mx;
+        __syncthreads();
+        mx = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+        s = m == mx ? s : s * exp2f((m - mx) * k);  // (an infinity less itself is NaN already)
+        for (int o = 1; o < 64; o <<= 1) s += __shfl_xor(s, o);
+        if (lane == 0) s_s[wave] = s;
+        __syncthreads();
+        if (tid == 0) w.stats[blockIdx.x] = {mx, s_s[0] + s_s[1] + s_s[2] + s_s[3], 0, 0};
+        return;
+    }
+    bool bad = false;
+    for (int64_t at = from; at < to; at += STEP) {
+        float v[E];
+        load16<TYPE>(a.x, row + at, row + to, v);
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            bad |= !(v[i] < __builtin_inff());
+            const int j = (int)(at + place16<TYPE>(i));
+            if (v[i] > m || (v[i] == m && v[i] > -__builtin_inff() && j < first)) m = v[i], first = j;
+        }
+    }
+    for (int o = 1; o < 64; o <<= 1) {
+        const float om = __shfl_xor(m, o);
+        const int of = __shfl_xor(first, o);
+        if (om > m || (om == m && of < first)) m = om, first = of;
+    }
+    bad = __any(bad);
+    if (lane == 0) s_m[wave] = m, s_i[wave] = first, s_s[wave] = bad ? __builtin_nanf("") : 0.0f;
+    __syncthreads();
+    if (tid == 0) {
+        for (int i = 1; i < 4; ++i)
+            if (s_m[i] > m || (s_m[i] == m && s_i[i] < first)) m = s_m[i], first = s_i[i];
+        s = s_s[0] + s_s[1] + s_s[2] + s_s[3];
+        if (first != 0x7FFFFFFF) s += 1.0f;
+        w.stats[blockIdx.x] = {m, s, first, 0};
+    }
+}
+
+// A row's parts as one.
+__device__ __forceinline__ Stat joined(const VerifyArgs& a, const Space& w, int row, float T) {
+    const Stat* p = w.stats + (int64_t)row * a.parts;
+    Stat r = p[0];
+    const float k = fminf(LOG2E / T, 3e38f);
+    for (int i = 1; i < a.parts; ++i) {
+        const Stat o = p[i];
+        if (T > 0.0f) {
+            const float m = fmaxf(r.m, o.m);
+            r.s = (r.m == m ? r.s : r.s * exp2f((r.m - m) * k)) + (o.m == m ? o.s : o.s * exp2f((o.m - m) * k));
+            r.m = m;
+        } else {
+            r.s += o.s;
+            if (o.m > r.m || (o.m == r.m && o.first < r.first)) r.m = o.m, r.first = o.first;
+        }
+    }
+    return r;
+}
+__device__ __forceinline__ bool usable(const Stat& s) { return s.s > 0.0f && s.s < __builtin_inff(); }
+
+__device__ __forceinline__ double lane_of(double v, int i) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)b, i), hi = __builtin_amdgcn_readlane((uint32_t)(b >> 32), i);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+
+// The chunk's tokens that are refused, as bits of s_out.  (All threads of the work-group.)
+__device__ __forceinline__ void mark(const Left& l, int64_t at, uint32_t (&s_out)[STEP / 32]) {
+    const int tid = threadIdx.x;
+    __syncthreads();
+    if (tid < STEP / 32) s_out[tid] = 0;
+    __syncthreads();
+    if (tid < l.refused) {
+        const int64_t i = l.token[tid] - at;
+        if (i >= 0 && i < STEP) atomicOr(&s_out[i >> 5], 1u << (i & 31));
+    }
+    __syncthreads();
+}
+
+__device__ __forceinline__ double sum_group(double v, double (&s)[4]) {
+    for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return s[0] + s[1] + s[2] + s[3];
+}
+
+// Request b's walk, by one wave; `out`: it writes what is accepted.
+template <int TYPE>
+__device__ __forceinline__ void walk(const VerifyArgs& a, const Space& w, int b, bool out, Left& to) {
+    const int lane = threadIdx.x & 63;
+    const int t0 = min(max(a.cu[b], 0), a.N), nt = min(max(a.cu[b + 1], t0), a.N) - t0;
+    const float T = a.temperature ? a.temperature[b] : 1.0f;
+    const double inv = T > 0.0f ? 1.0 / (double)T : 1.0;
+    int row = -1, q_row = -1, best = -1, refused = 0;
+    float m = 0.0f;
+    int accepted = 0, last = 0;
+    if (nt > 0) {
+        // p of token i of the request after token `up`
+        const auto chance = [&](int i, int up) {
+            const int token = a.tokens[t0 + i];
+            if (up < 0 || token < 0 || token >= a.V) return 0.0;
+            const Stat s = joined(a, w, t0 + up, T);
+            if (!usable(s)) return 0.0;
+            if (!(T > 0.0f)) return s.first == token ? 1.0 : 0.0;
+            const float x = load1<TYPE>(a.x, (int64_t)(t0 + up) * a.ld + token);
+            return exp(((double)x - (double)s.m) * inv) / (double)s.s;
+        };
+        if (!a.parents) {
+            accepted = 1;
+            for (int base = 1; base < nt; base += 64) {
+                const int i = base + lane;
+                bool good = false;
+                if (i < nt) {
+                    const double p = chance(i, i - 1);
+                    const int token = a.tokens[t0 + i];
+                    const bool known = token >= 0 && token < a.V;
+                    const double q = a.q && known ? (double)a.q[(int64_t)(t0 + i) * a.ldq + token] : 1.0;
+                    good = (double)a.u[t0 + i] * q < p;
+                }
+                const uint64_t no = __ballot(!good);
+                accepted += no ? __builtin_ctzll(no) : 64;
+                if (no) break;
+            }
+            last = accepted - 1;
+            if (out)
+                for (int i = lane; i < nt; i += 64) a.path[t0 + i] = i < accepted ? i : -1;
+            if (accepted < nt) {
+                if (a.q) {
+                    q_row = t0 + accepted;
+                } else {
+                    refused = 1;
+                    if (lane == 0) to.token[0] = a.tokens[t0 + accepted];
+                }
+            }
+        } else {
+            const int n = min(nt, LANES);
+            int par = -9, token = -1;
+            double p = 0.0, u = 0.0;
+            if (lane < n) {
+                par = a.parents[t0 + lane];
+                if (par < 0 || par >= lane) par = -9;
+                token = a.tokens[t0 + lane];
+                u = (double)a.u[t0 + lane];
+                p = chance(lane, par);
+            }
+            for (int j = 1; j < n; ++j) {  // refused before already
+                const int pj = __builtin_amdgcn_readlane(par, j), tj = __builtin_amdgcn_readlane(token, j);
+                if (j < lane && pj == par && tj == token) p = 0.0;
+            }
+            double mass = 1.0;
+            for (int j = 1; j < n; ++j) {
+                const int pj = __builtin_amdgcn_readlane(par, j);
+                const double v = lane_of(p, j);
+                if (j < lane && pj == par) mass -= v;
+            }
+            bool good = par >= 0 && u * mass < p;
+            const uint64_t all = __ballot(good);
+            bool before = false;
+            for (int j = 1; j < n; ++j)
+                before |= j < lane && (all >> j & 1) && __builtin_amdgcn_readlane(par, j) == par;
+            const uint64_t pass = __ballot(good && !before);
+            uint64_t acc = 1;
+            for (int i = 1; i < n; ++i)
+                if (pass >> i & 1) acc |= (acc >> __builtin_amdgcn_readlane(par, i) & 1) << i;
+            accepted = __builtin_popcountll(acc);
+            last = 63 - __builtin_clzll(acc);
+            if (out) {
+                for (int i = lane; i < nt; i += 64)
+                    if (i >= accepted) a.path[t0 + i] = -1;
+                if (acc >> lane & 1) a.path[t0 + __builtin_popcountll(acc & ((1ull << lane) - 1))] = lane;
+            }
+            const uint64_t kids = __ballot(lane < n && par == last);
+            refused = __builtin_popcountll(kids);
+            if (kids >> lane & 1) to.token[__builtin_popcountll(kids & ((1ull << lane) - 1))] = token;
+        }
+        const Stat s = joined(a, w, t0 + last, T);
+        if (usable(s)) {
+            row = t0 + last;
+            m = s.m;
+            if (!(T > 0.0f)) best = s.first;
+        }
+    }
+    if (lane == 0) {
+        to.row = row, to.q = q_row, to.refused = refused, to.best = best, to.m = m;
+        if (out) a.accepted[b] = accepted;
+    }
+}
+
+// Walk, and the sums over the chunks of the last row.
+template <int TYPE>
+__global__ __launch_bounds__(256) void walk_kernel(VerifyArgs a, Space w) {
+    __shared__ Left s_left;
+    __shared__ uint32_t s_out[STEP / 32];
+    __shared__ double s_sum[4];
+    const int b = blockIdx.x / w.chunks, c = blockIdx.x % w.chunks, tid = threadIdx.x;
+    if (tid < 64) walk<TYPE>(a, w, b, c == 0, s_left);
+    if (b == a.B - 1 && c == 0)  // padding
+        for (int64_t i = std::max(a.cu[a.B], 0) + tid; i < a.N; i += 256) a.path[i] = -1;
+    __syncthreads();
+    const Left& l = s_left;
+    if (c == 0) {
+        if (tid == 0) w.left[b].row = l.row, w.left[b].q = l.q, w.left[b].refused = l.refused,
+                      w.left[b].best = l.best, w.left[b].m = l.m;
+        if (tid < l.refused) w.left[b].token[tid] = l.token[tid];
+    }
+    if (l.row < 0 || l.best >= 0) return;
+    const double inv = a.temperature ? 1.0 / (double)a.temperature[b] : 1.0, m = l.m;
+    const int64_t end = std::min<int64_t>((int64_t)(c + 1) * w.chunk, a.V);
+    double whole = 0.0, rest = 0.0;
+    for (int64_t at = (int64_t)c * w.chunk; at < end; at += STEP) {
+        mark(l, at, s_out);
+        float v[E];
+        load16<TYPE>(a.x, (int64_t)l.row * a.ld + at, (int64_t)l.row * a.ld + end, v);
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            const double e = exp(((double)v[i] - m) * inv);
+            const int j = (int)place16<TYPE>(i);
+            whole += e;
+            rest += s_out[j >> 5] >> (j & 31) & 1 ? 0.0 : e;
+        }
+    }
+    whole = sum_group(whole, s_sum);
+    rest = sum_group(rest, s_sum);
+    if (tid == 0) {
+        w.whole[blockIdx.x] = whole;
+        w.rest[blockIdx.x] = rest;
+    }
+}
+
+// The sum of a request's n chunks, by the work-group.
+__device__ __forceinline__ double total_of(const double* p, int n, double (&s)[4]) {
+    double v = 0.0;
+    for (int i = threadIdx.x; i < n; i += 256) v += p[i];
+    return sum_group(v, s);
+}
+
+// With draft probabilities: what is left of each chunk.
+template <int TYPE>
+__global__ __launch_bounds__(256) void left_kernel(VerifyArgs a, Space w) {
+    __shared__ double s_sum[4];
+    const int b = blockIdx.x / w.chunks, c = blockIdx.x % w.chunks;
+    const int row = w.left[b].row, q = w.left[b].q;
+    if (row < 0 || w.left[b].best >= 0 || q < 0) return;
+    const double inv = a.temperature ? 1.0 / (double)a.temperature[b] : 1.0, m = w.left[b].m;
+    const double all = total_of(w.whole + (int64_t)b * w.chunks, w.chunks, s_sum);
+    const int64_t end = std::min<int64_t>((int64_t)(c + 1) * w.chunk, a.V);
+    double rest = 0.0;
+    for (int64_t at = (int64_t)c * w.chunk; at < end; at += STEP) {
+        float v[E], d[E];
+        load16<TYPE>(a.x, (int64_t)row * a.ld + at, (int64_t)row * a.ld + end, v);
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            const int64_t j = at + place16<TYPE>(i);
+            d[i] = j < end ? a.q[(int64_t)q * a.ldq + j] : 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < E; ++i) rest += fmax(exp(((double)v[i] - m) * inv) / all - (double)d[i], 0.0);
+    }
+    rest = sum_group(rest, s_sum);
+    if (threadIdx.x == 0) w.rest[blockIdx.x] = rest;
+}
+
+// The lowest token whose cumulated sum is above u times the whole.
+template <int TYPE>
+__global__ __launch_bounds__(256) void pick_kernel(VerifyArgs a, Space w) {
+    __shared__ uint32_t s_out[STEP / 32];
+    __shared__ double s_sum[4], s_pre[4], s_at;
+    __shared__ int s_chunk, s_token;
+    const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6);
+    const Left& l = w.left[b];
+    if (l.row < 0 || l.best >= 0) {
+        if (tid == 0) a.next[b] = l.row < 0 ? -1 : l.best;
+        return;
+    }
+    const double* whole = w.whole + (int64_t)b * w.chunks;
+    const double* rest = w.rest + (int64_t)b * w.chunks;
+    const double all = total_of(whole, w.chunks, s_sum);
+    const double left = total_of(rest, w.chunks, s_sum);
+    const bool some = left > 0.0;  // else p itself
+    const double* sums = some ? rest : whole;
+    const bool drafted = some && l.q >= 0;
+    const double target = (double)a.u[max(a.cu[b], 0)] * (some ? left : all);
+    if (tid == 0) s_chunk = -1, s_token = 0;
+    __syncthreads();
+    if (wave == 0) {  // the chunk, 64 at a time; else the last one that has something
+        double before = 0.0;
+        int chunk = -1;
+        double at = 0.0;
+        for (int base = 0; base < w.chunks; base += 64) {
+            const double v = base + lane < w.chunks ? sums[base + lane] : 0.0;
+            double upto = v;
+            for (int o = 1; o < 64; o <<= 1) {
+                const double x = __shfl_up(upto, o);
+                if (lane >= o) upto += x;
+            }
+            const uint64_t past = __ballot(v > 0.0 && before + upto > target), any = __ballot(v > 0.0);
+            const int i = past ? __builtin_ctzll(past) : any ? 63 - __builtin_clzll(any) : -1;
+            if (i >= 0) chunk = base + i, at = before + lane_of(upto, uni(i)) - lane_of(v, uni(i));
+            if (past) break;
+            before += lane_of(upto, 63);
+        }
+        if (lane == 0) s_chunk = chunk, s_at = at;
+    }
+    __syncthreads();
+    if (s_chunk < 0) {  // (nothing anywhere: not for a row that is usable)
+        if (tid == 0) a.next[b] = -1;
+        return;
+    }
+    const double inv = a.temperature ? 1.0 / (double)a.temperature[b] : 1.0, m = l.m;
+    const int64_t begin = (int64_t)s_chunk * w.chunk, end = std::min<int64_t>(begin + w.chunk, a.V);
+    double before = s_at;
+    for (int64_t at = begin; at < end; at += STEP) {
+        mark(l, at, s_out);
+        // a lane's elements lie next to each other here
+        double e[E], mine = 0.0;
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            const int in = tid * E + i;
+            const int64_t j = at + in;
+            e[i] = 0.0;
+            if (j < end) {
+                const double x = exp(((double)load1<TYPE>(a.x, (int64_t)l.row * a.ld + j) - m) * inv);
+                if (drafted) e[i] = fmax(x / all - (double)a.q[(int64_t)l.q * a.ldq + j], 0.0);
+                else e[i] = some && (s_out[in >> 5] >> (in & 31) & 1) ? 0.0 : x;
+            }
+            mine += e[i];
+        }
+        double upto = mine;
+        for (int o = 1; o < 64; o <<= 1) {
+            const double x = __shfl_up(upto, o);
+            if (lane >= o) upto += x;
+        }
+        __syncthreads();
+        if (lane == 63) s_pre[wave] = upto;
+        __syncthreads();
+        double base = before, step = 0.0;
+        for (int i = 0; i < 4; ++i) {
+            if (i < wave) base += s_pre[i];
+            step += s_pre[i];
+        }
+        double sum = base + upto - mine;
+        int found = 0x7FFFFFFF, last = -1;
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            sum += e[i];
+            if (e[i] > 0.0) {
+                last = (int)(at + tid * E + i);
+                if (found == 0x7FFFFFFF && sum > target) found = last;
+            }
+        }
+        for (int o = 1; o < 64; o <<= 1) {
+            found = min(found, __shfl_xor(found, o));
+            last = max(last, __shfl_xor(last, o));
+        }
+        __shared__ int s_found[4], s_last[4];
+        if (lane == 0) s_found[wave] = found, s_last[wave] = last;
+        __syncthreads();
+        if (tid == 0) {
+            for (int i = 0; i < 4; ++i) found = min(found, s_found[i]), last = max(last, s_last[i]);
+            if (found != 0x7FFFFFFF) {
+                a.next[b] = found;
+                s_token = 1;
+            } else if (last >= 0) {
+                a.next[b] = last;  // (stays where rounding leaves the chunk's end below the target)
+            }
+        }
+        __syncthreads();
+        if (s_token) return;
+        before += step;
+    }
+}
+
+template <int TYPE>
+hipError_t go(const VerifyArgs& a, const Space& w, hipStream_t st) {
+    const dim3 t(256), rows((unsigned)(a.N * a.parts)), sums((unsigned)(a.B * w.chunks));
+    if (a.N) {
+        if (a.temperature) hipLaunchKernelGGL((stats_kernel<TYPE, true>), rows, t, 0, st, a, w);
+        else hipLaunchKernelGGL((stats_kernel<TYPE, false>), rows, t, 0, st, a, w);
+    }
+    hipLaunchKernelGGL(walk_kernel<TYPE>, sums, t, 0, st, a, w);
+    if (a.q) hipLaunchKernelGGL(left_kernel<TYPE>, sums, t, 0, st, a, w);
+    hipLaunchKernelGGL(pick_kernel<TYPE>, dim3((unsigned)a.B), t, 0, st, a, w);
+    return hipGetLastError();
+}
+
+constexpr int MAX_B = 8192;
+
+}  // namespace
+
+size_t verify_part_bytes(int) {
+    return (size_t)MAX_STATS * sizeof(Stat) + MAX_B * sizeof(Left) + 2 * (size_t)(MAX_SUMS + MAX_B) * sizeof(double);
+}
+
+hipError_t launch_verify(const VerifyArgs& a0, int type, int cus, hipStream_t st) {
+    VerifyArgs a = a0;
+    // Rows are cut until there are two work-groups a CU, into parts of a step at least.
+    const int most = (a.V + STEP - 1) / STEP;
+    a.parts = a.N ? std::max(1, std::min(most, 2 * cus / a.N)) : 1;
+    a.seg = (most + a.parts - 1) / a.parts * STEP;
+    a.parts = (a.V + a.seg - 1) / a.seg;
+    Space w;
+    const int per = std::max(1, (int)(((int64_t)a.B * most + MAX_SUMS - 1) / MAX_SUMS));
+    w.chunk = per * STEP;
+    w.chunks = (a.V + w.chunk - 1) / w.chunk;
+    w.stats = (Stat*)a.ws;
+    w.left = (Left*)(w.stats + MAX_STATS);
+    w.whole = (double*)(w.left + MAX_B);
+    w.rest = w.whole + MAX_SUMS + MAX_B;
+    return type == 0 ? go<0>(a, w, st) : type == 1 ? go<1>(a, w, st) : go<2>(a, w, st);
+}
+
+}  // namespace fq

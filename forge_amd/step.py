@@ -12,12 +12,20 @@ the projections::
         ...
     scores = token_logprobs(logits, targets, top=5)
 
+or, where drafted tokens are sampled::
+
+    done = verify_draft(logits, tokens, plan.cu, uniforms, parents=parents)
+    for each layer:
+        keep_accepted(k_cache, v_cache, block_table, lengths, plan.cu, done.path, done.accepted)
+    lengths += done.accepted
+
 They stand where the reference verifies drafted tokens
 (src/inference/speculative.cpp:64) over its paged cache, with activations in
-fp32 as everywhere here and caches in fp16 or bf16.  All arithmetic runs in
+fp32 as everywhere here and caches in fp16 or bf16, or in 8 bits (Cache8).  All arithmetic runs in
 libforge_q.so (include/forge_step.h, which states the operators in full);
 nothing waits for the GPU, and no length is needed on the host but the sum of
-the new tokens.  examples/verify_step.py runs a small model through them.
+the new tokens.  examples/verify_step.py runs a small model through them, examples/sample_drafts.py the
+sampling of drafted trees over a cache of 8 bits.
 """
 from __future__ import annotations
 
@@ -46,6 +54,20 @@ class TokenLogprobs(NamedTuple):
     top_tokens: Optional[torch.Tensor]    # int32 [M, top]
 
 
+class Cache8(NamedTuple):
+    """Keys or values in 8 bits: codes times the scale of their 16 tokens and kv head.
+    What takes k_cache and v_cache takes a pair of these in their place."""
+    codes: torch.Tensor   # int8 [num_blocks, block_size, n_kv_heads, head_dim]
+    scales: torch.Tensor  # fp32 [num_blocks, n_kv_heads, block_size / 16]
+
+
+class Verified(NamedTuple):
+    """verify_draft's results for B requests of N tokens."""
+    accepted: torch.Tensor     # int32 [B]: accepted tokens, the known one included
+    path: torch.Tensor         # int32 [N]: path[cu[b] + d] is the number of the d-th accepted one, -1 behind
+    next_tokens: torch.Tensor  # int32 [B]: the token after the last accepted one; -1: none
+
+
 def _native():
     """The host side of these functions (csrc/fq_step_py.cpp); like the library it has no
     fallback."""
@@ -71,9 +93,16 @@ def paged_cache(num_blocks: int, block_size: int, n_kv_heads: int, head_dim: int
                 dtype: torch.dtype = torch.float16, device="cuda"):
     """Zeroed key and value caches [num_blocks, block_size, n_kv_heads, head_dim].
     A block's rows lie head by head in memory, so that a head's keys are read in
-    long runs; any other order of the first three axes is accepted as well."""
-    return tuple(torch.zeros((num_blocks, n_kv_heads, block_size, head_dim), dtype=dtype,
-                             device=device).transpose(1, 2) for _ in range(2))
+    long runs; any other order of the first three axes is accepted as well.  dtype int8: a
+    pair of Cache8, half the bytes; a head's tokens 16 n .. 16 n + 15 share a scale."""
+    def cache():
+        data = torch.zeros((num_blocks, n_kv_heads, block_size, head_dim), dtype=dtype,
+                           device=device).transpose(1, 2)
+        if dtype != torch.int8:
+            return data
+        return Cache8(data, torch.zeros((num_blocks, n_kv_heads, block_size // 16), device=device))
+
+    return cache(), cache()
 
 
 def plan_step(lengths: torch.Tensor, new_tokens: torch.Tensor, block_table: torch.Tensor,
@@ -111,7 +140,12 @@ def qk_norm_rope(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor
     and sin, whose width is the number of rotated elements of a head; bias: fp32,
     added to each row first; q_weight, k_weight: fp32 [D], the heads' RMS norms
     (none: not normalized); interleaved: pairs (2i, 2i + 1) instead of (i, i + rot / 2).
-    Tokens whose slot is -1 leave the caches as they are."""
+    Tokens whose slot is -1 leave the caches as they are.
+
+    Into a Cache8 the tokens of a request go as plan_step's slots have them, next to each other.  16
+    tokens and a kv head share a scale, the largest magnitude over 127; a token that
+    needs a larger one than its group has gives the group that, and the codes held are
+    rounded again.  Infinite elements are held to the largest finite one of the group, NaN is 0."""
     return _native().rope(qkv, positions, slots, table, k_cache, v_cache, bias, q_weight, k_weight, eps,
                           interleaved, _stream(qkv))
 
@@ -119,7 +153,7 @@ def qk_norm_rope(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor
 def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                    block_table: torch.Tensor, lengths: torch.Tensor, cu: torch.Tensor,
                    masks: Optional[torch.Tensor] = None, *, max_new: Optional[int] = None,
-                   scale: Optional[float] = None) -> torch.Tensor:
+                   scale: Optional[float] = None, window: Optional[int] = None, sinks: int = 0) -> torch.Tensor:
     """Attention of the step's tokens, fp32 [N, hq, D].
 
     q: fp32 [N, hq, D], tokens any distance apart; lengths: int32 [B], the cached tokens
@@ -129,9 +163,59 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     that is no block of the caches (-1: plan_step had none left) would hold is not
     there, so that info[1] of the plan, where it is not 0, says that answers lack it.  max_new:
     the most new tokens of one request where the caller knows it (it chooses how many
-    rows a tile has; without it their average is taken); scale: D^-0.5 unless given."""
+    rows a tile has; without it their average is taken); scale: D^-0.5 unless given.
+
+    window: of the keys above, a token sees those of the window positions up to its own and
+    those of the request's first sinks positions (a drafted token's position is that of plan_step);
+    what no token of the call sees is not read."""
     return _native().attention(q, k_cache, v_cache, block_table, lengths, cu, masks, max_new, scale,
-                               _stream(q))
+                               window, sinks, _stream(q))
+
+
+_READ = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 100}
+
+
+def read_cache(k_cache: Cache8, v_cache: Cache8, block_table: torch.Tensor, starts: torch.Tensor,
+               n_tokens: int, *, first: Optional[torch.Tensor] = None,
+               dtype: torch.dtype = torch.float16):
+    """Keys and values [n_tokens, kv heads, D] of caches of 8 bits in fp16, bf16 or fp32.
+
+    Rows starts[b] .. starts[b + 1] - 1 (int32 [B + 1], prefix sums) are the tokens of request
+    b from its number first[b] (int32 [B]; none: its first) on.  Tokens whose block the
+    table does not have, and rows past the last request's, are zeros."""
+    if dtype not in _READ:
+        raise RuntimeError("read_cache: dtype must be fp16, bf16 or fp32")
+    return _native().read(k_cache, v_cache, block_table, starts, n_tokens, _READ[dtype], first, _stream(starts))
+
+
+def verify_draft(logits: torch.Tensor, tokens: torch.Tensor, cu: torch.Tensor, uniforms: torch.Tensor, *,
+                 parents: Optional[torch.Tensor] = None, draft_probs: Optional[torch.Tensor] = None,
+                 temperature: Optional[torch.Tensor] = None) -> Verified:
+    """Which drafted tokens a step's logits accept, and each request's next token.
+
+    The step's tokens (int32 [N], plan_step's cu) are each request's last sampled token, which
+    is accepted, and drafted ones behind it; logits (fp32, fp16 or bf16 [N, V], rows any
+    distance apart) are what the model says after each; uniforms: fp32 [N] in [0, 1).
+    parents: as plan_step's (None: chains).  The accepted tokens and the next one
+    are distributed as tokens sampled one by one from softmax(logits / temperature), whatever was
+    drafted: token i is tried with uniforms[i] against what its refused siblings left, the next token
+    is drawn with the request's first one.  draft_probs: fp32 [N, V], row i the distribution that token i of a
+    chain was drawn from; without it drafted tokens are taken as given.  temperature: fp32 [B],
+    finite (None: 1; 0: the largest logit, of equal ones the lowest token).  With one
+    token a request this samples the next one.
+
+    A row with a NaN or +inf logit or nothing but -inf ends its request with next token -1."""
+    return Verified(*_native().verify(logits, tokens, cu, uniforms, parents, draft_probs, temperature,
+                                      _stream(logits)))
+
+
+def keep_accepted(k_cache, v_cache, block_table: torch.Tensor, lengths: torch.Tensor, cu: torch.Tensor,
+                  path: torch.Tensor, accepted: torch.Tensor) -> None:
+    """Moves verify_draft's accepted tokens behind the context: their keys and values, in caches of
+    any type, go to the slots of numbers lengths[b], lengths[b] + 1, .., after which
+    lengths + accepted are the requests' lengths.  lengths: those before the step.  Chains stay where they are.
+    In a Cache8 a moved token's codes are rounded again where its new group has another scale."""
+    _native().keep(k_cache, v_cache, block_table, lengths, cu, path, accepted, _stream(lengths))
 
 
 def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None,

@@ -8,6 +8,17 @@
  *   fq_tree_attention   drafted tokens over their context and their ancestors
  *   fq_token_logprobs   log probabilities, entropy and top alternatives of
  *                       the head's rows
+ *   fq_verify_draft     which drafted tokens are accepted, and the next one, from
+ *                       the head's rows and given random numbers
+ *   fq_keep_accepted    an accepted branch's keys and values to the slots behind
+ *                       the context
+ *
+ * and for caches of 8 bits and windows
+ *
+ *   fq_qk_norm_rope8    fq_qk_norm_rope into a cache of 8 bits
+ *   fq_read_cache8      such a cache's keys and values in 16 or 32 bits
+ *   fq_window_attention fq_tree_attention over either kind of cache, with a sliding
+ *                       window and first tokens that stay visible
  *
  * They take the place of the reference's verification of drafted tokens
  * (src/inference/speculative.cpp:64) and of its paged cache, attention mask,
@@ -33,7 +44,12 @@
  * token has a slot in it, and fq_tree_attention's tokens see no key of it.  Nor are there
  * slots or keys past the table's max_blocks columns, whatever the length.
  *
- * fq_tree_attention and fq_token_logprobs keep partial results in the
+ * A cache of 8 bits (FQ_TYPE_I8) has int8 codes in the place of elements (strides multiples of
+ * 16) and fp32 scales [num_blocks][kv heads][block_size / 16], contiguous: element =
+ * code * scale of the 16 tokens (a group) and kv head.  A scale that is no positive finite number
+ * counts as 0.  Codes are -127 .. 127 as written here; any are read.
+ *
+ * fq_tree_attention, fq_window_attention, fq_token_logprobs and fq_verify_draft keep partial results in the
  * library's per-stream workspace; fq_reserve_step sizes it for calls under
  * HIP-graph capture (fq_release_workspace frees it).
  */
@@ -52,6 +68,7 @@ extern "C" {
 #define FQ_TYPE_F32 0u
 #define FQ_TYPE_F16 1u
 #define FQ_TYPE_BF16 100u /* no forge::DataType of its own */
+#define FQ_TYPE_I8 101u   /* nor has this: codes with scales, for caches */
 
 /* Plans a step of up to B = 8192 requests and N tokens.
  *   cu [B+1]         prefix sums of new_tokens
@@ -108,6 +125,87 @@ int fq_tree_attention(const float* q, int64_t ldq, const int32_t* lengths, const
                       int num_blocks, int block_size, int64_t stride_block,
                       int64_t stride_token, int64_t stride_head, const int32_t* block_table,
                       int max_blocks, int64_t table_stride, float* out, void* stream);
+
+/* fq_qk_norm_rope with the keys and values rounded into a cache of 8 bits.  The tokens of a
+ * group that come in one call stand next to each other, in rising slots, as fq_plan_step
+ * gives them; the group's slots before its first one hold tokens of the request.  With y the
+ * largest finite magnitude of the new keys (values) of a group and kv head, the
+ * group's scale becomes
+ *   s = y / 127            where the first new token is the group's first, else
+ *   s = max(old s, y / 127), and where that is more, the codes held become
+ *                          rint(code * (old s * (1 / s)))
+ * and an element's code is rint(x * (1 / s)), held to -127 .. 127, 0 for NaN and where s is
+ * below 2^-126.  Codes behind the group's last new token stay as they are.  Where
+ * tokens of a group come otherwise, its codes and scale are unspecified.  D: a multiple of 16. */
+int fq_qk_norm_rope8(const float* qkv, int64_t ld, int N, int hq, int hkv, int D, int rot,
+                     int interleaved, const float* bias, const float* q_weight,
+                     const float* k_weight, float eps, const int32_t* positions,
+                     const int32_t* slots, const float* table, int table_rows, float* q,
+                     int8_t* k_cache, int8_t* v_cache, float* k_scales, float* v_scales,
+                     int num_blocks, int block_size, int64_t stride_block, int64_t stride_token,
+                     int64_t stride_head, void* stream);
+
+/* Keys and values of a cache of 8 bits as [N][hkv][D] of type F32, F16 or BF16: rows
+ * starts[b] .. starts[b+1]-1 are request b's tokens from number first[b] on (first
+ * NULL: from 0), zeros where the table has no block, and for rows past starts[B].  starts
+ * [B+1] rises from 0.  D: a multiple of 16, at most 512. */
+int fq_read_cache8(const int8_t* k_cache, const int8_t* v_cache, const float* k_scales,
+                   const float* v_scales, int num_blocks, int block_size, int hkv, int D,
+                   int64_t stride_block, int64_t stride_token, int64_t stride_head,
+                   const int32_t* block_table, int max_blocks, int64_t table_stride,
+                   const int32_t* starts, const int32_t* first, int B, int N, uint32_t type,
+                   void* k_out, void* v_out, void* stream);
+
+/* fq_tree_attention for caches of type F16, BF16 (scales unused) or I8.  With window > 0, a
+ * token at position p sees of these keys the ones at positions j with p - j < window or j <
+ * sinks; a cached token's position is its number, a new one's lengths[b] + its depth, which
+ * is, with masks, the number of its mask's bits less one (each of them a token that is
+ * the parent of the next).  window 0: no window. */
+int fq_window_attention(const float* q, int64_t ldq, const int32_t* lengths, const int32_t* cu,
+                        const uint64_t* masks, int B, int N, int max_new, int hq, int hkv, int D,
+                        float scale, int window, int sinks, uint32_t cache_type,
+                        const void* k_cache, const void* v_cache, const float* k_scales,
+                        const float* v_scales, int num_blocks, int block_size,
+                        int64_t stride_block, int64_t stride_token, int64_t stride_head,
+                        const int32_t* block_table, int max_blocks, int64_t table_stride,
+                        float* out, void* stream);
+
+/* Verifies drafted tokens.  Request b's tokens are cu[b] .. cu[b+1]-1 of N, each with the
+ * logits behind it (type F32, F16 or BF16, rows ld elements apart, V in each).  Token 0 of a request is known; token
+ * i is drafted to follow token parents[i] (a number within the request below i, else it is
+ * reached by nothing; NULL: i - 1).  With p = softmax(row / temperature[b]) (NULL: 1; at 0 or below: 1
+ * for the largest logit, of equal ones the lowest token), from token 0 on, the tokens that follow the
+ * last accepted one are tried in their order, token i with the random number uniforms[i]:
+ *   draft_probs [N][V] (rows ldp apart; chains only): row i is the distribution that token i was
+ *       drawn from; accepted where u q(token) < p(token).  Refused, max(p - q, 0) is left.
+ *   NULL: accepted where u m < p(token), m = 1 - the p of those refused before it (a token
+ *       that was refused already has p = 0).  Left is p without the tokens refused.
+ * Where none is accepted, the next token is drawn from what is left (from p where that is
+ * nothing): the lowest whose cumulated sum is above uniforms[cu[b]] times the whole.
+ *   accepted [B]     accepted tokens, token 0 included; 0 for a request without tokens
+ *   path [N]         path[cu[b] + d]: the number of the d-th accepted token; -1 behind
+ *   next_tokens [B]  the next token; -1 for a request without tokens and after a row that
+ *                    has a NaN or +inf logit or nothing but -inf: nothing is accepted behind it
+ * A drafted token outside 0 .. V-1 is refused.  Uniforms are in [0, 1).  Sums that random numbers are compared with are in
+ * 64 bits.  With parents, tokens from the 65th of a request on are reached by nothing.  N at most 2^20. */
+int fq_verify_draft(const void* logits, uint32_t type, int64_t ld, int V, const int32_t* tokens,
+                    const int32_t* cu, int B, int N, const int32_t* parents,
+                    const float* uniforms, const float* draft_probs, int64_t ldp,
+                    const float* temperature, int32_t* accepted, int32_t* path,
+                    int32_t* next_tokens, void* stream);
+
+/* Moves request b's new tokens path[cu[b] + d] (numbers within the request, as
+ * fq_verify_draft gives them), d < accepted[b], to the slots of its tokens lengths[b] + d: keys
+ * and values of caches of any type, all read before any is written.  Of the first 64 only; those whose path is d,
+ * or no new token, or whose slot is no block's, stay.  Caches of 8 bits: what is moved enters
+ * its groups as in fq_qk_norm_rope8, with y / 127 = its scale * (its largest code / 127).  D: a multiple of
+ * 8 (8 bits: 16), at most 512. */
+int fq_keep_accepted(uint32_t cache_type, void* k_cache, void* v_cache, float* k_scales,
+                     float* v_scales, int num_blocks, int block_size, int hkv, int D,
+                     int64_t stride_block, int64_t stride_token, int64_t stride_head,
+                     const int32_t* block_table, int max_blocks, int64_t table_stride,
+                     const int32_t* lengths, const int32_t* cu, const int32_t* path,
+                     const int32_t* accepted, int B, int N, void* stream);
 
 /* For each of M rows of V logits (type F32, F16 or BF16, rows ld elements apart),
  * with p = softmax(row):
