@@ -26,7 +26,7 @@ ARCH = "gfx950"
 SOURCES = ["fq_dequant.hip", "fq_gemv1.hip", "fq_gemvp.hip", "fq_gemvt.hip", "fq_pack.hip", "fq_mmq.hip",
            "fq_mmqi.hip", "fq_mmqs.hip", "fq_mmqp.hip", "fq_mmqk.hip", "fq_mmqt.hip",
            "fq_plan.hip", "fq_rope.hip", "fq_attn.hip", "fq_logp.hip", "fq_rope8.hip", "fq_cache8.hip",
-           "fq_attn8.hip", "fq_verify.hip", "fq_step_capi.cpp", "fq_capi.cpp"]
+           "fq_attnw.hip", "fq_attn8.hip", "fq_verify.hip", "fq_step_capi.cpp", "fq_capi.cpp"]
 
 COMMON = [
     "-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}",

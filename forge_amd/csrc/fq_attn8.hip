@@ -1,110 +1,704 @@
-// fq_attn8.hip -- attention with a sliding window, or over a cache of 8 bits.
+// fq_attn8.hip -- attention over a cache of 8 bits, with or without a window.
 //
-// A wave takes one token and one query head and walks the keys it sees, 64 at a time.
-#include <hip/hip_runtime.h>
-
-#include <algorithm>
-
+// Items, units and their shares among the work-groups, tiles in rings, scores as K Q^T with the
+// next tile's products beside this one's softmax, and lagging references are those of fq_attn.hip.  What
+// differs: tiles are int8 codes, 32 keys in two groups of 16 that have a scale each.
+//
+// Scores: the fp32 queries, 16 to 23 bits of their row's largest element, are three signed bytes
+// to the power-of-two base 256, so that all products with the codes are int8 matrix instructions
+// with exact sums: no key is converted, and three of them take as long as one and a half of fp16's
+// (two parts).  A score is its integer times the row's and the group's scale.
+//
+// Values: O = sum p s_v c.  Codes become fp16 (exactly: a byte beside 0x64 is 1024 and itself) and
+// p s_v two fp16 parts as in fq_attn.hip.  The references are of the scores plus log2 s_v, so that
+// p s_v stays in fp16's range whatever the groups' scales; the sums are of p.
+#include "fq_attn.h"
 #include "fq_group8.h"
-#include "fq_step.h"
 
 namespace fq {
 namespace {
 
-template <int TYPE>
-__device__ __forceinline__ float element(const uint8_t* base, int64_t at) {
-    if (TYPE == 2) return (float)((const int8_t*)base)[at];
-    const uint16_t b = ((const uint16_t*)base)[at];
-    return TYPE == 1 ? __uint_as_float((uint32_t)b << 16) : (float)__builtin_bit_cast(_Float16, b);
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef float f2 __attribute__((ext_vector_type(2)));
+typedef int i4 __attribute__((ext_vector_type(4)));
+typedef int i2 __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) i2 lds_i2;
+
+constexpr int KT = 32;  // keys of a tile
+constexpr int SUBS = KT / GROUP;
+// By how much (log2) a row's largest score may be above its sums' reference, and what the probabilities'
+// parts are raised by: together they stay below fp16's largest.
+constexpr float LAG = 4.0f;
+constexpr float UP = 2048.0f;
+constexpr float MOST = 8355711.0f;  // 127 (1 + 256 + 65536): the largest that three signed bytes hold
+constexpr int LIMBS = 3;
+
+// Where a token lies in a cache whose page that is, in bytes (where it is no block, in the last one).
+__device__ __forceinline__ uint64_t place_of(const AttnArgs& a, int page, int key) {
+    const uint32_t pg = min((uint32_t)page, (uint32_t)a.c.num_blocks - 1);
+    const uint32_t in = (uint32_t)key & ((1u << a.c.bs_log2) - 1);
+    return (uint64_t)pg * (uint32_t)a.c.sb + (uint64_t)in * (uint32_t)a.c.st;
 }
 
-template <int TYPE>
-__global__ __launch_bounds__(64) void window_kernel(AttnArgs a, int D) {
-    __shared__ float s_q[256], s_p[64];
-    __shared__ int s_slot[64];
-    const int n = blockIdx.x / a.hq, h = blockIdx.x % a.hq, lane = threadIdx.x, kvh = h / a.G;
-    int b = 0, hi = a.B;
-    while (hi - b > 1) {
-        const int mid = (b + hi) >> 1;
-        if (a.cu[mid] <= n) b = mid;
-        else hi = mid;
+// A uniform scale, 0 where it is no positive finite number.
+__device__ __forceinline__ float scale_of(int bits) {
+    return __uint_as_float((uint32_t)(bits - 1) < 0x7F7FFFFFu ? (uint32_t)bits : 0u);
+}
+
+// x0, x1 as two pairs of fp16 that add up to them.  minus1: -1 where the compiler does not see it, so that
+// the rest is one fused multiply-add from the packed part.
+__device__ __forceinline__ void split2(float x0, float x1, float minus1, uint32_t& hi, uint32_t& lo) {
+    const h2 first = __builtin_convertvector((f2{x0, x1}), h2);
+    hi = __builtin_bit_cast(uint32_t, first);
+    asm("" : "+v"(hi));
+    const h2 back = __builtin_bit_cast(h2, hi);
+    const h2 rest = {(_Float16)fmaf((float)back[0], minus1, x0), (_Float16)fmaf((float)back[1], minus1, x1)};
+    lo = __builtin_bit_cast(uint32_t, rest);
+}
+
+// Four codes as fp16: a byte with its sign turned beside 0x64 is 1024 + 128 + code.
+__device__ __forceinline__ void four_halves(uint32_t w, uint32_t& a, uint32_t& b) {
+    const uint32_t x = w ^ 0x80808080u;
+    const h2 off = {(_Float16)-1152.0f, (_Float16)-1152.0f};
+    const h2 lo = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, x, 0x04010400u)) + off;
+    const h2 hi = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, x, 0x04030402u)) + off;
+    a = __builtin_bit_cast(uint32_t, lo);
+    b = __builtin_bit_cast(uint32_t, hi);
+}
+
+// WR x WK waves: each group of WR shares tiles of 32 keys, each of its waves with 16 NR rows of its own; the
+// groups take every WK-th tile.  NS tiles of a group are in LDS.  PC work-groups to a CU.
+template <int D_, int NR_, int WR_, int WK_, int NS_, int PC_>
+struct Shape {
+    static constexpr int D = D_, NR = NR_, WR = WR_, WK = WK_, NS = NS_, PC = PC_;
+    static constexpr int WAVES = WR * WK;
+    static constexpr int PITCH = D <= 64 ? 64 : D <= 128 ? 128 : 256;  // LDS row, bytes
+    static constexpr int RT = 16 * NR * WR;
+    static constexpr int KU = KT * WK;
+    static constexpr int ROWS = 1024 / PITCH;  // rows of one copy
+    static constexpr int J = 16 / ROWS;        // copies of 16 rows
+    static constexpr int NI = SUBS * J;        // copies of a tile's keys, and of its values
+    static constexpr int CW = 2 * NI / WR;     // copies of a wave for a tile
+    // Bytes from copy to copy and (values) from group to group in LDS, and which bits of a row's number change
+    // places of its 16-byte pieces among four: chosen so that the 16 keys of a read of keys, and the
+    // 8 keys that two of the lanes' quarters take of both groups, lie in 16 places of the 256 bytes that
+    // the banks span, with every place an immediate offset from few registers.
+    static constexpr int KSTEP = 1024 + (D == 64 ? 0 : 64);
+    static constexpr int VSTEP = 1024 + (D == 256 ? 64 : 0);
+    static constexpr int VGROUP = J * VSTEP + (D == 64 ? 32 : D == 256 ? 128 : 64);
+    static __device__ __forceinline__ int turn(int row) {
+        return D == 64 ? (row >> 2) & 3 : D == 256 ? row & 3 : (row >> 1) & 3;
     }
-    const int t0 = min(max(a.cu[b], 0), a.N), t1 = min(max(a.cu[b + 1], t0), a.N);
-    float* out = a.out + ((int64_t)n * a.hq + h) * D;
-    if (n < t0 || n >= t1) {
-        for (int d = lane; d < D; d += 64) out[d] = 0.0f;
+    static constexpr int KTILE = NI * KSTEP, VTILE = SUBS * VGROUP, STAGE = KTILE + VTILE;
+    static constexpr int GROUPS = NS * STAGE;
+    // the waves' outputs are exchanged where the tiles were
+    static constexpr size_t LDS = std::max((size_t)WK * GROUPS, WK > 1 ? (size_t)WAVES * NR * 16 * D * 4 : 0);
+    static constexpr int PART = RT * (D + 2);  // floats of a partial result
+    // What an item costs beside its units, in units.
+    static constexpr int OV = 256 / KU;
+    static_assert(2 * NI % WR == 0 && (WR == 1 ? NS >= 2 : NS >= 3), "copies");
+    static_assert(2 * (NS - 1) * NI < 64, "vmcnt");
+    static_assert(D / 16 % WK == 0, "join");
+    static_assert(PC * (LDS + 8 * WK * RT + 64) <= 160 * 1024, "LDS");
+    static_assert(PC <= MAX_GRID && (size_t)PC * PART <= MAX_PART, "workspace");
+};
+
+template <class S>
+__global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void attn8_kernel(AttnArgs a) {
+    constexpr int D = S::D, NR = S::NR, WR = S::WR, WK = S::WK, NS = S::NS;
+    constexpr int RT = S::RT, KU = S::KU, PITCH = S::PITCH, J = S::J, NI = S::NI, ROWS = S::ROWS;
+    constexpr int OV = S::OV;
+    constexpr int STEPS = (D + 63) / 64, DT = D / 16, SLOTS = PITCH / 16;
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+    __shared__ float s_ml[2][WK][RT];
+    const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6);
+    const int wr = wave % WR, wk = wave / WR;
+    const int n16 = lane & 15, g = lane >> 4;
+    const int wg = blockIdx.x;
+
+    // --- the work-group's units (every wave finds them for itself) ---
+    int64_t total, span, off;
+    int b;
+    {
+        const int per = (a.B + 63) / 64, first = lane * per;
+        int64_t mine = 0;
+        for (int i = first; i < min(first + per, a.B); ++i)
+            mine += request<RT, KU, OV, true>(a, a.cu[i], a.cu[i + 1], a.lengths[i]).units;
+        int64_t upto = mine;
+        for (int o = 1; o < 64; o <<= 1) {
+            const int64_t v = __shfl_up(upto, o);
+            if (lane >= o) upto += v;
+        }
+        total = uni64(__shfl(upto, 63));
+        span = (total + gridDim.x - 1) / gridDim.x;
+        const int64_t u0 = wg * span;
+        const uint64_t past = __ballot(upto > u0);
+        const int at = past ? __builtin_ctzll(past) : 0;
+        b = at * per;
+        off = u0 - uni64(__shfl(upto - mine, at));
+    }
+    int* desc = a.desc + MAX_ITEMS + wg * DESC;
+    // padding tokens
+    {
+        const int end = min(max(sload(a.cu + a.B), 0), a.N);
+        const int64_t row = (int64_t)a.hq * D;
+        for (int64_t i = end * row + (int64_t)wg * blockDim.x + tid; i < a.N * row;
+             i += (int64_t)gridDim.x * blockDim.x)
+            a.out[i] = 0.0f;
+    }
+    int64_t u = wg * span;
+    if (u >= total) {
+        if (tid == 0) a.desc[wg] = 0;
         return;
     }
-    const int t = n - t0;
-    const int64_t most = (int64_t)a.max_blocks << a.c.bs_log2;
-    const int keys = (int)min(min((int64_t)max(a.lengths[b], 0) + (t1 - t0), most), (int64_t)INT32_MAX - 4096);
-    const int len = min(max(a.lengths[b], 0), keys);
-    for (int d = lane; d < D; d += 64) s_q[d] = a.q[n * a.ldq + (int64_t)h * D + d] * a.scale;
-    const uint64_t mask = a.masks ? a.masks[n] : 0;
-    const int depth = a.masks ? __builtin_popcountll(mask) - 1 : t;
-    const TableView table{a.table, a.max_blocks, a.table_stride};
-    const int groups = (1 << a.c.bs_log2) / GROUP;
-    float m = -3.4e38f, l = 0.0f, acc[4] = {0, 0, 0, 0};
-    __syncthreads();
-    for (int k0 = 0; k0 < keys; k0 += 64) {
-        const int key = k0 + lane;
-        bool see = key < keys;
-        int place = key;  // its position
-        if (see && key >= len) {
-            const int j = key - len;
-            if (a.masks) {
-                see = j < 64 && (mask >> j & 1);
-                place = see ? len + __builtin_popcountll(mask & ((1ull << j) - 1)) : 0;
-            } else {
-                see = j <= t;
-            }
-        }
-        if (a.window && see) see = len + depth - place < a.window || place < a.sinks;
-        const int slot = see ? table.slot(b, key, a.c) : -1;
-        float s = -__builtin_inff();
-        if (slot >= 0) {
-            const int page = slot >> a.c.bs_log2, row = slot & ((1 << a.c.bs_log2) - 1);
-            const int64_t at = page * a.c.sb + row * a.c.st + (int64_t)kvh * a.c.sh;
-            float dot = 0.0f;
-            for (int d = 0; d < D; ++d) dot = fmaf(s_q[d], element<TYPE>(a.k, at + d), dot);
-            s = TYPE == 2 ? dot * held_scale(a.ks[((int64_t)page * a.hkv + kvh) * groups + row / GROUP]) : dot;
-        }
-        float mx = s;
-        for (int o = 1; o < 64; o <<= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
-        mx = fmaxf(mx, m);
-        const float p = exp2f(s - mx), f = exp2f(m - mx);
-        float sum = p;
-        for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o);
-        l = l * f + sum;
-        m = mx;
-        __syncthreads();
-        s_p[lane] = p;
-        s_slot[lane] = p != 0.0f ? slot : -1;
-        __syncthreads();
-        for (int e = 0; e < 4; ++e) acc[e] *= f;
-        for (int i = 0; i < 64; ++i) {
-            const int sl = s_slot[i];
-            if (sl < 0) continue;
-            const int page = sl >> a.c.bs_log2, row = sl & ((1 << a.c.bs_log2) - 1);
-            const int64_t at = page * a.c.sb + row * a.c.st + (int64_t)kvh * a.c.sh;
-            float w = s_p[i];
-            if (TYPE == 2) w *= held_scale(a.vs[((int64_t)page * a.hkv + kvh) * groups + row / GROUP]);
-            for (int e = 0; e < 4; ++e)
-                if (lane + 64 * e < D) acc[e] = fmaf(w, element<TYPE>(a.v, at + lane + 64 * e), acc[e]);
-        }
+    int64_t left = min(span, total - u);
+    bool cut = false;  // an item begun here goes on in the next work-group
+
+    // --- constants of a lane ---
+    float minus1 = -1.0f;
+    asm("" : "+s"(minus1));
+    const uint32_t gbase = lds_addr(lds) + wk * S::GROUPS;
+    uint32_t src;  // a copy's source: bytes from its first row
+    {
+        const int row = lane / SLOTS, slot = lane % SLOTS;
+        int piece = slot ^ S::turn(row);
+        if (16 * piece >= D) piece -= 4;  // (rows of 6 pieces among 8: the rest meets queries of 0)
+        src = (uint32_t)(row * a.c.st) + piece * 16;
     }
-    for (int e = 0; e < 4; ++e)
-        if (lane + 64 * e < D) out[lane + 64 * e] = l != 0.0f ? acc[e] / l : 0.0f;
+    const uint32_t klane = gbase + n16 / ROWS * S::KSTEP + n16 % ROWS * PITCH + ((g ^ S::turn(n16)) << 4);
+    uint32_t vlane[4];
+    {
+        const int i = n16 >> 1, row = 4 * g + (i & 3);  // of the lanes' 8 keys: 4 of each group
+#pragma unroll
+        for (int d = 0; d < 4; ++d)
+            vlane[d] = gbase + S::KTILE + (i >> 2) * S::VGROUP + row / ROWS * S::VSTEP + row % ROWS * PITCH +
+                       ((d ^ S::turn(row)) << 4) + (n16 & 1) * 8;
+    }
+    const int groups = (1 << a.c.bs_log2) / GROUP;
+
+    for (; left > 0; ++b) {
+        const Request rq = request<RT, KU, OV, true>(a, sload(a.cu + b), sload(a.cu + b + 1), sload(a.lengths + b));
+        const int len = rq.len, keys = rq.keys, nu = rq.nu, t0 = rq.t0, nt = rq.nt;
+        if (off >= rq.units) {
+            off -= rq.units;
+            continue;
+        }
+        int item = 0, pos = 0;
+        if (off) {
+            item = (int)(off / rq.cost);
+            pos = (int)(off % rq.cost);
+        }
+        while (off < rq.units && left > 0) {
+            const int take = (int)min((int64_t)(rq.cost - pos), left);
+            const int first = a.whole ? 0 : max(pos - OV, 0);
+            const int count = a.whole ? nu : max(pos + take - OV, 0) - first;
+            const int64_t start = u - pos;  // the item's
+            u += take;
+            off += take;
+            left -= take;
+            pos = 0;
+            if (count == 0) break;  // (the item's work begins in the next work-group)
+            const int h = item / rq.rts, rt = item % rq.rts;
+            ++item;
+            // --- this group's tiles: wk, wk + WK, .. of the segment's (with a window, units behind the
+            // sinks are left out).  Waves that share tiles keep step: as many tiles for each group ---
+            const auto key_at = [&](int i) {
+                const int unit = first + i;
+                return (unit >= rq.su ? unit + rq.skip : unit) * KU + wk * KT;
+            };
+            const int n = WR > 1 || key_at(count - 1) < keys ? count : count - 1;
+            const int last16 = (keys - 1) & ~15;
+            const uint8_t* kb = a.k + (int64_t)h * a.c.sh;
+            const uint8_t* vb = a.v + (int64_t)h * a.c.sh;
+            const int* table = a.table + b * a.table_stride;
+            // The first key that all of the item's rows see, and all from there on to the context's end.
+            const int clear = a.window ? (int)min((int64_t)len + (a.masks ? 63 : min(nt - 1, (rt * RT + RT - 1) / a.G)) + 1 - a.window,
+                                                  (int64_t)INT32_MAX) : 0;
+            // A tile's pages, read ahead; the places of its groups in a cache and their scales;
+            // its copies.  (Past the last key: its page again.)
+            const auto key_of = [&](int i, int hf) { return min(key_at(i) + 16 * hf, last16); };
+            int page[SUBS];
+            const auto read_pages = [&](int i) {
+#pragma unroll
+                for (int hf = 0; hf < SUBS; ++hf) page[hf] = sload(table + (key_of(i, hf) >> a.c.bs_log2));
+            };
+            uint64_t at_k[SUBS], at_v[SUBS];  // of the tiles whose keys, values are copied next
+            uint32_t highest = 0;             // of the pages placed so far (unsigned: -1 is above all blocks)
+            const auto place = [&](int i) {
+#pragma unroll
+                for (int hf = 0; hf < SUBS; ++hf) {
+                    at_v[hf] = at_k[hf];
+                    at_k[hf] = place_of(a, page[hf], key_of(i, hf));
+                    highest = max(highest, (uint32_t)page[hf]);
+                }
+            };
+            const auto scales_at = [&](int i, int hf) {
+                const int key = key_of(i, hf);
+                const uint32_t pg = min((uint32_t)sload(table + (key >> a.c.bs_log2)), (uint32_t)a.c.num_blocks - 1);
+                return ((int64_t)pg * a.hkv + h) * groups + (((uint32_t)key & ((1u << a.c.bs_log2) - 1)) / GROUP);
+            };
+            // The keys of a tile that lie in a block.
+            const auto there = [&](int i) {
+                uint32_t m = ~0u;
+#pragma unroll
+                for (int hf = 0; hf < SUBS; ++hf)
+                    if (no_block(a, sload(table + (key_of(i, hf) >> a.c.bs_log2)))) m &= ~(0xFFFFu << (16 * hf));
+                return m;
+            };
+            const int64_t step = ROWS * a.c.st;  // bytes from copy to copy
+            const auto copy_k = [&](int stage) {
+#pragma unroll
+                for (int hf = 0; hf < SUBS; ++hf) {
+                    const uint8_t* at = kb + at_k[hf];
+#pragma unroll
+                    for (int j = 0; j < J; ++j, at += step)
+                        dma16s(src, at, gbase + stage * S::STAGE + (hf * J + j) * S::KSTEP);
+                }
+            };
+            const auto copy_v = [&](int stage) {
+#pragma unroll
+                for (int hf = 0; hf < SUBS; ++hf) {
+                    const uint8_t* at = vb + at_v[hf];
+#pragma unroll
+                    for (int j = 0; j < J; ++j, at += step)
+                        dma16s(src, at, gbase + stage * S::STAGE + S::KTILE + hf * S::VGROUP + j * S::VSTEP);
+                }
+            };
+            // This wave's share of a tile's keys and of the one before's values: copies wr, wr + WR, .. of the
+            // NI of keys and the NI of values, copy c being number c % J of group c / J.
+            const auto copy_share = [&](bool ks, int kstage, bool vs, int vstage) {
+#pragma unroll
+                for (int x = 0; x < S::CW; ++x) {
+                    const int c = WR * x + wr;
+                    const bool isv = c >= NI;
+                    const int i = isv ? c - NI : c, hf = i / J, j = i % J;
+                    const uint64_t in = j * step;
+                    if (isv) {
+                        if (vs) dma16s(src, vb + ((hf ? at_v[1] : at_v[0]) + in),
+                                       gbase + vstage * S::STAGE + S::KTILE + hf * S::VGROUP + j * S::VSTEP);
+                    } else if (ks) {
+                        dma16s(src, kb + ((hf ? at_k[1] : at_k[0]) + in), gbase + kstage * S::STAGE + i * S::KSTEP);
+                    }
+                }
+            };
+
+            at_k[0] = at_k[1] = 0;
+            read_pages(0);
+            if constexpr (WR == 1) {
+                // K0 V0 K1 V1 ..; then the keys of tile i + NS once tile i's are used, and its values once those are
+#pragma unroll
+                for (int i = 0; i < NS; ++i) {
+                    place(i);
+                    at_v[0] = at_k[0], at_v[1] = at_k[1];
+                    read_pages(i + 1);
+                    if (i < n) {
+                        copy_k(i);
+                        copy_v(i);
+                    }
+                }
+            } else {
+                // K0, K1 V0, K2 V1, ..: each step's batch has the keys of one tile and the values of the one before
+#pragma unroll
+                for (int i = 0; i < NS; ++i) {
+                    place(i);
+                    read_pages(i + 1);
+                    copy_share(i < n, i, i > 0 && i <= n, i - 1);
+                }
+            }
+            // --- queries (on their way while the first tiles are): bytes of the row's largest's 2^-23 ---
+            i4 qf[NR][STEPS][LIMBS];
+            float rs[NR];
+            uint64_t mask[NR];
+            int from[NR];
+#pragma unroll
+            for (int c = 0; c < NR; ++c) {
+                const int r = rt * RT + wr * 16 * NR + 16 * c + n16;
+                const int t = r / a.G, hh = h * a.G + r % a.G;
+                const bool on = t < nt;
+                // (a chain: how many of the new tokens the row sees)
+                mask[c] = !on ? 0 : a.masks ? a.masks[t0 + t] : (uint64_t)t + 1;
+                from[c] = 0;
+                if (on) {
+                    const Reach reached = reach(a, len, t, mask[c]);
+                    mask[c] = reached.mask, from[c] = reached.from;
+                }
+                const float* q = a.q + (int64_t)(t0 + (on ? t : 0)) * a.ldq + (int64_t)(on ? hh : 0) * D;
+                f4 x[STEPS][4];
+                float mx = 0.0f;
+                bool finite = true;
+#pragma unroll
+                for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const bool in = on && (D % 64 == 0 || 64 * s + 16 * g < D);
+                        x[s][i] = in ? *(const f4u*)(q + 64 * s + 16 * g + 4 * i) : f4{0, 0, 0, 0};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            finite &= fabsf(x[s][i][e]) < __builtin_inff();
+                            mx = fmaxf(mx, fabsf(x[s][i][e]));
+                        }
+                    }
+                mx = max4(finite ? mx : __builtin_inff());
+                float up = 0.0f, down = 1.0f;
+                if (mx < __builtin_inff()) {
+                    int e = min(23 - __builtin_amdgcn_frexp_expf(mx), 126);
+                    if (ldexpf(mx, e) > MOST) --e;
+                    up = mx > 0.0f ? ldexpf(1.0f, e) : 0.0f;
+                    down = ldexpf(1.0f, -e);
+                }
+                // (the scale's sign goes with the query: the largest score is that of the largest
+                // product; a row that is not finite has no score that is a number)
+                up = copysignf(up, a.scale);
+                rs[c] = mx < __builtin_inff() ? down * 256.0f * fabsf(a.scale) : __builtin_nanf("");
+#pragma unroll
+                for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        uint32_t v[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)  // a byte and 128 in each place
+                            v[e] = (uint32_t)((mx < __builtin_inff() ? (int)rintf(x[s][i][e] * up) : 0) + 0x808080);
+                        const uint32_t lo = __builtin_amdgcn_perm(v[1], v[0], 0x05010400u);  // bytes 0, 1 of two
+                        const uint32_t hi = __builtin_amdgcn_perm(v[3], v[2], 0x05010400u);
+                        const uint32_t top = __builtin_amdgcn_perm(v[1], v[0], 0x0C0C0602u) |
+                                             __builtin_amdgcn_perm(v[3], v[2], 0x06020C0Cu);
+                        qf[c][s][0][i] = (int)(top ^ 0x80808080u);
+                        qf[c][s][1][i] = (int)(__builtin_amdgcn_perm(hi, lo, 0x07060302u) ^ 0x80808080u);
+                        qf[c][s][2][i] = (int)(__builtin_amdgcn_perm(hi, lo, 0x05040100u) ^ 0x80808080u);
+                    }
+            }
+
+            f4 o[DT][NR];
+            float mrow[NR], lrow[NR];
+#pragma unroll
+            for (int c = 0; c < NR; ++c) {
+                mrow[c] = LOWEST;
+                lrow[c] = 0.0f;
+#pragma unroll
+                for (int d = 0; d < DT; ++d) o[d][c] = f4{0, 0, 0, 0};
+            }
+            // Products of the keys at `at`, STEPS times LIMBS SUBS NR matrix instructions with beside(piece)
+            // after each of STEPS LIMBS runs of them; scores are their bytes' sums over 256.
+            const auto products = [&](uint32_t at, f4 (&sc)[SUBS][NR], const auto& beside) {
+                i4 acc[LIMBS][SUBS][NR];
+                i4 kf[2][SUBS];
+                const auto keys_of = [&](int s, i4 (&k)[SUBS]) {
+#pragma unroll
+                    for (int sub = 0; sub < SUBS; ++sub)
+                        k[sub] = __builtin_bit_cast(i4, *(lds_u4*)(uintptr_t)(klane + at + J * sub * S::KSTEP + 64 * s));
+                };
+                keys_of(0, kf[0]);
+#pragma unroll
+                for (int s = 0; s < STEPS; ++s) {
+                    if (s + 1 < STEPS) keys_of(s + 1, kf[(s + 1) & 1]);
+#pragma unroll
+                    for (int l = 0; l < LIMBS; ++l) {
+#pragma unroll
+                        for (int sub = 0; sub < SUBS; ++sub)
+#pragma unroll
+                            for (int c = 0; c < NR; ++c)
+                                acc[l][sub][c] = __builtin_amdgcn_mfma_i32_16x16x64_i8(
+                                    kf[s & 1][sub], qf[c][s][l], s ? acc[l][sub][c] : i4{0, 0, 0, 0}, 0, 0, 0);
+                        __builtin_amdgcn_sched_barrier(0);
+                        beside(s * LIMBS + l);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                }
+                // (the upper two together stay below 2^31: 127 128 256 (256 + 1))
+#pragma unroll
+                for (int sub = 0; sub < SUBS; ++sub)
+#pragma unroll
+                    for (int c = 0; c < NR; ++c)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            sc[sub][c][r] = fmaf((float)acc[2][sub][c][r], 1.0f / 256.0f,
+                                                 (float)((acc[0][sub][c][r] << 8) + acc[1][sub][c][r]));
+            };
+            f4 sc[SUBS][NR];
+            int kbits[SUBS], vbits[SUBS];  // the scales of the tile whose softmax is next
+            const auto read_scales = [&](int i) {
+#pragma unroll
+                for (int hf = 0; hf < SUBS; ++hf) {
+                    const int64_t at = scales_at(i, hf);
+                    kbits[hf] = sload((const int*)a.ks + at);
+                    vbits[hf] = sload((const int*)a.vs + at);
+                }
+            };
+            read_scales(0);
+            if constexpr (WR == 1) {
+                if (n >= NS) wait_vm<(2 * NS - 1) * NI>();
+                else wait_vm<0>();
+            } else {
+                if (n >= NS) wait_vm<(NS - 1) * S::CW>();
+                else wait_vm<0>();
+                lds_barrier();
+            }
+            products(0, sc, [](int) {});
+            int stage = 0;
+            for (int i = 0; i < n; ++i) {
+                const int key0 = key_at(i);
+                const int stage1 = stage + 1 < NS ? stage + 1 : 0;
+                // this tile's values and the next one's keys have landed: this wave's copies of them, then
+                // everyone's; and all are done with this one's keys and the last one's values, whose places are
+                // filled anew
+                if constexpr (WR == 1) {
+                    wait_lds();
+                    if (i + NS < n) {
+                        place(i + NS);
+                        read_pages(i + NS + 1);
+                        copy_k(stage);
+                        wait_vm<2 * (NS - 1) * NI>();
+                    } else if (NS > 2 && i + 2 < n) {
+                        if (NS > 3 && i + 3 < n) wait_vm<5 * NI>();
+                        else wait_vm<3 * NI>();
+                    } else if (i + 1 < n) {
+                        wait_vm<NI>();
+                    } else {
+                        wait_vm<0>();
+                    }
+                } else {
+                    if (i + NS - 1 < n) wait_vm<(NS - 2) * S::CW>();
+                    else wait_vm<0>();
+                    lds_barrier();
+                    if (i + NS - 1 < n) {
+                        place(i + NS);
+                        read_pages(i + NS + 1);
+                        copy_share(i + NS < n, stage, true, stage ? stage - 1 : NS - 1);
+                    }
+                }
+                const bool holes = no_block(a, (int)highest);
+                const bool tail = holes || key0 + KT > len || (key0 < clear && key0 + KT > a.sinks);
+                float mul[SUBS][NR], sv[SUBS], lift[SUBS];
+#pragma unroll
+                for (int sub = 0; sub < SUBS; ++sub) {
+                    const float sk = scale_of(kbits[sub]);
+                    sv[sub] = scale_of(vbits[sub]);
+                    // (any number near log2 sv; a group of zeros still has its part in the sums)
+                    lift[sub] = fmaxf(__builtin_amdgcn_logf(sv[sub]), -80.0f);
+#pragma unroll
+                    for (int c = 0; c < NR; ++c) mul[sub][c] = rs[c] * sk;
+                }
+                if (i + 1 < n) read_scales(i + 1);
+                if (tail) {
+                    const int old = len - key0, all = keys - key0;
+                    const uint32_t in = holes ? there(i) : ~0u;
+#pragma unroll
+                    for (int c = 0; c < NR; ++c) {
+                        const uint32_t see = (seen<true>(a, mask[c], from[c], key0, old, all) & in) >> (4 * g);
+#pragma unroll
+                        for (int sub = 0; sub < SUBS; ++sub) {
+#pragma unroll
+                            for (int r = 0; r < 4; ++r)
+                                sc[sub][c][r] = see >> (16 * sub + r) & 1 ? sc[sub][c][r] * mul[sub][c]
+                                                                          : -__builtin_inff();
+                            mul[sub][c] = 1.0f;
+                        }
+                    }
+                }
+
+                // the next tile's products (of whatever is there, after the last) beside this one's softmax
+                f4 next[SUBS][NR];
+                u4 ph[NR], pl[NR];  // the probabilities' parts
+                float alpha[NR], sum[NR];
+                bool moved = false;
+                const auto maximum = [&](int c) {
+                    float mx = LOWEST;
+#pragma unroll
+                    for (int sub = 0; sub < SUBS; ++sub) {
+                        const f4 v = sc[sub][c];
+                        mx = fmaxf(mx, fmaf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), mul[sub][c], lift[sub]));
+                    }
+                    mx = max4(mx);
+                    // the sums' reference follows the maximum in steps: exponentials of up to 2^LAG are as
+                    // good as those up to 1
+                    const float m = mx > mrow[c] + LAG ? mx : mrow[c];
+                    moved |= m > mrow[c];
+                    alpha[c] = __builtin_amdgcn_exp2f(mrow[c] - m);
+                    mrow[c] = m;
+                    sum[c] = 0.0f;
+                };
+                const auto exponentials = [&](int c, int sub) {
+                    float p[4];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        p[r] = __builtin_amdgcn_exp2f(fmaf(sc[sub][c][r], mul[sub][c], -mrow[c]));
+                        sum[c] += p[r];
+                        p[r] *= UP * sv[sub];
+                    }
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        uint32_t hi, lo;
+                        split2(p[2 * e], p[2 * e + 1], minus1, hi, lo);
+                        ph[c][2 * sub + e] = hi;
+                        pl[c][2 * sub + e] = lo;
+                    }
+                    if (sub == SUBS - 1) lrow[c] = lrow[c] * alpha[c] + sum[c];
+                };
+                __builtin_amdgcn_s_setprio(1);
+                products(stage1 * S::STAGE, next, [&](int s) {
+                    // the rows' maxima, then their groups' exponentials, spread over the runs
+                    constexpr int PIECES = (1 + SUBS) * NR, RUNS = STEPS * LIMBS;
+#pragma unroll
+                    for (int x = s * PIECES / RUNS; x < (s + 1) * PIECES / RUNS; ++x) {
+                        if (x < NR) maximum(x);
+                        else exponentials((x - NR) / SUBS, (x - NR) % SUBS);
+                    }
+                });
+                __builtin_amdgcn_s_setprio(0);
+                if (__any(moved))
+#pragma unroll
+                    for (int c = 0; c < NR; ++c)
+#pragma unroll
+                        for (int d = 0; d < DT; ++d) o[d][c] *= alpha[c];
+
+                const auto value = [&](int d) {
+                    const uint32_t at = vlane[d & 3] + stage * S::STAGE + (d >> 2) * 64;
+                    const i2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i2*)(uintptr_t)at);
+                    const uint32_t w0 = (uint32_t)w[0], w1 = (uint32_t)w[1];
+                    u4 r;
+                    uint32_t x, y;
+                    four_halves(w0, x, y);
+                    r[0] = x, r[1] = y;
+                    four_halves(w1, x, y);
+                    r[2] = x, r[3] = y;
+                    return __builtin_bit_cast(h8, r);
+                };
+#pragma unroll
+                for (int d = 0; d < DT; d += 2) {
+                    const h8 vf[2] = {value(d), value(d + 1)};
+#pragma unroll
+                    for (int l = 1; l >= 0; --l)
+#pragma unroll
+                        for (int x = 0; x < 2; ++x)
+#pragma unroll
+                            for (int c = 0; c < NR; ++c)
+                                o[d + x][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                                    vf[x], __builtin_bit_cast(h8, l ? pl[c] : ph[c]), o[d + x][c], 0, 0, 0);
+                }
+                if constexpr (WR == 1) {
+                    wait_lds();
+                    if (i + NS < n) {
+                        at_v[0] = at_k[0], at_v[1] = at_k[1];
+                        copy_v(stage);
+                    }
+                }
+#pragma unroll
+                for (int sub = 0; sub < SUBS; ++sub)
+#pragma unroll
+                    for (int c = 0; c < NR; ++c) sc[sub][c] = next[sub][c];
+                stage = stage1;
+            }
+
+            // --- join the groups: each takes D / WK of the columns ---
+            int ln = lane;  // (opaque: addresses made from it are not kept through the tiles)
+            asm volatile("" : "+v"(ln));
+#pragma unroll
+            for (int c = 0; c < NR; ++c) {
+                lrow[c] = sum4(lrow[c]);
+                if (ln < 16) {
+                    s_ml[0][wk][16 * (wr * NR + c) + ln % 16] = mrow[c];
+                    s_ml[1][wk][16 * (wr * NR + c) + ln % 16] = lrow[c];
+                }
+            }
+            lds_barrier();
+            float* buf = (float*)lds;  // the tiles are not needed any more
+            float lsum[NR];
+#pragma unroll
+            for (int c = 0; c < NR; ++c) {
+                const int rl = 16 * (wr * NR + c) + ln % 16;
+                float m = LOWEST;
+#pragma unroll
+                for (int w = 0; w < WK; ++w) m = fmaxf(m, s_ml[0][w][rl]);
+                lsum[c] = 0.0f;
+#pragma unroll
+                for (int w = 0; w < WK; ++w)
+                    lsum[c] += s_ml[1][w][rl] * __builtin_amdgcn_exp2f(s_ml[0][w][rl] - m);
+                const float f = __builtin_amdgcn_exp2f(mrow[c] - m) * (1.0f / UP);
+                mrow[c] = m;
+#pragma unroll
+                for (int d = 0; d < DT; ++d) {
+                    o[d][c] *= f;
+                    if (WK > 1) *(f4*)(buf + (((wave * NR + c) * DT + d) * 64 + ln) * 4) = o[d][c];
+                }
+            }
+            lds_barrier();
+            const bool whole = count == nu;
+            float* part = a.part + (int64_t)(2 * wg + (first == 0)) * S::PART;
+#pragma unroll
+            for (int c = 0; c < NR; ++c) {
+                const int rl = 16 * (wr * NR + c) + ln % 16, r = rt * RT + rl;
+                const int t = r / a.G, hh = h * a.G + r % a.G;
+                const float inv = lsum[c] != 0.0f ? 1.0f / lsum[c] : 0.0f;
+                float* to = whole ? a.out + ((int64_t)(t0 + t) * a.hq + hh) * D : part + rl * D;
+#pragma unroll
+                for (int d0 = 0; d0 < DT / WK; ++d0) {
+                    const int d = wk * (DT / WK) + d0;
+                    f4 v;
+                    if (WK > 1) {
+                        v = f4{0, 0, 0, 0};
+#pragma unroll
+                        for (int w = 0; w < WK; ++w)
+                            v += *(const f4*)(buf + ((((w * WR + wr) * NR + c) * DT + d) * 64 + ln) * 4);
+                    } else {
+                        v = o[d0][c];
+                    }
+                    if (whole) v = lsum[c] != 0.0f ? v * inv : f4{0, 0, 0, 0};
+                    if (t < nt) *(f4*)(to + 16 * d + 4 * (ln / 16)) = v;
+                }
+                if (!whole && wk == 0 && ln < 16 && t < nt) {
+                    part[RT * D + rl] = mrow[c];
+                    part[RT * D + RT + rl] = lsum[c];
+                }
+            }
+            if (first == 0 && !whole) {
+                cut = true;
+                if (tid == 0) {
+                    const int64_t end = start + OV + nu - 1;  // the item's last unit
+                    a.desc[wg] = (int)(end / span) - wg + 1;
+                    desc[0] = t0, desc[1] = nt, desc[2] = h, desc[3] = rt;
+                }
+            }
+            lds_barrier();  // the exchanged outputs are read
+        }
+        off -= rq.units;
+    }
+    if (!cut && tid == 0) a.desc[wg] = 0;
+}
+
+template <class S>
+hipError_t go(AttnArgs a, int cus, uint8_t* ws, hipStream_t st) {
+    a.grid = std::min(S::PC * cus, MAX_ITEMS);
+    a.desc = (int*)ws;
+    a.part = (float*)(ws + DESC_BYTES);
+    // (as for 16 bits: short tables are not cut)
+    a.whole = (int64_t)a.max_blocks << a.c.bs_log2 <= 6 * std::max(S::KU, 64);
+    hipLaunchKernelGGL(attn8_kernel<S>, dim3(a.grid), dim3(64 * S::WAVES), S::LDS, st, a);
+    if (!a.whole) hipLaunchKernelGGL((attn_join<S::D, S::RT>), dim3(JOIN_WGS * cus), dim3(256), 0, st, a);
+    return hipGetLastError();
+}
+
+template <int D>
+hipError_t rows(const AttnArgs& a, int max_new, int cus, uint8_t* ws, hipStream_t st) {
+    const int64_t r = (int64_t)max_new * a.G;
+    if constexpr (D == 256) {
+        if (r <= 16) return go<Shape<D, 1, 1, 2, 2, 2>>(a, cus, ws, st);
+        return go<Shape<D, 1, 4, 1, 3, 1>>(a, cus, ws, st);
+    } else {
+        if (r <= 16) return go<Shape<D, 1, 1, 2, 4, 2>>(a, cus, ws, st);
+        if (r <= 32) return go<Shape<D, 2, 1, 2, 4, 2>>(a, cus, ws, st);
+        return go<Shape<D, 1, 4, 1, 4, 3>>(a, cus, ws, st);
+    }
 }
 
 }  // namespace
 
-hipError_t launch_attn_window(const AttnArgs& a, int type, int D, int, int, uint8_t*, hipStream_t st) {
-    const dim3 g((unsigned)((int64_t)a.N * a.hq)), t(64);
-    if (type == 0) hipLaunchKernelGGL(window_kernel<0>, g, t, 0, st, a, D);
-    else if (type == 1) hipLaunchKernelGGL(window_kernel<1>, g, t, 0, st, a, D);
-    else hipLaunchKernelGGL(window_kernel<2>, g, t, 0, st, a, D);
-    return hipGetLastError();
+hipError_t launch_attn8(const AttnArgs& a, int D, int max_new, int cus, uint8_t* ws, hipStream_t st) {
+    switch (D) {
+        case 64: return rows<64>(a, max_new, cus, ws, st);
+        case 96: return rows<96>(a, max_new, cus, ws, st);
+        case 128: return rows<128>(a, max_new, cus, ws, st);
+        default: return rows<256>(a, max_new, cus, ws, st);
+    }
 }
 
 }  // namespace fq

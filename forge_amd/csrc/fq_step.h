@@ -66,9 +66,10 @@ struct AttnArgs {
 size_t attn_part_bytes(int cus);  // of the largest call
 hipError_t launch_attn(const AttnArgs& a, bool bf16, int D, int max_new, int cus, uint8_t* ws,
                        hipStream_t st);
-// With a window, or over a cache of 8 bits (type 0: fp16, 1: bf16, 2: 8 bits).
-hipError_t launch_attn_window(const AttnArgs& a, int type, int D, int max_new, int cus, uint8_t* ws,
-                              hipStream_t st);
+// The same with a window (window 0: none); over a cache of 8 bits, with and without.
+hipError_t launch_attn_window16(const AttnArgs& a, bool bf16, int D, int max_new, int cus, uint8_t* ws,
+                                hipStream_t st);
+hipError_t launch_attn8(const AttnArgs& a, int D, int max_new, int cus, uint8_t* ws, hipStream_t st);
 
 // A cache of 8 bits: codes at a CacheView's places (elements of one byte) and scales
 // [block][kv head][16 tokens].

@@ -346,9 +346,11 @@ int fq_window_attention(const float* q, int64_t ldq, const int32_t* lengths, con
     uint8_t* ws = nullptr;
     const int rs = lease.get(step_bytes(cus), st, &ws);
     if (rs != FQ_OK) return rs;
-    if (codes || window)
-        return done(fq::launch_attn_window(a, codes ? 2 : cache_type == FQ_TYPE_BF16, D, std::min(max_new, N), cus, ws, st));
-    return done(fq::launch_attn(a, cache_type == FQ_TYPE_BF16, D, std::min(max_new, N), cus, ws, st));
+    const bool bf16 = cache_type == FQ_TYPE_BF16;
+    max_new = std::min(max_new, N);
+    if (codes) return done(fq::launch_attn8(a, D, max_new, cus, ws, st));
+    return done(window ? fq::launch_attn_window16(a, bf16, D, max_new, cus, ws, st)
+                       : fq::launch_attn(a, bf16, D, max_new, cus, ws, st));
 }
 
 int fq_token_logprobs(const void* logits, uint32_t type, int64_t ld, int M, int V,

@@ -160,7 +160,7 @@ int fq_read_cache8(const int8_t* k_cache, const int8_t* v_cache, const float* k_
  * token at position p sees of these keys the ones at positions j with p - j < window or j <
  * sinks; a cached token's position is its number, a new one's lengths[b] + its depth, which
  * is, with masks, the number of its mask's bits less one (each of them a token that is
- * the parent of the next).  window 0: no window. */
+ * the parent of the next; 0 for a mask of none).  window 0: no window. */
 int fq_window_attention(const float* q, int64_t ldq, const int32_t* lengths, const int32_t* cu,
                         const uint64_t* masks, int B, int N, int max_new, int hq, int hkv, int D,
                         float scale, int window, int sinks, uint32_t cache_type,

@@ -25,8 +25,7 @@ def sees(length, n, masks, window, sinks):
     for i in range(n):
         bits = {j for j in range(i + 1)} if masks is None else {j for j in range(min(n, 64)) if int(masks[i]) >> j & 1}
         draft.append(bits)
-        place[length + i] = length + len({j for j in range(64 if masks is not None else i + 1) if
-                                          masks is None or int(masks[i]) >> j & 1}) - 1
+        place[length + i] = length + (i if masks is None else max(bin(int(masks[i]) % 2 ** 64).count("1") - 1, 0))
         for j in bits:
             see[i, length + j] = True
     if window:
