@@ -38,8 +38,9 @@ COMMON = [
 # Per-file flags.  The prefill kernel adds one FMA per block to each of its 64
 # MFMA results per lane: with the results in AGPRs (the compiler's default
 # under that register pressure) every FMA needs a v_accvgpr_read first, so
-# the MFMA results are kept in VGPRs.
-EXTRA = {f: ["-mllvm", "-amdgpu-mfma-vgpr-form"] for f in ("fq_mmqp.hip", "fq_mmqk.hip", "fq_mmqt.hip")}
+# the MFMA results are kept in VGPRs.  So are the 8-bit attention's, whose scores are
+# put together from three integers each.
+EXTRA = {f: ["-mllvm", "-amdgpu-mfma-vgpr-form"] for f in ("fq_mmqp.hip", "fq_mmqk.hip", "fq_mmqt.hip", "fq_attn8.hip")}
 
 
 def _compile(src: str) -> str:

@@ -33,16 +33,9 @@ constexpr float UP = 2048.0f;
 constexpr float MOST = 8355711.0f;  // 127 (1 + 256 + 65536): the largest that three signed bytes hold
 constexpr int LIMBS = 3;
 
-// Where a token lies in a cache whose page that is, in bytes (where it is no block, in the last one).
-__device__ __forceinline__ uint64_t place_of(const AttnArgs& a, int page, int key) {
-    const uint32_t pg = min((uint32_t)page, (uint32_t)a.c.num_blocks - 1);
-    const uint32_t in = (uint32_t)key & ((1u << a.c.bs_log2) - 1);
-    return (uint64_t)pg * (uint32_t)a.c.sb + (uint64_t)in * (uint32_t)a.c.st;
-}
-
-// A uniform scale, 0 where it is no positive finite number.
-__device__ __forceinline__ float scale_of(int bits) {
-    return __uint_as_float((uint32_t)(bits - 1) < 0x7F7FFFFFu ? (uint32_t)bits : 0u);
+// a / b, in 32 bits where that does (a 64-bit division takes a third of a microsecond).
+__device__ __forceinline__ int64_t divided(int64_t a, int64_t b) {
+    return (uint64_t)(a | b) >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
 }
 
 // x0, x1 as two pairs of fp16 that add up to them.  minus1: -1 where the compiler does not see it, so that
@@ -78,7 +71,7 @@ struct Shape {
     static constexpr int ROWS = 1024 / PITCH;  // rows of one copy
     static constexpr int J = 16 / ROWS;        // copies of 16 rows
     static constexpr int NI = SUBS * J;        // copies of a tile's keys, and of its values
-    static constexpr int CW = 2 * NI / WR;     // copies of a wave for a tile
+    static constexpr int CW = 2 * NI / WR + 1;  // copies of a wave for a tile, its scales' among them
     // Bytes from copy to copy and (values) from group to group in LDS, and which bits of a row's number change
     // places of its 16-byte pieces among four: chosen so that the 16 keys of a read of keys, and the
     // 8 keys that two of the lanes' quarters take of both groups, lie in 16 places of the 256 bytes that
@@ -89,7 +82,8 @@ struct Shape {
     static __device__ __forceinline__ int turn(int row) {
         return D == 64 ? (row >> 2) & 3 : D == 256 ? row & 3 : (row >> 1) & 3;
     }
-    static constexpr int KTILE = NI * KSTEP, VTILE = SUBS * VGROUP, STAGE = KTILE + VTILE;
+    static constexpr int KTILE = NI * KSTEP, VTILE = SUBS * VGROUP;
+    static constexpr int SCALES = KTILE + VTILE, STAGE = SCALES + 256;  // (the scales of 16 lanes' four each)
     static constexpr int GROUPS = NS * STAGE;
     // the waves' outputs are exchanged where the tiles were
     static constexpr size_t LDS = std::max((size_t)WK * GROUPS, WK > 1 ? (size_t)WAVES * NR * 16 * D * 4 : 0);
@@ -97,8 +91,7 @@ struct Shape {
     // What an item costs beside its units, in units.
     static constexpr int OV = 256 / KU;
     static_assert(2 * NI % WR == 0 && (WR == 1 ? NS >= 2 : NS >= 3), "copies");
-    static_assert(2 * (NS - 1) * NI < 64, "vmcnt");
-    static_assert(D / 16 % WK == 0, "join");
+    static_assert(NI + (NS - 1) * (2 * NI + 1) < 64, "vmcnt");
     static_assert(PC * (LDS + 8 * WK * RT + 64) <= 160 * 1024, "LDS");
     static_assert(PC <= MAX_GRID && (size_t)PC * PART <= MAX_PART, "workspace");
 };
@@ -119,18 +112,23 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
     // --- the work-group's units (every wave finds them for itself) ---
     int64_t total, span, off;
     int b;
+    // (up to 64 requests stay in the lanes, so that a request's numbers are not fetched again)
+    const int per = (a.B + 63) / 64;
+    int cu0 = 0, cu1 = 0, cached = 0;
     {
-        const int per = (a.B + 63) / 64, first = lane * per;
+        const int first = lane * per;
         int64_t mine = 0;
-        for (int i = first; i < min(first + per, a.B); ++i)
-            mine += request<RT, KU, OV, true>(a, a.cu[i], a.cu[i + 1], a.lengths[i]).units;
+        for (int i = first; i < min(first + per, a.B); ++i) {
+            cu0 = a.cu[i], cu1 = a.cu[i + 1], cached = a.lengths[i];
+            mine += request<RT, KU, OV, true>(a, cu0, cu1, cached).units;
+        }
         int64_t upto = mine;
         for (int o = 1; o < 64; o <<= 1) {
             const int64_t v = __shfl_up(upto, o);
             if (lane >= o) upto += v;
         }
         total = uni64(__shfl(upto, 63));
-        span = (total + gridDim.x - 1) / gridDim.x;
+        span = divided(total + gridDim.x - 1, gridDim.x);
         const int64_t u0 = wg * span;
         const uint64_t past = __ballot(upto > u0);
         const int at = past ? __builtin_ctzll(past) : 0;
@@ -158,12 +156,17 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
     float minus1 = -1.0f;
     asm("" : "+s"(minus1));
     const uint32_t gbase = lds_addr(lds) + wk * S::GROUPS;
-    uint32_t src;  // a copy's source: bytes from its first row
+    // a copy's source: bytes from the first row of its 16; and of this wave's share of the copies
+    uint32_t src[J], mine[2 * NI / WR];
     {
         const int row = lane / SLOTS, slot = lane % SLOTS;
         int piece = slot ^ S::turn(row);
         if (16 * piece >= D) piece -= 4;  // (rows of 6 pieces among 8: the rest meets queries of 0)
-        src = (uint32_t)(row * a.c.st) + piece * 16;
+        const uint32_t at = (uint32_t)(row * a.c.st) + piece * 16;
+#pragma unroll
+        for (int j = 0; j < J; ++j) src[j] = at + (uint32_t)(j * ROWS * a.c.st);
+#pragma unroll
+        for (int x = 0; x < 2 * NI / WR; ++x) mine[x] = at + (uint32_t)((WR * x + wr) % J * ROWS * a.c.st);
     }
     const uint32_t klane = gbase + n16 / ROWS * S::KSTEP + n16 % ROWS * PITCH + ((g ^ S::turn(n16)) << 4);
     uint32_t vlane[4];
@@ -174,10 +177,15 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
             vlane[d] = gbase + S::KTILE + (i >> 2) * S::VGROUP + row / ROWS * S::VSTEP + row % ROWS * PITCH +
                        ((d ^ S::turn(row)) << 4) + (n16 & 1) * 8;
     }
-    const int groups = (1 << a.c.bs_log2) / GROUP;
+    // lane l's of a tile's scales: of the keys' two groups, then the values'
+    const uint8_t* scales = (const uint8_t*)(lane & 2 ? a.vs : a.ks);
 
     for (; left > 0; ++b) {
-        const Request rq = request<RT, KU, OV, true>(a, sload(a.cu + b), sload(a.cu + b + 1), sload(a.lengths + b));
+        const Request rq = per == 1 ? request<RT, KU, OV, true>(a, __builtin_amdgcn_readlane(cu0, b),
+                                                                __builtin_amdgcn_readlane(cu1, b),
+                                                                __builtin_amdgcn_readlane(cached, b))
+                                    : request<RT, KU, OV, true>(a, sload(a.cu + b), sload(a.cu + b + 1),
+                                                                sload(a.lengths + b));
         const int len = rq.len, keys = rq.keys, nu = rq.nu, t0 = rq.t0, nt = rq.nt;
         if (off >= rq.units) {
             off -= rq.units;
@@ -185,8 +193,8 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
         }
         int item = 0, pos = 0;
         if (off) {
-            item = (int)(off / rq.cost);
-            pos = (int)(off % rq.cost);
+            item = (int)divided(off, rq.cost);
+            pos = (int)(off - (int64_t)item * rq.cost);
         }
         while (off < rq.units && left > 0) {
             const int take = (int)min((int64_t)(rq.cost - pos), left);
@@ -207,107 +215,86 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
                 return (unit >= rq.su ? unit + rq.skip : unit) * KU + wk * KT;
             };
             const int n = WR > 1 || key_at(count - 1) < keys ? count : count - 1;
-            const int last16 = (keys - 1) & ~15;
+            const int last16 = (keys - 1) & ~15, last32 = (keys - 1) & ~31;
             const uint8_t* kb = a.k + (int64_t)h * a.c.sh;
             const uint8_t* vb = a.v + (int64_t)h * a.c.sh;
             const int* table = a.table + b * a.table_stride;
             // The first key that all of the item's rows see, and all from there on to the context's end.
             const int clear = a.window ? (int)min((int64_t)len + (a.masks ? 63 : min(nt - 1, (rt * RT + RT - 1) / a.G)) + 1 - a.window,
                                                   (int64_t)INT32_MAX) : 0;
-            // A tile's pages, read ahead; the places of its groups in a cache and their scales;
-            // its copies.  (Past the last key: its page again.)
-            const auto key_of = [&](int i, int hf) { return min(key_at(i) + 16 * hf, last16); };
+            // A tile's pages, read ahead; where its two groups lie in a cache, and their scales; its
+            // copies.  (Past the last tile: it again.)  In blocks of 32 tokens and more both are in one.
+            const auto key_of = [&](int i) { return min(key_at(i), last32); };
             int page[SUBS];
             const auto read_pages = [&](int i) {
-#pragma unroll
-                for (int hf = 0; hf < SUBS; ++hf) page[hf] = sload(table + (key_of(i, hf) >> a.c.bs_log2));
+                const int key = key_of(i);
+                page[0] = page[1] = sload(table + (key >> a.c.bs_log2));
+                if (a.c.bs_log2 < 5) page[1] = sload(table + (min(key + GROUP, last16) >> a.c.bs_log2));
             };
             uint64_t at_k[SUBS], at_v[SUBS];  // of the tiles whose keys, values are copied next
+            uint64_t at_s[SUBS];              // and of the first one's scales
             uint32_t highest = 0;             // of the pages placed so far (unsigned: -1 is above all blocks)
             const auto place = [&](int i) {
-#pragma unroll
-                for (int hf = 0; hf < SUBS; ++hf) {
-                    at_v[hf] = at_k[hf];
-                    at_k[hf] = place_of(a, page[hf], key_of(i, hf));
-                    highest = max(highest, (uint32_t)page[hf]);
+                const uint32_t in = (uint32_t)key_of(i) & ((1u << a.c.bs_log2) - 1);
+                const uint32_t pg = min((uint32_t)page[0], (uint32_t)a.c.num_blocks - 1);
+                at_v[0] = at_k[0], at_v[1] = at_k[1];
+                at_k[0] = (uint64_t)pg * (uint32_t)a.c.sb + (uint64_t)in * (uint32_t)a.c.st;
+                at_s[0] = (((uint64_t)pg * (uint32_t)a.hkv + (uint32_t)h) << (a.c.bs_log2 - 2)) + in / 4;  // (4 bytes a group)
+                at_k[1] = at_k[0] + (uint64_t)(GROUP * (uint32_t)a.c.st);
+                at_s[1] = at_s[0] + 4;
+                highest = max(highest, (uint32_t)page[0]);
+                if (a.c.bs_log2 < 5) {
+                    const uint32_t other = min((uint32_t)page[1], (uint32_t)a.c.num_blocks - 1);
+                    at_k[1] = (uint64_t)other * (uint32_t)a.c.sb;
+                    at_s[1] = ((uint64_t)other * (uint32_t)a.hkv + (uint32_t)h) * 4;
+                    highest = max(highest, (uint32_t)page[1]);
                 }
-            };
-            const auto scales_at = [&](int i, int hf) {
-                const int key = key_of(i, hf);
-                const uint32_t pg = min((uint32_t)sload(table + (key >> a.c.bs_log2)), (uint32_t)a.c.num_blocks - 1);
-                return ((int64_t)pg * a.hkv + h) * groups + (((uint32_t)key & ((1u << a.c.bs_log2) - 1)) / GROUP);
             };
             // The keys of a tile that lie in a block.
             const auto there = [&](int i) {
-                uint32_t m = ~0u;
+                read_pages(i);
+                return (no_block(a, page[0]) ? 0u : 0xFFFFu) | (no_block(a, page[1]) ? 0u : 0xFFFF0000u);
+            };
+            const auto copy_scales = [&](int stage) {
+                dma4(scales + (lane & 1 ? at_s[1] : at_s[0]), gbase + stage * S::STAGE + S::SCALES);
+            };
+            const auto copy_k = [&](int stage) {
+                copy_scales(stage);
 #pragma unroll
                 for (int hf = 0; hf < SUBS; ++hf)
-                    if (no_block(a, sload(table + (key_of(i, hf) >> a.c.bs_log2)))) m &= ~(0xFFFFu << (16 * hf));
-                return m;
-            };
-            const int64_t step = ROWS * a.c.st;  // bytes from copy to copy
-            const auto copy_k = [&](int stage) {
 #pragma unroll
-                for (int hf = 0; hf < SUBS; ++hf) {
-                    const uint8_t* at = kb + at_k[hf];
-#pragma unroll
-                    for (int j = 0; j < J; ++j, at += step)
-                        dma16s(src, at, gbase + stage * S::STAGE + (hf * J + j) * S::KSTEP);
-                }
+                    for (int j = 0; j < J; ++j)
+                        dma16s(src[j], kb + at_k[hf], gbase + stage * S::STAGE + (hf * J + j) * S::KSTEP);
             };
             const auto copy_v = [&](int stage) {
 #pragma unroll
-                for (int hf = 0; hf < SUBS; ++hf) {
-                    const uint8_t* at = vb + at_v[hf];
+                for (int hf = 0; hf < SUBS; ++hf)
 #pragma unroll
-                    for (int j = 0; j < J; ++j, at += step)
-                        dma16s(src, at, gbase + stage * S::STAGE + S::KTILE + hf * S::VGROUP + j * S::VSTEP);
-                }
+                    for (int j = 0; j < J; ++j)
+                        dma16s(src[j], vb + at_v[hf], gbase + stage * S::STAGE + S::KTILE + hf * S::VGROUP + j * S::VSTEP);
             };
             // This wave's share of a tile's keys and of the one before's values: copies wr, wr + WR, .. of the
             // NI of keys and the NI of values, copy c being number c % J of group c / J.
+            // (Every wave copies the scales, to the same place.)
             const auto copy_share = [&](bool ks, int kstage, bool vs, int vstage) {
+                if (ks) copy_scales(kstage);
 #pragma unroll
-                for (int x = 0; x < S::CW; ++x) {
+                for (int x = 0; x < 2 * NI / WR; ++x) {
                     const int c = WR * x + wr;
                     const bool isv = c >= NI;
                     const int i = isv ? c - NI : c, hf = i / J, j = i % J;
-                    const uint64_t in = j * step;
                     if (isv) {
-                        if (vs) dma16s(src, vb + ((hf ? at_v[1] : at_v[0]) + in),
+                        if (vs) dma16s(mine[x], vb + (hf ? at_v[1] : at_v[0]),
                                        gbase + vstage * S::STAGE + S::KTILE + hf * S::VGROUP + j * S::VSTEP);
                     } else if (ks) {
-                        dma16s(src, kb + ((hf ? at_k[1] : at_k[0]) + in), gbase + kstage * S::STAGE + i * S::KSTEP);
+                        dma16s(mine[x], kb + (hf ? at_k[1] : at_k[0]), gbase + kstage * S::STAGE + i * S::KSTEP);
                     }
                 }
             };
 
-            at_k[0] = at_k[1] = 0;
             read_pages(0);
-            if constexpr (WR == 1) {
-                // K0 V0 K1 V1 ..; then the keys of tile i + NS once tile i's are used, and its values once those are
-#pragma unroll
-                for (int i = 0; i < NS; ++i) {
-                    place(i);
-                    at_v[0] = at_k[0], at_v[1] = at_k[1];
-                    read_pages(i + 1);
-                    if (i < n) {
-                        copy_k(i);
-                        copy_v(i);
-                    }
-                }
-            } else {
-                // K0, K1 V0, K2 V1, ..: each step's batch has the keys of one tile and the values of the one before
-#pragma unroll
-                for (int i = 0; i < NS; ++i) {
-                    place(i);
-                    read_pages(i + 1);
-                    copy_share(i < n, i, i > 0 && i <= n, i - 1);
-                }
-            }
-            // --- queries (on their way while the first tiles are): bytes of the row's largest's 2^-23 ---
-            i4 qf[NR][STEPS][LIMBS];
-            float rs[NR];
+            // --- queries: asked for before the tiles, so that the first scores wait for one tile only ---
+            f4 x[NR][STEPS][4];
             uint64_t mask[NR];
             int from[NR];
 #pragma unroll
@@ -317,27 +304,61 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
                 const bool on = t < nt;
                 // (a chain: how many of the new tokens the row sees)
                 mask[c] = !on ? 0 : a.masks ? a.masks[t0 + t] : (uint64_t)t + 1;
-                from[c] = 0;
-                if (on) {
-                    const Reach reached = reach(a, len, t, mask[c]);
-                    mask[c] = reached.mask, from[c] = reached.from;
-                }
                 const float* q = a.q + (int64_t)(t0 + (on ? t : 0)) * a.ldq + (int64_t)(on ? hh : 0) * D;
-                f4 x[STEPS][4];
-                float mx = 0.0f;
-                bool finite = true;
 #pragma unroll
                 for (int s = 0; s < STEPS; ++s)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const bool in = on && (D % 64 == 0 || 64 * s + 16 * g < D);
-                        x[s][i] = in ? *(const f4u*)(q + 64 * s + 16 * g + 4 * i) : f4{0, 0, 0, 0};
+                        x[c][s][i] = in ? *(const f4u*)(q + 64 * s + 16 * g + 4 * i) : f4{0, 0, 0, 0};
+                    }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            // (Rolled: a launch begins with none of its instructions in the cache.)
+            at_k[0] = at_k[1] = 0;
+            if constexpr (WR == 1) {
+                // K0 V0 K1 V1 ..; then the keys of tile i + NS once tile i's are used, and its values once those are
+#pragma unroll 1
+                for (int i = 0; i < NS; ++i) {
+                    place(i);
+                    read_pages(i + 1);
+                    at_v[0] = at_k[0], at_v[1] = at_k[1];
+                    if (i < n) {
+                        copy_k(i);
+                        copy_v(i);
+                    }
+                }
+            } else {
+                // K0, K1 V0, K2 V1, ..: each step's batch has the keys of one tile and the values of the one before
+#pragma unroll 1
+                for (int i = 0; i < NS; ++i) {
+                    place(i);
+                    read_pages(i + 1);
+                    copy_share(i < n, i, i > 0 && i <= n, i - 1);
+                }
+            }
+            // --- the queries' bytes, of their row's largest's 2^-23 ---
+            i4 qf[NR][STEPS][LIMBS];
+            float rs[NR];
+#pragma unroll
+            for (int c = 0; c < NR; ++c) {
+                const int r = rt * RT + wr * 16 * NR + 16 * c + n16, t = r / a.G;
+                from[c] = 0;
+                if (t < nt) {
+                    const Reach reached = reach(a, len, t, mask[c]);
+                    mask[c] = reached.mask, from[c] = reached.from;
+                }
+                float mx = 0.0f;
+                bool finite = true;
+#pragma unroll
+                for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            finite &= fabsf(x[s][i][e]) < __builtin_inff();
-                            mx = fmaxf(mx, fabsf(x[s][i][e]));
+                            finite &= fabsf(x[c][s][i][e]) < __builtin_inff();
+                            mx = fmaxf(mx, fabsf(x[c][s][i][e]));
                         }
-                    }
                 mx = max4(finite ? mx : __builtin_inff());
                 float up = 0.0f, down = 1.0f;
                 if (mx < __builtin_inff()) {
@@ -357,7 +378,7 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
                         uint32_t v[4];
 #pragma unroll
                         for (int e = 0; e < 4; ++e)  // a byte and 128 in each place
-                            v[e] = (uint32_t)((mx < __builtin_inff() ? (int)rintf(x[s][i][e] * up) : 0) + 0x808080);
+                            v[e] = (uint32_t)((mx < __builtin_inff() ? (int)rintf(x[c][s][i][e] * up) : 0) + 0x808080);
                         const uint32_t lo = __builtin_amdgcn_perm(v[1], v[0], 0x05010400u);  // bytes 0, 1 of two
                         const uint32_t hi = __builtin_amdgcn_perm(v[3], v[2], 0x05010400u);
                         const uint32_t top = __builtin_amdgcn_perm(v[1], v[0], 0x0C0C0602u) |
@@ -415,18 +436,8 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
                                                  (float)((acc[0][sub][c][r] << 8) + acc[1][sub][c][r]));
             };
             f4 sc[SUBS][NR];
-            int kbits[SUBS], vbits[SUBS];  // the scales of the tile whose softmax is next
-            const auto read_scales = [&](int i) {
-#pragma unroll
-                for (int hf = 0; hf < SUBS; ++hf) {
-                    const int64_t at = scales_at(i, hf);
-                    kbits[hf] = sload((const int*)a.ks + at);
-                    vbits[hf] = sload((const int*)a.vs + at);
-                }
-            };
-            read_scales(0);
             if constexpr (WR == 1) {
-                if (n >= NS) wait_vm<(2 * NS - 1) * NI>();
+                if (n >= NS) wait_vm<NI + (NS - 1) * (2 * NI + 1)>();
                 else wait_vm<0>();
             } else {
                 if (n >= NS) wait_vm<(NS - 1) * S::CW>();
@@ -438,6 +449,8 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
             for (int i = 0; i < n; ++i) {
                 const int key0 = key_at(i);
                 const int stage1 = stage + 1 < NS ? stage + 1 : 0;
+                // (landed with its keys; its place is filled anew from the next wait on)
+                const u4 ts = *(lds_u4*)(uintptr_t)(gbase + stage * S::STAGE + S::SCALES);
                 // this tile's values and the next one's keys have landed: this wave's copies of them, then
                 // everyone's; and all are done with this one's keys and the last one's values, whose places are
                 // filled anew
@@ -447,10 +460,10 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
                         place(i + NS);
                         read_pages(i + NS + 1);
                         copy_k(stage);
-                        wait_vm<2 * (NS - 1) * NI>();
+                        wait_vm<(NS - 1) * (2 * NI + 1)>();
                     } else if (NS > 2 && i + 2 < n) {
-                        if (NS > 3 && i + 3 < n) wait_vm<5 * NI>();
-                        else wait_vm<3 * NI>();
+                        if (NS > 3 && i + 3 < n) wait_vm<5 * NI + 2>();
+                        else wait_vm<3 * NI + 1>();
                     } else if (i + 1 < n) {
                         wait_vm<NI>();
                     } else {
@@ -471,14 +484,13 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
                 float mul[SUBS][NR], sv[SUBS], lift[SUBS];
 #pragma unroll
                 for (int sub = 0; sub < SUBS; ++sub) {
-                    const float sk = scale_of(kbits[sub]);
-                    sv[sub] = scale_of(vbits[sub]);
+                    const float sk = held_scale(__uint_as_float(ts[sub]));
+                    sv[sub] = held_scale(__uint_as_float(ts[SUBS + sub]));
                     // (any number near log2 sv; a group of zeros still has its part in the sums)
                     lift[sub] = fmaxf(__builtin_amdgcn_logf(sv[sub]), -80.0f);
 #pragma unroll
                     for (int c = 0; c < NR; ++c) mul[sub][c] = rs[c] * sk;
                 }
-                if (i + 1 < n) read_scales(i + 1);
                 if (tail) {
                     const int old = len - key0, all = keys - key0;
                     const uint32_t in = holes ? there(i) : ~0u;
@@ -589,7 +601,8 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
                 stage = stage1;
             }
 
-            // --- join the groups: each takes D / WK of the columns ---
+            // --- join the groups: each takes DW of the columns' 16s ---
+            constexpr int DW = (DT + WK - 1) / WK;
             int ln = lane;  // (opaque: addresses made from it are not kept through the tiles)
             asm volatile("" : "+v"(ln));
 #pragma unroll
@@ -631,8 +644,9 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
                 const float inv = lsum[c] != 0.0f ? 1.0f / lsum[c] : 0.0f;
                 float* to = whole ? a.out + ((int64_t)(t0 + t) * a.hq + hh) * D : part + rl * D;
 #pragma unroll
-                for (int d0 = 0; d0 < DT / WK; ++d0) {
-                    const int d = wk * (DT / WK) + d0;
+                for (int d0 = 0; d0 < DW; ++d0) {
+                    const int d = wk * DW + d0;
+                    if (DT % WK && d >= DT) break;
                     f4 v;
                     if (WK > 1) {
                         v = f4{0, 0, 0, 0};
@@ -665,13 +679,28 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
     if (!cut && tid == 0) a.desc[wg] = 0;
 }
 
+// Whether items are left whole, so that nothing is to be joined: where they have few units at most, by
+// the table's columns and the window, or take no longer one after the other on the work-groups than
+// cut into even shares, with the begin of a second part and the second launch (about JOIN units).
 template <class S>
-hipError_t go(AttnArgs a, int cus, uint8_t* ws, hipStream_t st) {
+bool uncut(const AttnArgs& a, int max_new) {
+    constexpr int JOIN = 2 + 256 / S::KU;
+    int64_t keys = (int64_t)a.max_blocks << a.c.bs_log2;
+    if (keys <= 6 * std::max(S::KU, 64)) return true;
+    if (!a.window) return false;
+    // (a request may have more new tokens than it was said: its items are whole as well, only longer)
+    keys = std::min<int64_t>(keys, (int64_t)a.window + max_new + (a.sinks ? S::KU + std::min<int64_t>(a.sinks, keys) : 0));
+    const int64_t units = keys / S::KU + 2, items = (int64_t)a.B * a.hkv * (((int64_t)max_new * a.G + S::RT - 1) / S::RT);
+    const int64_t turns = (items + a.grid - 1) / a.grid;
+    return turns * (units + S::OV) <= items * (units + 2 * S::OV) / a.grid + JOIN;
+}
+
+template <class S>
+hipError_t go(AttnArgs a, int max_new, int cus, uint8_t* ws, hipStream_t st) {
     a.grid = std::min(S::PC * cus, MAX_ITEMS);
     a.desc = (int*)ws;
     a.part = (float*)(ws + DESC_BYTES);
-    // (as for 16 bits: short tables are not cut)
-    a.whole = (int64_t)a.max_blocks << a.c.bs_log2 <= 6 * std::max(S::KU, 64);
+    a.whole = uncut<S>(a, max_new);
     hipLaunchKernelGGL(attn8_kernel<S>, dim3(a.grid), dim3(64 * S::WAVES), S::LDS, st, a);
     if (!a.whole) hipLaunchKernelGGL((attn_join<S::D, S::RT>), dim3(JOIN_WGS * cus), dim3(256), 0, st, a);
     return hipGetLastError();
@@ -681,12 +710,12 @@ template <int D>
 hipError_t rows(const AttnArgs& a, int max_new, int cus, uint8_t* ws, hipStream_t st) {
     const int64_t r = (int64_t)max_new * a.G;
     if constexpr (D == 256) {
-        if (r <= 16) return go<Shape<D, 1, 1, 2, 2, 2>>(a, cus, ws, st);
-        return go<Shape<D, 1, 4, 1, 3, 1>>(a, cus, ws, st);
+        if (r <= 16) return go<Shape<D, 1, 1, 2, 2, 2>>(a, max_new, cus, ws, st);
+        return go<Shape<D, 1, 4, 1, 3, 1>>(a, max_new, cus, ws, st);
     } else {
-        if (r <= 16) return go<Shape<D, 1, 1, 2, 4, 2>>(a, cus, ws, st);
-        if (r <= 32) return go<Shape<D, 2, 1, 2, 4, 2>>(a, cus, ws, st);
-        return go<Shape<D, 1, 4, 1, 4, 3>>(a, cus, ws, st);
+        if (r <= 16) return go<Shape<D, 1, 1, 4, 2, 2>>(a, max_new, cus, ws, st);
+        if (r <= 32) return go<Shape<D, 2, 1, 2, 3, 2>>(a, max_new, cus, ws, st);
+        return go<Shape<D, 2, 2, 2, 3, 2>>(a, max_new, cus, ws, st);
     }
 }
 

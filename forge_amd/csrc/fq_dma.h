@@ -32,6 +32,15 @@ __device__ __forceinline__ void dma16s(uint32_t off, const uint8_t* base, uint32
                  : "memory");
 }
 
+// The same of 4 bytes per lane, from an address of each lane's own, to lds + 4 lane.
+__device__ __forceinline__ void dma4(const void* at, uint32_t lds) {
+    uint32_t m0;
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %1, off"
+                 : "=&{m0}"(m0)
+                 : "v"(at), "s"(lds)
+                 : "memory");
+}
+
 // Wait until at most N vector-memory loads of this wave are outstanding.
 template <int N>
 __device__ __forceinline__ void wait_vm() {
