@@ -38,15 +38,19 @@ __device__ __forceinline__ int64_t divided(int64_t a, int64_t b) {
     return (uint64_t)(a | b) >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
 }
 
-// x0, x1 as two pairs of fp16 that add up to them.  minus1: -1 where the compiler does not see it, so that
-// the rest is one fused multiply-add from the packed part.
-__device__ __forceinline__ void split2(float x0, float x1, float minus1, uint32_t& hi, uint32_t& lo) {
-    const h2 first = __builtin_convertvector((f2{x0, x1}), h2);
-    hi = __builtin_bit_cast(uint32_t, first);
-    asm("" : "+v"(hi));
-    const h2 back = __builtin_bit_cast(h2, hi);
-    const h2 rest = {(_Float16)fmaf((float)back[0], minus1, x0), (_Float16)fmaf((float)back[1], minus1, x1)};
-    lo = __builtin_bit_cast(uint32_t, rest);
+// The largest of three.  (Written out: the compiler makes numbers that may be signalling NaN quiet first.)
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+
+// x0, x1 as two pairs of fp16 that add up to them.  (The rest is one fused multiply-add from the packed part
+// with its own rounding.)
+__device__ __forceinline__ void split2(float x0, float x1, uint32_t& hi, uint32_t& lo) {
+    hi = __builtin_bit_cast(uint32_t, __builtin_convertvector((f2{x0, x1}), h2));
+    asm("v_fma_mixlo_f16 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(lo) : "v"(hi), "v"(x0));
+    asm("v_fma_mixhi_f16 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "+v"(lo) : "v"(hi), "v"(x1));
 }
 
 // Four codes as fp16: a byte with its sign turned beside 0x64 is 1024 + 128 + code.
@@ -105,7 +109,9 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
     __shared__ float s_ml[2][WK][RT];
     const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6);
-    const int wr = wave % WR, wk = wave / WR;
+    // (the waves of a second work-group on a CU take their rows in another order: where an item has
+    // fewer than RT, those without would be on the same SIMDs)
+    const int wr = (wave + (int)(blockIdx.x * S::PC / gridDim.x) * (WR / 2)) % WR, wk = wave / WR;
     const int n16 = lane & 15, g = lane >> 4;
     const int wg = blockIdx.x;
 
@@ -153,8 +159,6 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
     bool cut = false;  // an item begun here goes on in the next work-group
 
     // --- constants of a lane ---
-    float minus1 = -1.0f;
-    asm("" : "+s"(minus1));
     const uint32_t gbase = lds_addr(lds) + wk * S::GROUPS;
     // a copy's source: bytes from the first row of its 16; and of this wave's share of the copies
     uint32_t src[J], mine[2 * NI / WR];
@@ -231,32 +235,33 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
                 page[0] = page[1] = sload(table + (key >> a.c.bs_log2));
                 if (a.c.bs_log2 < 5) page[1] = sload(table + (min(key + GROUP, last16) >> a.c.bs_log2));
             };
-            uint64_t at_k[SUBS], at_v[SUBS];  // of the tiles whose keys, values are copied next
-            uint64_t at_s[SUBS];              // and of the first one's scales
+            uint64_t at_k0 = 0, at_k1 = 0, at_v0 = 0, at_v1 = 0;  // of the tiles whose keys, values are copied next
+            uint64_t at_s0 = 0, at_s1 = 0;                        // and of the first one's scales
             uint32_t highest = 0;             // of the pages placed so far (unsigned: -1 is above all blocks)
             const auto place = [&](int i) {
                 const uint32_t in = (uint32_t)key_of(i) & ((1u << a.c.bs_log2) - 1);
                 const uint32_t pg = min((uint32_t)page[0], (uint32_t)a.c.num_blocks - 1);
-                at_v[0] = at_k[0], at_v[1] = at_k[1];
-                at_k[0] = (uint64_t)pg * (uint32_t)a.c.sb + (uint64_t)in * (uint32_t)a.c.st;
-                at_s[0] = (((uint64_t)pg * (uint32_t)a.hkv + (uint32_t)h) << (a.c.bs_log2 - 2)) + in / 4;  // (4 bytes a group)
-                at_k[1] = at_k[0] + (uint64_t)(GROUP * (uint32_t)a.c.st);
-                at_s[1] = at_s[0] + 4;
+                at_v0 = at_k0, at_v1 = at_k1;
+                at_k0 = (uint64_t)pg * (uint32_t)a.c.sb + (uint64_t)in * (uint32_t)a.c.st;
+                at_s0 = (((uint64_t)pg * (uint32_t)a.hkv + (uint32_t)h) << (a.c.bs_log2 - 2)) + in / 4;  // (4 bytes a group)
+                at_k1 = at_k0 + (uint64_t)(GROUP * (uint32_t)a.c.st);
+                at_s1 = at_s0 + 4;
                 highest = max(highest, (uint32_t)page[0]);
                 if (a.c.bs_log2 < 5) {
                     const uint32_t other = min((uint32_t)page[1], (uint32_t)a.c.num_blocks - 1);
-                    at_k[1] = (uint64_t)other * (uint32_t)a.c.sb;
-                    at_s[1] = ((uint64_t)other * (uint32_t)a.hkv + (uint32_t)h) * 4;
+                    at_k1 = (uint64_t)other * (uint32_t)a.c.sb;
+                    at_s1 = ((uint64_t)other * (uint32_t)a.hkv + (uint32_t)h) * 4;
                     highest = max(highest, (uint32_t)page[1]);
                 }
             };
             // The keys of a tile that lie in a block.
             const auto there = [&](int i) {
-                read_pages(i);
-                return (no_block(a, page[0]) ? 0u : 0xFFFFu) | (no_block(a, page[1]) ? 0u : 0xFFFF0000u);
+                const int key = key_of(i), more = min(key + GROUP, last16);
+                return (no_block(a, sload(table + (key >> a.c.bs_log2))) ? 0u : 0xFFFFu) |
+                       (no_block(a, sload(table + (more >> a.c.bs_log2))) ? 0u : 0xFFFF0000u);
             };
             const auto copy_scales = [&](int stage) {
-                dma4(scales + (lane & 1 ? at_s[1] : at_s[0]), gbase + stage * S::STAGE + S::SCALES);
+                dma4(scales + (lane & 1 ? at_s1 : at_s0), gbase + stage * S::STAGE + S::SCALES);
             };
             const auto copy_k = [&](int stage) {
                 copy_scales(stage);
@@ -264,14 +269,14 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
                 for (int hf = 0; hf < SUBS; ++hf)
 #pragma unroll
                     for (int j = 0; j < J; ++j)
-                        dma16s(src[j], kb + at_k[hf], gbase + stage * S::STAGE + (hf * J + j) * S::KSTEP);
+                        dma16s(src[j], kb + (hf ? at_k1 : at_k0), gbase + stage * S::STAGE + (hf * J + j) * S::KSTEP);
             };
             const auto copy_v = [&](int stage) {
 #pragma unroll
                 for (int hf = 0; hf < SUBS; ++hf)
 #pragma unroll
                     for (int j = 0; j < J; ++j)
-                        dma16s(src[j], vb + at_v[hf], gbase + stage * S::STAGE + S::KTILE + hf * S::VGROUP + j * S::VSTEP);
+                        dma16s(src[j], vb + (hf ? at_v1 : at_v0), gbase + stage * S::STAGE + S::KTILE + hf * S::VGROUP + j * S::VSTEP);
             };
             // This wave's share of a tile's keys and of the one before's values: copies wr, wr + WR, .. of the
             // NI of keys and the NI of values, copy c being number c % J of group c / J.
@@ -284,45 +289,23 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
                     const bool isv = c >= NI;
                     const int i = isv ? c - NI : c, hf = i / J, j = i % J;
                     if (isv) {
-                        if (vs) dma16s(mine[x], vb + (hf ? at_v[1] : at_v[0]),
+                        if (vs) dma16s(mine[x], vb + (hf ? at_v1 : at_v0),
                                        gbase + vstage * S::STAGE + S::KTILE + hf * S::VGROUP + j * S::VSTEP);
                     } else if (ks) {
-                        dma16s(mine[x], kb + (hf ? at_k[1] : at_k[0]), gbase + kstage * S::STAGE + i * S::KSTEP);
+                        dma16s(mine[x], kb + (hf ? at_k1 : at_k0), gbase + kstage * S::STAGE + i * S::KSTEP);
                     }
                 }
             };
 
             read_pages(0);
-            // --- queries: asked for before the tiles, so that the first scores wait for one tile only ---
-            f4 x[NR][STEPS][4];
-            uint64_t mask[NR];
-            int from[NR];
-#pragma unroll
-            for (int c = 0; c < NR; ++c) {
-                const int r = rt * RT + wr * 16 * NR + 16 * c + n16;
-                const int t = r / a.G, hh = h * a.G + r % a.G;
-                const bool on = t < nt;
-                // (a chain: how many of the new tokens the row sees)
-                mask[c] = !on ? 0 : a.masks ? a.masks[t0 + t] : (uint64_t)t + 1;
-                const float* q = a.q + (int64_t)(t0 + (on ? t : 0)) * a.ldq + (int64_t)(on ? hh : 0) * D;
-#pragma unroll
-                for (int s = 0; s < STEPS; ++s)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const bool in = on && (D % 64 == 0 || 64 * s + 16 * g < D);
-                        x[c][s][i] = in ? *(const f4u*)(q + 64 * s + 16 * g + 4 * i) : f4{0, 0, 0, 0};
-                    }
-            }
-            __builtin_amdgcn_sched_barrier(0);
             // (Rolled: a launch begins with none of its instructions in the cache.)
-            at_k[0] = at_k[1] = 0;
             if constexpr (WR == 1) {
                 // K0 V0 K1 V1 ..; then the keys of tile i + NS once tile i's are used, and its values once those are
 #pragma unroll 1
                 for (int i = 0; i < NS; ++i) {
                     place(i);
                     read_pages(i + 1);
-                    at_v[0] = at_k[0], at_v[1] = at_k[1];
+                    at_v0 = at_k0, at_v1 = at_k1;
                     if (i < n) {
                         copy_k(i);
                         copy_v(i);
@@ -337,28 +320,39 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
                     copy_share(i < n, i, i > 0 && i <= n, i - 1);
                 }
             }
-            // --- the queries' bytes, of their row's largest's 2^-23 ---
+            // --- queries (on their way while the first tiles are): bytes of their row's largest's 2^-23 ---
             i4 qf[NR][STEPS][LIMBS];
             float rs[NR];
+            uint64_t mask[NR];
+            int from[NR];
 #pragma unroll
             for (int c = 0; c < NR; ++c) {
-                const int r = rt * RT + wr * 16 * NR + 16 * c + n16, t = r / a.G;
+                const int r = rt * RT + wr * 16 * NR + 16 * c + n16;
+                const int t = r / a.G, hh = h * a.G + r % a.G;
+                const bool on = t < nt;
+                // (a chain: how many of the new tokens the row sees)
+                mask[c] = !on ? 0 : a.masks ? a.masks[t0 + t] : (uint64_t)t + 1;
                 from[c] = 0;
-                if (t < nt) {
+                if (on) {
                     const Reach reached = reach(a, len, t, mask[c]);
                     mask[c] = reached.mask, from[c] = reached.from;
                 }
+                const float* q = a.q + (int64_t)(t0 + (on ? t : 0)) * a.ldq + (int64_t)(on ? hh : 0) * D;
+                f4 x[STEPS][4];
                 float mx = 0.0f;
                 bool finite = true;
 #pragma unroll
                 for (int s = 0; s < STEPS; ++s)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
+                    for (int i = 0; i < 4; ++i) {
+                        const bool in = on && (D % 64 == 0 || 64 * s + 16 * g < D);
+                        x[s][i] = in ? *(const f4u*)(q + 64 * s + 16 * g + 4 * i) : f4{0, 0, 0, 0};
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            finite &= fabsf(x[c][s][i][e]) < __builtin_inff();
-                            mx = fmaxf(mx, fabsf(x[c][s][i][e]));
+                            finite &= fabsf(x[s][i][e]) < __builtin_inff();
+                            mx = fmaxf(mx, fabsf(x[s][i][e]));
                         }
+                    }
                 mx = max4(finite ? mx : __builtin_inff());
                 float up = 0.0f, down = 1.0f;
                 if (mx < __builtin_inff()) {
@@ -378,7 +372,7 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
                         uint32_t v[4];
 #pragma unroll
                         for (int e = 0; e < 4; ++e)  // a byte and 128 in each place
-                            v[e] = (uint32_t)((mx < __builtin_inff() ? (int)rintf(x[c][s][i][e] * up) : 0) + 0x808080);
+                            v[e] = (uint32_t)((mx < __builtin_inff() ? (int)rintf(x[s][i][e] * up) : 0) + 0x808080);
                         const uint32_t lo = __builtin_amdgcn_perm(v[1], v[0], 0x05010400u);  // bytes 0, 1 of two
                         const uint32_t hi = __builtin_amdgcn_perm(v[3], v[2], 0x05010400u);
                         const uint32_t top = __builtin_amdgcn_perm(v[1], v[0], 0x0C0C0602u) |
@@ -389,6 +383,8 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
                     }
             }
 
+            // (a wave whose rows are none of the item's copies its share and waits with the others)
+            const bool busy = WR == 1 || rt * RT + wr * 16 * NR < nt * a.G;
             f4 o[DT][NR];
             float mrow[NR], lrow[NR];
 #pragma unroll
@@ -398,42 +394,47 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
 #pragma unroll
                 for (int d = 0; d < DT; ++d) o[d][c] = f4{0, 0, 0, 0};
             }
-            // Products of the keys at `at`, STEPS times LIMBS SUBS NR matrix instructions with beside(piece)
-            // after each of STEPS LIMBS runs of them; scores are their bytes' sums over 256.
-            const auto products = [&](uint32_t at, f4 (&sc)[SUBS][NR], const auto& beside) {
-                i4 acc[LIMBS][SUBS][NR];
-                i4 kf[2][SUBS];
-                const auto keys_of = [&](int s, i4 (&k)[SUBS]) {
+            // Products of the keys at `at`, LIMBS STEPS runs of SUBS NR matrix instructions with beside(run)
+            // after each.  Scores in units of 256: the lowest bytes' sums are shifted down (the
+            // fraction, below 2^-15 of a largest element times one code, is the same to within
+            // that for all keys) and the middle ones' added to them by the instructions themselves.  (All of
+            // it stays below 2^31: 127 128 256 (256 + 2).)
+            const auto products = [&](uint32_t at, i4 (&low)[SUBS][NR], i4 (&high)[SUBS][NR], const auto& begun,
+                                      const auto& beside) {
+                i4 kf[STEPS][SUBS];
+#pragma unroll
+                for (int s = 0; s < STEPS; ++s)
 #pragma unroll
                     for (int sub = 0; sub < SUBS; ++sub)
-                        k[sub] = __builtin_bit_cast(i4, *(lds_u4*)(uintptr_t)(klane + at + J * sub * S::KSTEP + 64 * s));
+                        kf[s][sub] = __builtin_bit_cast(i4, *(lds_u4*)(uintptr_t)(klane + at + J * sub * S::KSTEP + 64 * s));
+                begun();
+                const auto run = [&](int l, int s, i4 (&acc)[SUBS][NR], bool begin) {
+#pragma unroll
+                    for (int sub = 0; sub < SUBS; ++sub)
+#pragma unroll
+                        for (int c = 0; c < NR; ++c)
+                            acc[sub][c] = __builtin_amdgcn_mfma_i32_16x16x64_i8(
+                                kf[s][sub], qf[c][s][l], begin ? i4{0, 0, 0, 0} : acc[sub][c], 0, 0, 0);
                 };
-                keys_of(0, kf[0]);
 #pragma unroll
-                for (int s = 0; s < STEPS; ++s) {
-                    if (s + 1 < STEPS) keys_of(s + 1, kf[(s + 1) & 1]);
-#pragma unroll
-                    for (int l = 0; l < LIMBS; ++l) {
+                for (int x = 0; x < LIMBS * STEPS; ++x) {
+                    const int s = x % STEPS;
+                    if (x < STEPS) run(2, s, low, s == 0);
+                    else if (x < 2 * STEPS) run(0, s, high, s == 0);
+                    else run(1, s, low, false);
+                    __builtin_amdgcn_sched_barrier(0);
+                    beside(x);
+                    if (x == 2 * STEPS - 1)
 #pragma unroll
                         for (int sub = 0; sub < SUBS; ++sub)
 #pragma unroll
-                            for (int c = 0; c < NR; ++c)
-                                acc[l][sub][c] = __builtin_amdgcn_mfma_i32_16x16x64_i8(
-                                    kf[s & 1][sub], qf[c][s][l], s ? acc[l][sub][c] : i4{0, 0, 0, 0}, 0, 0, 0);
-                        __builtin_amdgcn_sched_barrier(0);
-                        beside(s * LIMBS + l);
-                        __builtin_amdgcn_sched_barrier(0);
-                    }
+                            for (int c = 0; c < NR; ++c) low[sub][c] >>= 8;
+                    __builtin_amdgcn_sched_barrier(0);
                 }
-                // (the upper two together stay below 2^31: 127 128 256 (256 + 1))
+            };
+            const auto score = [&](const i4 (&low)[SUBS][NR], const i4 (&high)[SUBS][NR], f4 (&sc)[SUBS][NR], int sub, int c) {
 #pragma unroll
-                for (int sub = 0; sub < SUBS; ++sub)
-#pragma unroll
-                    for (int c = 0; c < NR; ++c)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            sc[sub][c][r] = fmaf((float)acc[2][sub][c][r], 1.0f / 256.0f,
-                                                 (float)((acc[0][sub][c][r] << 8) + acc[1][sub][c][r]));
+                for (int r = 0; r < 4; ++r) sc[sub][c][r] = (float)((high[sub][c][r] << 8) + low[sub][c][r]);
             };
             f4 sc[SUBS][NR];
             if constexpr (WR == 1) {
@@ -444,7 +445,12 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
                 else wait_vm<0>();
                 lds_barrier();
             }
-            products(0, sc, [](int) {});
+            if (busy) {
+                i4 low[SUBS][NR], high[SUBS][NR];
+                products(0, low, high, [] {}, [](int) {});
+#pragma unroll
+                for (int x = 0; x < SUBS * NR; ++x) score(low, high, sc, x / NR, x % NR);
+            }
             int stage = 0;
             for (int i = 0; i < n; ++i) {
                 const int key0 = key_at(i);
@@ -479,6 +485,10 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
                         copy_share(i + NS < n, stage, true, stage ? stage - 1 : NS - 1);
                     }
                 }
+                if (!busy) {
+                    stage = stage1;
+                    continue;
+                }
                 const bool holes = no_block(a, (int)highest);
                 const bool tail = holes || key0 + KT > len || (key0 < clear && key0 + KT > a.sinks);
                 float mul[SUBS][NR], sv[SUBS], lift[SUBS];
@@ -509,18 +519,19 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
                 }
 
                 // the next tile's products (of whatever is there, after the last) beside this one's softmax
-                f4 next[SUBS][NR];
+                i4 low[SUBS][NR], high[SUBS][NR];
+                i2 raw[DT];  // this tile's values, asked for behind the keys: nothing waits for them
                 u4 ph[NR], pl[NR];  // the probabilities' parts
                 float alpha[NR], sum[NR];
                 bool moved = false;
                 const auto maximum = [&](int c) {
-                    float mx = LOWEST;
+                    float most[SUBS];
 #pragma unroll
                     for (int sub = 0; sub < SUBS; ++sub) {
                         const f4 v = sc[sub][c];
-                        mx = fmaxf(mx, fmaf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), mul[sub][c], lift[sub]));
+                        most[sub] = fmaf(max3(v[0], v[1], max3(v[2], v[3], v[3])), mul[sub][c], lift[sub]);
                     }
-                    mx = max4(mx);
+                    const float mx = max4(max3(most[0], most[1], LOWEST));
                     // the sums' reference follows the maximum in steps: exponentials of up to 2^LAG are as
                     // good as those up to 1
                     const float m = mx > mrow[c] + LAG ? mx : mrow[c];
@@ -540,14 +551,19 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
                         uint32_t hi, lo;
-                        split2(p[2 * e], p[2 * e + 1], minus1, hi, lo);
+                        split2(p[2 * e], p[2 * e + 1], hi, lo);
                         ph[c][2 * sub + e] = hi;
                         pl[c][2 * sub + e] = lo;
                     }
                     if (sub == SUBS - 1) lrow[c] = lrow[c] * alpha[c] + sum[c];
                 };
                 __builtin_amdgcn_s_setprio(1);
-                products(stage1 * S::STAGE, next, [&](int s) {
+                products(stage1 * S::STAGE, low, high, [&] {
+#pragma unroll
+                    for (int d = 0; d < DT; ++d)
+                        raw[d] = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+                            (lds_i2*)(uintptr_t)(vlane[d & 3] + stage * S::STAGE + (d >> 2) * 64));
+                }, [&](int s) {
                     // the rows' maxima, then their groups' exponentials, spread over the runs
                     constexpr int PIECES = (1 + SUBS) * NR, RUNS = STEPS * LIMBS;
 #pragma unroll
@@ -564,8 +580,7 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
                         for (int d = 0; d < DT; ++d) o[d][c] *= alpha[c];
 
                 const auto value = [&](int d) {
-                    const uint32_t at = vlane[d & 3] + stage * S::STAGE + (d >> 2) * 64;
-                    const i2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i2*)(uintptr_t)at);
+                    const i2 w = raw[d];
                     const uint32_t w0 = (uint32_t)w[0], w1 = (uint32_t)w[1];
                     u4 r;
                     uint32_t x, y;
@@ -575,9 +590,12 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
                     r[2] = x, r[3] = y;
                     return __builtin_bit_cast(h8, r);
                 };
+                // Two of the columns' 16s at a time: their matrix instructions, and between these, while the
+                // unit has them, the next two's conversion and some of the next scores.
+                h8 vf[2] = {value(0), value(1)};
 #pragma unroll
                 for (int d = 0; d < DT; d += 2) {
-                    const h8 vf[2] = {value(d), value(d + 1)};
+                    h8 after[2];
 #pragma unroll
                     for (int l = 1; l >= 0; --l)
 #pragma unroll
@@ -586,18 +604,26 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
                             for (int c = 0; c < NR; ++c)
                                 o[d + x][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
                                     vf[x], __builtin_bit_cast(h8, l ? pl[c] : ph[c]), o[d + x][c], 0, 0, 0);
+                    if (d + 2 < DT) after[0] = value(d + 2), after[1] = value(d + 3);
+                    constexpr int PIECES = SUBS * NR, RUNS = DT / 2;
+#pragma unroll
+                    for (int x = d / 2 * PIECES / RUNS; x < (d / 2 + 1) * PIECES / RUNS; ++x)
+                        score(low, high, sc, x / NR, x % NR);
+#pragma unroll
+                    for (int x = 0; x < 4 * NR; ++x) {
+                        __builtin_amdgcn_sched_group_barrier(8, 1, 0);
+                        __builtin_amdgcn_sched_group_barrier(2, NR == 1 ? 7 : 4, 0);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (d + 2 < DT) vf[0] = after[0], vf[1] = after[1];
                 }
                 if constexpr (WR == 1) {
                     wait_lds();
                     if (i + NS < n) {
-                        at_v[0] = at_k[0], at_v[1] = at_k[1];
+                        at_v0 = at_k0, at_v1 = at_k1;
                         copy_v(stage);
                     }
                 }
-#pragma unroll
-                for (int sub = 0; sub < SUBS; ++sub)
-#pragma unroll
-                    for (int c = 0; c < NR; ++c) sc[sub][c] = next[sub][c];
                 stage = stage1;
             }
 
@@ -631,7 +657,7 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
 #pragma unroll
                 for (int d = 0; d < DT; ++d) {
                     o[d][c] *= f;
-                    if (WK > 1) *(f4*)(buf + (((wave * NR + c) * DT + d) * 64 + ln) * 4) = o[d][c];
+                    if (WK > 1) *(f4*)(buf + ((((wk * WR + wr) * NR + c) * DT + d) * 64 + ln) * 4) = o[d][c];
                 }
             }
             lds_barrier();
