@@ -19,13 +19,14 @@ namespace {
 constexpr int W = 16;  // tokens of a work-group
 
 template <int GS, bool INTER>
-__global__ __launch_bounds__(256) void rope8_kernel(RopeArgs a, Cache8 c, int q_blocks) {
+__global__ __launch_bounds__(256) void rope8_kernel(RopeArgs a, Cache8 c, int kv_blocks) {
     constexpr int TOK = 256 / GS;  // tokens that the lanes take at a time
     constexpr int R = (2 * W + TOK - 1) / TOK;
     const int p = threadIdx.x % GS, sub = threadIdx.x / GS;
     const bool lane_on = 8 * p < a.D;
-    if ((int)blockIdx.x < q_blocks) {  // query heads
-        const int64_t item = (int64_t)blockIdx.x * TOK + sub;
+    // (keys and values, which take longer, first)
+    if ((int)blockIdx.x >= kv_blocks) {  // query heads
+        const int64_t item = (int64_t)((int)blockIdx.x - kv_blocks) * TOK + sub;
         if (item >= (int64_t)a.N * a.hq) return;
         const int n = (int)(item / a.hq), h = (int)(item % a.hq);
         const auto [x0, x1, d0, d1] = head_runs<GS, INTER>(a, n, h, p, lane_on);
@@ -35,12 +36,17 @@ __global__ __launch_bounds__(256) void rope8_kernel(RopeArgs a, Cache8 c, int q_
         *(f4u*)(q + d1) = x1;
         return;
     }
-    const int64_t item = (int)blockIdx.x - q_blocks;
-    const int hh = (int)(item % (2 * c.hkv)), n0 = (int)(item / (2 * c.hkv)) * W;
+    const int hh = blockIdx.x % (2 * c.hkv), n0 = blockIdx.x / (2 * c.hkv) * W;
     const int h = hh % c.hkv;
     const bool isv = hh >= c.hkv;
     __shared__ int s_slot[2 * W + 1];
     __shared__ float s_max[2 * W];
+    // (the first tokens' rows are on their way before it shows which of them are this work-group's)
+    HeadRuns x[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+        if ((r + 1) * TOK <= W)
+            x[r] = head_runs<GS, INTER>(a, n0 + r * TOK + sub, a.hq + hh, p, lane_on && n0 + r * TOK + sub < a.N);
     // slots of tokens n0 - 1 .. n0 + 31
     if (threadIdx.x < 2 * W + 1) {
         const int n = n0 - 1 + (int)threadIdx.x;
@@ -56,7 +62,6 @@ __global__ __launch_bounds__(256) void rope8_kernel(RopeArgs a, Cache8 c, int q_
         const bool on = slot >= 0 && slot % GROUP && s_slot[j] == slot - 1;
         goes_on = (uint32_t)__ballot(on);
     }
-    HeadRuns x[R];
     int slot[R], lead[R];  // lead: where the token's run begins; -1: not this work-group's
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -68,7 +73,7 @@ __global__ __launch_bounds__(256) void rope8_kernel(RopeArgs a, Cache8 c, int q_
             lead[r] = begins ? 31 - __builtin_clz(begins) : -1;
             if (lead[r] >= W) lead[r] = -1;
         }
-        x[r] = head_runs<GS, INTER>(a, n0 + j, a.hq + hh, p, lane_on && lead[r] >= 0);
+        if ((r + 1) * TOK > W) x[r] = head_runs<GS, INTER>(a, n0 + j, a.hq + hh, p, lane_on && lead[r] >= 0);
         float m = 0.0f;
         if (lane_on && lead[r] >= 0)
 #pragma unroll
@@ -115,8 +120,8 @@ hipError_t go(const RopeArgs& a, const Cache8& c, bool inter, hipStream_t st) {
     const int64_t q_blocks = ((int64_t)a.N * a.hq + TOK - 1) / TOK;
     const int64_t kv_blocks = (int64_t)((a.N + W - 1) / W) * 2 * c.hkv;
     const dim3 g((unsigned)(q_blocks + kv_blocks)), t(256);
-    if (inter) hipLaunchKernelGGL((rope8_kernel<GS, true>), g, t, 0, st, a, c, (int)q_blocks);
-    else hipLaunchKernelGGL((rope8_kernel<GS, false>), g, t, 0, st, a, c, (int)q_blocks);
+    if (inter) hipLaunchKernelGGL((rope8_kernel<GS, true>), g, t, 0, st, a, c, (int)kv_blocks);
+    else hipLaunchKernelGGL((rope8_kernel<GS, false>), g, t, 0, st, a, c, (int)kv_blocks);
     return hipGetLastError();
 }
 

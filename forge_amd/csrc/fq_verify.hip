@@ -16,6 +16,7 @@
 
 #include <algorithm>
 
+#include "fq_search.h"
 #include "fq_step.h"
 
 namespace fq {
@@ -98,14 +99,27 @@ __device__ __forceinline__ void load16(const void* x, int64_t at, int64_t end, f
     }
 }
 
-// The request that row n belongs to; cu rises.  (A row before cu[0] or past cu[B]: any.)
-__device__ __forceinline__ int request_of(const int* cu, int B, int n) {
-    int lo = 0, hi = B;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        (cu[mid] <= n ? lo : hi) = mid;
-    }
-    return lo;
+// e^y for y <= 0 in 64 bits: y = n ln 2 + r, |r| <= ln 2 / 2, and e^r by its series up to r^12 / 12!, 2e-16
+// of it off (the remainder r^13 / 13! is below 1.7e-16).  Below e^-1000 nothing.
+__device__ __forceinline__ double exp_of(double y) {
+    y = fmax(y, -1000.0);
+    const double n = rint(y * 1.4426950408889634074);
+    double r = fma(n, -744261117.0 / 1073741824.0, y);  // (ln 2's first 30 bits, whose products are exact; the rest)
+    r = fma(n, -8.893134238886677e-10, r);
+    double p = 1.0 / 479001600.0;
+    p = fma(p, r, 1.0 / 39916800.0);
+    p = fma(p, r, 1.0 / 3628800.0);
+    p = fma(p, r, 1.0 / 362880.0);
+    p = fma(p, r, 1.0 / 40320.0);
+    p = fma(p, r, 1.0 / 5040.0);
+    p = fma(p, r, 1.0 / 720.0);
+    p = fma(p, r, 1.0 / 120.0);
+    p = fma(p, r, 1.0 / 24.0);
+    p = fma(p, r, 1.0 / 6.0);
+    p = fma(p, r, 0.5);
+    p = fma(p, r, 1.0);
+    p = fma(p, r, 1.0);
+    return __builtin_amdgcn_ldexp(p, (int)n);
 }
 
 template <int TYPE, bool TEMP>
@@ -115,7 +129,7 @@ __global__ __launch_bounds__(256) void stats_kernel(VerifyArgs a, Space w) {
     __shared__ float s_m[4], s_s[4];
     __shared__ int s_i[4];
     float T = 1.0f;
-    if (TEMP) T = a.temperature[uni(request_of(a.cu, a.B, n))];
+    if (TEMP) T = a.temperature[request_of(a.cu, a.B, n)];
     const int64_t row = (int64_t)n * a.ld, from = (int64_t)part * a.seg, to = std::min<int64_t>(from + a.seg, a.V);
     float m = LOWEST, s = 0.0f;
     int first = 0x7FFFFFFF;
@@ -174,20 +188,26 @@ __global__ __launch_bounds__(256) void stats_kernel(VerifyArgs a, Space w) {
     }
 }
 
-// A row's parts as one.
+// A row's parts as one (four at a time on their way).
 __device__ __forceinline__ Stat joined(const VerifyArgs& a, const Space& w, int row, float T) {
     const Stat* p = w.stats + (int64_t)row * a.parts;
-    Stat r = p[0];
     const float k = fminf(LOG2E / T, 3e38f);
-    for (int i = 1; i < a.parts; ++i) {
-        const Stat o = p[i];
-        if (T > 0.0f) {
-            const float m = fmaxf(r.m, o.m);
-            r.s = (r.m == m ? r.s : r.s * exp2f((r.m - m) * k)) + (o.m == m ? o.s : o.s * exp2f((o.m - m) * k));
-            r.m = m;
-        } else {
-            r.s += o.s;
-            if (o.m > r.m || (o.m == r.m && o.first < r.first)) r.m = o.m, r.first = o.first;
+    Stat r{LOWEST, 0.0f, 0x7FFFFFFF, 0};
+    for (int i0 = 0; i0 < a.parts; i0 += 4) {
+        Stat o[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] = p[min(i0 + i, a.parts - 1)];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (i0 + i >= a.parts) continue;
+            if (T > 0.0f) {
+                const float m = fmaxf(r.m, o[i].m);
+                r.s = (r.m == m ? r.s : r.s * exp2f((r.m - m) * k)) + (o[i].m == m ? o[i].s : o[i].s * exp2f((o[i].m - m) * k));
+                r.m = m;
+            } else {
+                r.s += o[i].s;
+                if (o[i].m > r.m || (o[i].m == r.m && o[i].first < r.first)) r.m = o[i].m, r.first = o[i].first;
+            }
         }
     }
     return r;
@@ -350,7 +370,7 @@ __global__ __launch_bounds__(256) void walk_kernel(VerifyArgs a, Space w) {
         load16<TYPE>(a.x, (int64_t)l.row * a.ld + at, (int64_t)l.row * a.ld + end, v);
 #pragma unroll
         for (int i = 0; i < E; ++i) {
-            const double e = exp(((double)v[i] - m) * inv);
+            const double e = exp_of(((double)v[i] - m) * inv);
             const int j = (int)place16<TYPE>(i);
             whole += e;
             rest += s_out[j >> 5] >> (j & 31) & 1 ? 0.0 : e;
@@ -381,6 +401,7 @@ __global__ __launch_bounds__(256) void left_kernel(VerifyArgs a, Space w) {
     const double inv = a.temperature ? 1.0 / (double)a.temperature[b] : 1.0, m = w.left[b].m;
     const double all = total_of(w.whole + (int64_t)b * w.chunks, w.chunks, s_sum);
     const int64_t end = std::min<int64_t>((int64_t)(c + 1) * w.chunk, a.V);
+    const double share = 1.0 / all;
     double rest = 0.0;
     for (int64_t at = (int64_t)c * w.chunk; at < end; at += STEP) {
         float v[E], d[E];
@@ -391,38 +412,41 @@ __global__ __launch_bounds__(256) void left_kernel(VerifyArgs a, Space w) {
             d[i] = j < end ? a.q[(int64_t)q * a.ldq + j] : 0.0f;
         }
 #pragma unroll
-        for (int i = 0; i < E; ++i) rest += fmax(exp(((double)v[i] - m) * inv) / all - (double)d[i], 0.0);
+        for (int i = 0; i < E; ++i) rest += fmax(exp_of(((double)v[i] - m) * inv) * share - (double)d[i], 0.0);
     }
     rest = sum_group(rest, s_sum);
     if (threadIdx.x == 0) w.rest[blockIdx.x] = rest;
 }
 
-// The lowest token whose cumulated sum is above u times the whole.
+// The lowest token whose cumulated sum is above u times the whole: the chunk by one wave, the
+// token by 16, a step of the chunk at a time.
+constexpr int PICK = 1024, PE = STEP / PICK;
+
 template <int TYPE>
-__global__ __launch_bounds__(256) void pick_kernel(VerifyArgs a, Space w) {
+__global__ __launch_bounds__(PICK) void pick_kernel(VerifyArgs a, Space w) {
     __shared__ uint32_t s_out[STEP / 32];
-    __shared__ double s_sum[4], s_pre[4], s_at;
-    __shared__ int s_chunk, s_token;
+    __shared__ double s_pre[PICK / 64], s_before, s_target, s_share;
+    __shared__ int s_chunk, s_some, s_found, s_last;
     const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6);
     const Left& l = w.left[b];
-    if (l.row < 0 || l.best >= 0) {
-        if (tid == 0) a.next[b] = l.row < 0 ? -1 : l.best;
+    const int row = l.row, q = l.q, refused = l.refused;
+    if (row < 0 || l.best >= 0) {
+        if (tid == 0) a.next[b] = row < 0 ? -1 : l.best;
         return;
     }
-    const double* whole = w.whole + (int64_t)b * w.chunks;
-    const double* rest = w.rest + (int64_t)b * w.chunks;
-    const double all = total_of(whole, w.chunks, s_sum);
-    const double left = total_of(rest, w.chunks, s_sum);
-    const bool some = left > 0.0;  // else p itself
-    const double* sums = some ? rest : whole;
-    const bool drafted = some && l.q >= 0;
-    const double target = (double)a.u[max(a.cu[b], 0)] * (some ? left : all);
-    if (tid == 0) s_chunk = -1, s_token = 0;
-    __syncthreads();
-    if (wave == 0) {  // the chunk, 64 at a time; else the last one that has something
-        double before = 0.0;
+    if (wave == 0) {
+        const double* whole = w.whole + (int64_t)b * w.chunks;
+        const double* rest = w.rest + (int64_t)b * w.chunks;
+        const float u = a.u[max(a.cu[b], 0)];
+        double all = 0.0, left = 0.0;
+        for (int i = lane; i < w.chunks; i += 64) all += whole[i], left += rest[i];
+        for (int o = 1; o < 64; o <<= 1) all += __shfl_xor(all, o), left += __shfl_xor(left, o);
+        const bool some = left > 0.0;  // else p itself
+        const double* sums = some ? rest : whole;
+        const double target = (double)u * (some ? left : all);
+        // 64 chunks at a time; where none passes the target (by rounding), the last one that has something
+        double before = 0.0, at = 0.0;
         int chunk = -1;
-        double at = 0.0;
         for (int base = 0; base < w.chunks; base += 64) {
             const double v = base + lane < w.chunks ? sums[base + lane] : 0.0;
             double upto = v;
@@ -436,75 +460,74 @@ __global__ __launch_bounds__(256) void pick_kernel(VerifyArgs a, Space w) {
             if (past) break;
             before += lane_of(upto, 63);
         }
-        if (lane == 0) s_chunk = chunk, s_at = at;
+        if (lane == 0) s_chunk = chunk, s_before = at, s_target = target, s_some = some, s_share = 1.0 / all;
     }
+    if (tid == 0) s_found = 0x7FFFFFFF, s_last = -1;
     __syncthreads();
     if (s_chunk < 0) {  // (nothing anywhere: not for a row that is usable)
         if (tid == 0) a.next[b] = -1;
         return;
     }
-    const double inv = a.temperature ? 1.0 / (double)a.temperature[b] : 1.0, m = l.m;
+    const bool some = s_some, drafted = some && q >= 0;
+    const double inv = a.temperature ? 1.0 / (double)a.temperature[b] : 1.0, m = l.m, target = s_target, share = s_share;
     const int64_t begin = (int64_t)s_chunk * w.chunk, end = std::min<int64_t>(begin + w.chunk, a.V);
-    double before = s_at;
+    double before = s_before;
     for (int64_t at = begin; at < end; at += STEP) {
-        mark(l, at, s_out);
-        // a lane's elements lie next to each other here
-        double e[E], mine = 0.0;
+        float x[PE], d[PE];
 #pragma unroll
-        for (int i = 0; i < E; ++i) {
-            const int in = tid * E + i;
-            const int64_t j = at + in;
-            e[i] = 0.0;
-            if (j < end) {
-                const double x = exp(((double)load1<TYPE>(a.x, (int64_t)l.row * a.ld + j) - m) * inv);
-                if (drafted) e[i] = fmax(x / all - (double)a.q[(int64_t)l.q * a.ldq + j], 0.0);
-                else e[i] = some && (s_out[in >> 5] >> (in & 31) & 1) ? 0.0 : x;
-            }
+        for (int i = 0; i < PE; ++i) {
+            const int64_t j = at + tid * PE + i;
+            x[i] = j < end ? load1<TYPE>(a.x, (int64_t)row * a.ld + j) : -__builtin_inff();
+            d[i] = drafted && j < end ? a.q[(int64_t)q * a.ldq + j] : 0.0f;
+        }
+        if (tid < STEP / 32) s_out[tid] = 0;
+        __syncthreads();
+        if (some && tid < refused) {
+            const int64_t i = l.token[tid] - at;
+            if (i >= 0 && i < STEP) atomicOr(&s_out[i >> 5], 1u << (i & 31));
+        }
+        __syncthreads();
+        double e[PE], mine = 0.0;
+#pragma unroll
+        for (int i = 0; i < PE; ++i) {
+            const int in = tid * PE + i;
+            e[i] = exp_of(((double)x[i] - m) * inv);
+            if (drafted) e[i] = fmax(e[i] * share - (double)d[i], 0.0);
+            else if (s_out[in >> 5] >> (in & 31) & 1) e[i] = 0.0;
             mine += e[i];
         }
         double upto = mine;
         for (int o = 1; o < 64; o <<= 1) {
-            const double x = __shfl_up(upto, o);
-            if (lane >= o) upto += x;
+            const double y = __shfl_up(upto, o);
+            if (lane >= o) upto += y;
         }
-        __syncthreads();
         if (lane == 63) s_pre[wave] = upto;
         __syncthreads();
         double base = before, step = 0.0;
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < PICK / 64; ++i) {
             if (i < wave) base += s_pre[i];
             step += s_pre[i];
         }
         double sum = base + upto - mine;
         int found = 0x7FFFFFFF, last = -1;
 #pragma unroll
-        for (int i = 0; i < E; ++i) {
+        for (int i = 0; i < PE; ++i) {
             sum += e[i];
             if (e[i] > 0.0) {
-                last = (int)(at + tid * E + i);
+                last = (int)(at + tid * PE + i);
                 if (found == 0x7FFFFFFF && sum > target) found = last;
             }
         }
-        for (int o = 1; o < 64; o <<= 1) {
-            found = min(found, __shfl_xor(found, o));
-            last = max(last, __shfl_xor(last, o));
-        }
-        __shared__ int s_found[4], s_last[4];
-        if (lane == 0) s_found[wave] = found, s_last[wave] = last;
+        // (of a wave the first and the last: a thousand at one place would wait for each other)
+        const uint64_t passed = __ballot(found != 0x7FFFFFFF), any = __ballot(last >= 0);
+        if (passed && lane == __builtin_ctzll(passed)) atomicMin(&s_found, found);
+        if (any && lane == 63 - __builtin_clzll(any)) atomicMax(&s_last, last);
         __syncthreads();
-        if (tid == 0) {
-            for (int i = 0; i < 4; ++i) found = min(found, s_found[i]), last = max(last, s_last[i]);
-            if (found != 0x7FFFFFFF) {
-                a.next[b] = found;
-                s_token = 1;
-            } else if (last >= 0) {
-                a.next[b] = last;  // (stays where rounding leaves the chunk's end below the target)
-            }
-        }
-        __syncthreads();
-        if (s_token) return;
+        if (s_found != 0x7FFFFFFF) break;
         before += step;
     }
+    // (the last one that counts, where rounding leaves the chunk's end below the target)
+    if (tid == 0) a.next[b] = s_found != 0x7FFFFFFF ? s_found : s_last;
 }
 
 template <int TYPE>
@@ -516,7 +539,7 @@ hipError_t go(const VerifyArgs& a, const Space& w, hipStream_t st) {
     }
     hipLaunchKernelGGL(walk_kernel<TYPE>, sums, t, 0, st, a, w);
     if (a.q) hipLaunchKernelGGL(left_kernel<TYPE>, sums, t, 0, st, a, w);
-    hipLaunchKernelGGL(pick_kernel<TYPE>, dim3((unsigned)a.B), t, 0, st, a, w);
+    hipLaunchKernelGGL(pick_kernel<TYPE>, dim3((unsigned)a.B), dim3(PICK), 0, st, a, w);
     return hipGetLastError();
 }
 
