@@ -14,14 +14,16 @@ __device__ __forceinline__ float inverse_of(float s) { return s >= TINY && s < _
 // A scale read from a cache: 0 where it is no positive finite number.
 __device__ __forceinline__ float held_scale(float s) { return s > 0.0f && s < __builtin_inff() ? s : 0.0f; }
 
-// x / scale to the nearest code (ties to even), held to -127 .. 127; NaN: 0.
+// x / scale to the nearest code (ties to even), held to -127 .. 127; NaN (an infinity times 0
+// as well): 0, as the conversion has it, which also holds what is beyond integers to their ends.
 __device__ __forceinline__ int code_of(float x, float inverse) {
-    const float y = x * inverse;  // (an infinity times 0 is NaN as well)
-    return y == y ? (int)rintf(fminf(fmaxf(y, -127.0f), 127.0f)) : 0;
+    int i;
+    asm("v_cvt_i32_f32 %0, %1" : "=v"(i) : "v"(rintf(x * inverse)));
+    return min(max(i, -127), 127);
 }
 __device__ __forceinline__ uint32_t four_codes(float a, float b, float c, float d, float inverse) {
-    return (uint32_t)(code_of(a, inverse) & 255) | (uint32_t)(code_of(b, inverse) & 255) << 8 |
-           (uint32_t)(code_of(c, inverse) & 255) << 16 | (uint32_t)code_of(d, inverse) << 24;
+    const uint32_t ab = __builtin_amdgcn_perm(code_of(b, inverse), code_of(a, inverse), 0x0C0C0400u);
+    return __builtin_amdgcn_perm(code_of(d, inverse), code_of(c, inverse), 0x04000C0Cu) | ab;
 }
 __device__ __forceinline__ float code_at(uint32_t w, int i) { return (float)(int8_t)(w >> (8 * i)); }
 

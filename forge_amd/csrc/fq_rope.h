@@ -4,12 +4,41 @@
 
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "fq_step.h"
 
 namespace fq {
 
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
+
+// f over the group's GS lanes, in each of them, by halves of pairs: within rows of 16 by data-parallel moves,
+// beyond by swaps of rows.  (Of lanes that hold the same, which of them a move takes is the same.)
+template <int GS, class F>
+__device__ __forceinline__ float over_group(float x, F f) {
+    typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+    const auto moved = [&](auto ctrl) {
+        return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), ctrl.value, 0xF, 0xF, false));
+    };
+    x = f(x, moved(std::integral_constant<int, 0xB1>()));   // lanes 1 0 3 2 of each four
+    x = f(x, moved(std::integral_constant<int, 0x4E>()));   // 2 3 0 1
+    x = f(x, moved(std::integral_constant<int, 0x141>()));  // the other four of eight
+    if constexpr (GS >= 16) x = f(x, moved(std::integral_constant<int, 0x140>()));  // the other eight of 16
+    if constexpr (GS >= 32) {
+        const uint32_t u = __builtin_bit_cast(uint32_t, x);
+        const u2 p = __builtin_bit_cast(u2, __builtin_amdgcn_permlane16_swap(u, u, false, false));
+        const uint32_t a = p[0], b = p[1];
+        x = f(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
+    }
+    if constexpr (GS >= 64) {
+        const uint32_t u = __builtin_bit_cast(uint32_t, x);
+        const u2 p = __builtin_bit_cast(u2, __builtin_amdgcn_permlane32_swap(u, u, false, false));
+        const uint32_t a = p[0], b = p[1];
+        x = f(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
+    }
+    return x;
+}
 
 // A lane's elements d0 .. d0+3 and d1 .. d1+3 of head h of token n (none where not on: lanes past
 // D / 8 and those the caller leaves out, which still have their part in the norm's sums).  The
@@ -39,7 +68,7 @@ __device__ __forceinline__ HeadRuns head_runs(const RopeArgs& a, int n, int h, i
     if (wt) {
         float ss = 0.0f;
         for (int i = 0; i < 4; ++i) ss = fmaf(x0[i], x0[i], fmaf(x1[i], x1[i], ss));
-        for (int o = 1; o < GS; o <<= 1) ss += __shfl_xor(ss, o, GS);
+        ss = over_group<GS>(ss, [](float u, float v) { return u + v; });
         const float r = 1.0f / sqrtf(ss / (float)a.D + a.eps);
         if (on) {
             const f4 w0 = *(const f4u*)(wt + d0), w1 = *(const f4u*)(wt + d1);

@@ -39,14 +39,8 @@ __global__ __launch_bounds__(256) void rope8_kernel(RopeArgs a, Cache8 c, int kv
     const int hh = blockIdx.x % (2 * c.hkv), n0 = blockIdx.x / (2 * c.hkv) * W;
     const int h = hh % c.hkv;
     const bool isv = hh >= c.hkv;
-    __shared__ int s_slot[2 * W + 1];
-    __shared__ float s_max[2 * W];
-    // (the first tokens' rows are on their way before it shows which of them are this work-group's)
-    HeadRuns x[R];
-#pragma unroll
-    for (int r = 0; r < R; ++r)
-        if ((r + 1) * TOK <= W)
-            x[r] = head_runs<GS, INTER>(a, n0 + r * TOK + sub, a.hq + hh, p, lane_on && n0 + r * TOK + sub < a.N);
+    __shared__ int s_slot[2 * W + 1], s_max[W];
+    __shared__ float s_inv[W];
     // slots of tokens n0 - 1 .. n0 + 31
     if (threadIdx.x < 2 * W + 1) {
         const int n = n0 - 1 + (int)threadIdx.x;
@@ -54,63 +48,77 @@ __global__ __launch_bounds__(256) void rope8_kernel(RopeArgs a, Cache8 c, int kv
         if (slot < 0 || (slot >> c.c.bs_log2) >= c.c.num_blocks) slot = -1;
         s_slot[threadIdx.x] = slot;
     }
+    if (threadIdx.x < W) s_max[threadIdx.x] = 0;
     __syncthreads();
-    // bit j: token n0 + j goes on with the run of the one before
-    uint32_t goes_on = 0;
+    // bit j: token n0 + j has a slot; goes on with the run of the one before
+    uint32_t there, goes_on;
     {
         const int j = threadIdx.x & 31, slot = s_slot[j + 1];
-        const bool on = slot >= 0 && slot % GROUP && s_slot[j] == slot - 1;
-        goes_on = (uint32_t)__ballot(on);
+        there = (uint32_t)__ballot(slot >= 0);
+        goes_on = (uint32_t)__ballot(slot >= 0 && slot % GROUP && s_slot[j] == slot - 1);
     }
-    int slot[R], lead[R];  // lead: where the token's run begins; -1: not this work-group's
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-        const int j = r * TOK + sub;
-        slot[r] = j < 2 * W ? s_slot[j + 1] : -1;
-        lead[r] = -1;
-        if (slot[r] >= 0) {
-            const uint32_t begins = ~goes_on & (j < 31 ? (2u << j) - 1 : ~0u);
-            lead[r] = begins ? 31 - __builtin_clz(begins) : -1;
-            if (lead[r] >= W) lead[r] = -1;
-        }
-        if ((r + 1) * TOK > W) x[r] = head_runs<GS, INTER>(a, n0 + j, a.hq + hh, p, lane_on && lead[r] >= 0);
-        float m = 0.0f;
-        if (lane_on && lead[r] >= 0)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) m = largest(largest(m, x[r].x0[i]), x[r].x1[i]);
-        for (int o = 1; o < GS; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, GS));
-        if (p == 0 && j < 2 * W) s_max[j] = m;
-    }
-    __syncthreads();
+    // the tokens from the first run that begins among the W on to the end of the last one that does
+    const uint32_t begins = there & ~goes_on & ((1u << W) - 1);
+    if (!begins) return;
+    const int from = __builtin_ctz(begins);
+    int end = 32 - __builtin_clz(begins);
+    end += __builtin_ctzll(~(uint64_t)(goes_on >> end));  // (a run has 16 tokens at most)
     int8_t* cache = (isv ? c.v : c.k) + (int64_t)h * c.c.sh;
     float* scales = isv ? c.vs : c.ks;
+    HeadRuns x[R];
+    int slot[R], lead[R];  // lead: where the token's run begins; -1: none
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        if (lead[r] < 0) continue;
-        const int j = r * TOK + sub;
-        const int page = slot[r] >> c.c.bs_log2, row = slot[r] & ((1 << c.c.bs_log2) - 1);
+        lead[r] = -1;
+        if (from + r * TOK >= end) continue;
+        const int j = from + r * TOK + sub;
+        if (j < end && (there >> j & 1)) {
+            slot[r] = s_slot[j + 1];
+            lead[r] = 31 - __builtin_clz(there & ~goes_on & ((2u << j) - 1));
+        }
+        const bool on = lane_on && lead[r] >= 0;
+        x[r] = head_runs<GS, INTER>(a, n0 + j, a.hq + hh, p, on);
+        const auto most = [](float u, float v) { return fmaxf(u, v); };
+        float m = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m = fmaxf(fmaxf(m, fabsf(x[r].x0[i])), fabsf(x[r].x1[i]));
+        if (__any(on && m == __builtin_inff())) {  // of the finite ones
+            m = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) m = largest(largest(m, x[r].x0[i]), x[r].x1[i]);
+        }
+        m = over_group<GS>(on ? m : 0.0f, most);
+        if (p == 0 && lead[r] >= 0) atomicMax(&s_max[lead[r]], __builtin_bit_cast(int, m));
+    }
+    __syncthreads();
+    // A run's scale, by its first token's lanes.
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int j = from + r * TOK + sub;
+        if (lead[r] < 0 || lead[r] != j) continue;
+        const int page = slot[r] >> c.c.bs_log2, row = slot[r] & ((1 << c.c.bs_log2) - 1), held = row % GROUP;
         float* sp = scales + ((int64_t)page * c.hkv + h) * c.groups() + row / GROUP;
-        // the run's largest: its tokens follow `lead` without a gap
-        float m = s_max[lead[r]];
-        for (int i = lead[r] + 1; i < 2 * W && (goes_on >> i & 1); ++i) m = fmaxf(m, s_max[i]);
-        const int held = row % GROUP - (j - lead[r]);  // tokens before the run
-        const float need = m / 127.0f, old = held ? held_scale(*sp) : 0.0f;
+        const float need = __builtin_bit_cast(float, s_max[j]) / 127.0f, old = held ? held_scale(*sp) : 0.0f;
         const float s = fmaxf(need, old), inv = inverse_of(s);
-        if (!lane_on) continue;
-        int8_t* to = cache + page * c.c.sb + row * c.c.st;
+        if (p == 0) s_inv[j] = inv, *sp = s;
+        if (s > old && lane_on) {
+            const float times = old * inv;
+            int8_t* to = cache + page * c.c.sb + row * c.c.st + 8 * p;
+            for (int i = 1; i <= held; ++i) {
+                uint2* w = (uint2*)(to - i * c.c.st);
+                *w = make_uint2(again(w->x, times), again(w->y, times));
+            }
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        if (lead[r] < 0 || !lane_on) continue;
+        const float inv = s_inv[lead[r]];
+        int8_t* to = cache + (slot[r] >> c.c.bs_log2) * c.c.sb + (slot[r] & ((1 << c.c.bs_log2) - 1)) * c.c.st;
         const f4 y0 = x[r].x0, y1 = x[r].x1;
         *(uint32_t*)(to + x[r].d0) = four_codes(y0[0], y0[1], y0[2], y0[3], inv);
         *(uint32_t*)(to + x[r].d1) = four_codes(y1[0], y1[1], y1[2], y1[3], inv);
-        if (j == lead[r]) {
-            if (s > old) {
-                const float times = old * inv;
-                for (int i = 1; i <= held; ++i) {
-                    uint2* w = (uint2*)(to - i * c.c.st + 8 * p);
-                    *w = make_uint2(again(w->x, times), again(w->y, times));
-                }
-            }
-            if (p == 0) *sp = s;
-        }
     }
 }
 
