@@ -300,25 +300,28 @@ __device__ __forceinline__ void walk(const VerifyArgs& a, const Space& w, int b,
                 u = (double)a.u[t0 + lane];
                 p = chance(lane, par);
             }
-            for (int j = 1; j < n; ++j) {  // refused before already
-                const int pj = __builtin_amdgcn_readlane(par, j), tj = __builtin_amdgcn_readlane(token, j);
-                if (j < lane && pj == par && tj == token) p = 0.0;
-            }
-            double mass = 1.0;
+            // The siblings before a token, as bits; one that was refused before already has nothing.
+            uint64_t siblings = 0;
+            bool refused_before = false;
             for (int j = 1; j < n; ++j) {
-                const int pj = __builtin_amdgcn_readlane(par, j);
-                const double v = lane_of(p, j);
-                if (j < lane && pj == par) mass -= v;
+                const bool is = j < lane && __builtin_amdgcn_readlane(par, j) == par;
+                siblings |= (uint64_t)is << j;
+                refused_before |= is && __builtin_amdgcn_readlane(token, j) == token;
             }
-            bool good = par >= 0 && u * mass < p;
-            const uint64_t all = __ballot(good);
-            bool before = false;
-            for (int j = 1; j < n; ++j)
-                before |= j < lane && (all >> j & 1) && __builtin_amdgcn_readlane(par, j) == par;
-            const uint64_t pass = __ballot(good && !before);
+            if (par < 0) siblings = 0;
+            if (refused_before) p = 0.0;
+            double mass = 1.0;
+            for (uint64_t rest = siblings; __any(rest != 0); rest &= rest - 1) {
+                const double v = __shfl(p, rest ? __builtin_ctzll(rest) : 0);
+                if (rest) mass -= v;
+            }
+            const uint64_t good = __ballot(par >= 0 && u * mass < p);
+            const uint64_t pass = __ballot((good >> lane & 1) && !(siblings & good));
             uint64_t acc = 1;
-            for (int i = 1; i < n; ++i)
-                if (pass >> i & 1) acc |= (acc >> __builtin_amdgcn_readlane(par, i) & 1) << i;
+            for (uint64_t more = 1; more;) {  // a level of the branch at a time
+                more = __ballot((pass >> lane & 1) && (acc >> (par & 63) & 1)) & ~acc;
+                acc |= more;
+            }
             accepted = __builtin_popcountll(acc);
             last = 63 - __builtin_clzll(acc);
             if (out) {
