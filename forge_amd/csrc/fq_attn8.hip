@@ -563,14 +563,15 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
                     for (int d = 0; d < DT; ++d)
                         raw[d] = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
                             (lds_i2*)(uintptr_t)(vlane[d & 3] + stage * S::STAGE + (d >> 2) * 64));
-                }, [&](int s) {
-                    // the rows' maxima, then their groups' exponentials, spread over the runs
-                    constexpr int PIECES = (1 + SUBS) * NR, RUNS = STEPS * LIMBS;
+                    // (the rows' maxima while the keys are on their way from LDS)
+                    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                    for (int x = s * PIECES / RUNS; x < (s + 1) * PIECES / RUNS; ++x) {
-                        if (x < NR) maximum(x);
-                        else exponentials((x - NR) / SUBS, (x - NR) % SUBS);
-                    }
+                    for (int c = 0; c < NR; ++c) maximum(c);
+                }, [&](int s) {
+                    // the groups' exponentials, spread over the runs
+                    constexpr int PIECES = SUBS * NR, RUNS = STEPS * LIMBS;
+#pragma unroll
+                    for (int x = s * PIECES / RUNS; x < (s + 1) * PIECES / RUNS; ++x) exponentials(x / SUBS, x % SUBS);
                 });
                 __builtin_amdgcn_s_setprio(0);
                 if (__any(moved))
@@ -579,42 +580,34 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
 #pragma unroll
                         for (int d = 0; d < DT; ++d) o[d][c] *= alpha[c];
 
-                const auto value = [&](int d) {
-                    const i2 w = raw[d];
-                    const uint32_t w0 = (uint32_t)w[0], w1 = (uint32_t)w[1];
-                    u4 r;
+                // Two of the columns' 16s at a time.  After each of their matrix instructions, while the unit
+                // has it: four codes of the next two's, or some of the next scores.
+                const auto four = [&](int d, int half, u4& to) {
                     uint32_t x, y;
-                    four_halves(w0, x, y);
-                    r[0] = x, r[1] = y;
-                    four_halves(w1, x, y);
-                    r[2] = x, r[3] = y;
-                    return __builtin_bit_cast(h8, r);
+                    four_halves((uint32_t)raw[d][half], x, y);
+                    to[2 * half] = x, to[2 * half + 1] = y;
                 };
-                // Two of the columns' 16s at a time: their matrix instructions, and between these, while the
-                // unit has them, the next two's conversion and some of the next scores.
-                h8 vf[2] = {value(0), value(1)};
+                u4 vf[2];
+#pragma unroll
+                for (int x = 0; x < 4; ++x) four(x >> 1, x & 1, vf[x >> 1]);
 #pragma unroll
                 for (int d = 0; d < DT; d += 2) {
-                    h8 after[2];
+                    constexpr int RUN = 4 * NR, SCORES = SUBS * NR * 4, TWOS = DT / 2;
+                    u4 after[2];
 #pragma unroll
-                    for (int l = 1; l >= 0; --l)
+                    for (int m = 0; m < RUN; ++m) {
+                        const int l = m < RUN / 2, x = m / NR % 2, c = m % NR;  // (the lower parts first)
+                        o[d + x][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                            __builtin_bit_cast(h8, vf[x]), __builtin_bit_cast(h8, l ? pl[c] : ph[c]), o[d + x][c], 0, 0, 0);
+                        if (d + 2 < DT && m % NR == 0) four(d + 2 + m / NR / 2, m / NR % 2, after[m / NR / 2]);
+                        const int s0 = d / 2 * SCORES / TWOS, s1 = (d / 2 + 1) * SCORES / TWOS;
 #pragma unroll
-                        for (int x = 0; x < 2; ++x)
-#pragma unroll
-                            for (int c = 0; c < NR; ++c)
-                                o[d + x][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                                    vf[x], __builtin_bit_cast(h8, l ? pl[c] : ph[c]), o[d + x][c], 0, 0, 0);
-                    if (d + 2 < DT) after[0] = value(d + 2), after[1] = value(d + 3);
-                    constexpr int PIECES = SUBS * NR, RUNS = DT / 2;
-#pragma unroll
-                    for (int x = d / 2 * PIECES / RUNS; x < (d / 2 + 1) * PIECES / RUNS; ++x)
-                        score(low, high, sc, x / NR, x % NR);
-#pragma unroll
-                    for (int x = 0; x < 4 * NR; ++x) {
-                        __builtin_amdgcn_sched_group_barrier(8, 1, 0);
-                        __builtin_amdgcn_sched_group_barrier(2, NR == 1 ? 7 : 4, 0);
+                        for (int e = s0 + m * (s1 - s0) / RUN; e < s0 + (m + 1) * (s1 - s0) / RUN; ++e) {
+                            const int sub = e / 4 / NR, k = e / 4 % NR, r = e % 4;
+                            sc[sub][k][r] = (float)((high[sub][k][r] << 8) + low[sub][k][r]);
+                        }
+                        __builtin_amdgcn_sched_barrier(0);
                     }
-                    __builtin_amdgcn_sched_barrier(0);
                     if (d + 2 < DT) vf[0] = after[0], vf[1] = after[1];
                 }
                 if constexpr (WR == 1) {
