@@ -140,7 +140,7 @@ __device__ __forceinline__ bool no_block(const AttnArgs& a, int page) {
 }
 constexpr int DESC = 4;          // ints of a work-group's record, beside the number of parts
 constexpr int MAX_ITEMS = 1024;  // work-groups at most
-constexpr int MAX_GRID = 3;      // work-groups to a CU at most,
+constexpr int MAX_GRID = 4;      // work-groups to a CU at most,
 constexpr size_t MAX_PART = 3 * 64 * (128 + 2);  // and floats of a part of all of them
 
 

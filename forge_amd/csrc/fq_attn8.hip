@@ -729,12 +729,11 @@ template <int D>
 hipError_t rows(const AttnArgs& a, int max_new, int cus, uint8_t* ws, hipStream_t st) {
     const int64_t r = (int64_t)max_new * a.G;
     if constexpr (D == 256) {
-        if (r <= 16) return go<Shape<D, 1, 1, 2, 2, 2>>(a, max_new, cus, ws, st);
-        if (r <= 32) return go<Shape<D, 1, 2, 2, 3, 1>>(a, max_new, cus, ws, st);
+        if (r <= 32) return go<Shape<D, 1, 1, 2, 2, 2>>(a, max_new, cus, ws, st);
         return go<Shape<D, 1, 2, 1, 3, 2>>(a, max_new, cus, ws, st);
     } else {
-        if (r <= (D == 64 ? 32 : 16)) return go<Shape<D, 1, 1, 4, 2, 2>>(a, max_new, cus, ws, st);
-        if (r <= 96) return go<Shape<D, 2, 1, 4, 2, 2>>(a, max_new, cus, ws, st);
+        if (r <= 32) return go<Shape<D, 1, 1, 4, 2, 2>>(a, max_new, cus, ws, st);
+        if (r <= 128) return go<Shape<D, 2, 1, 2, 2, 4>>(a, max_new, cus, ws, st);
         return go<Shape<D, 2, 2, 2, 3, 2>>(a, max_new, cus, ws, st);
     }
 }
