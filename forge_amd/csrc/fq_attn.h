@@ -140,6 +140,7 @@ __device__ __forceinline__ bool no_block(const AttnArgs& a, int page) {
 }
 constexpr int DESC = 4;          // ints of a work-group's record, beside the number of parts
 constexpr int MAX_ITEMS = 1024;  // work-groups at most
+constexpr int WIDE = MAX_ITEMS * (DESC + 1);  // behind them: whether an item may have more than NARROW parts
 constexpr int MAX_GRID = 4;      // work-groups to a CU at most,
 constexpr size_t MAX_PART = 3 * 64 * (128 + 2);  // and floats of a part of all of them
 
@@ -150,7 +151,7 @@ constexpr size_t MAX_PART = 3 * 64 * (128 + 2);  // and floats of a part of all 
 constexpr int JOIN_WGS = 8;  // work-groups to a CU
 constexpr int NARROW = 16;   // parts of an item that one wave joins
 
-template <int D, int RT>
+template <int D, int RT, bool NEAR = false>
 __global__ __launch_bounds__(256) void attn_join(AttnArgs a) {
     constexpr int PART = RT * (D + 2), E = D == 64 ? 1 : D == 256 ? 4 : 2;
     typedef float fe __attribute__((ext_vector_type(E)));
@@ -161,6 +162,65 @@ __global__ __launch_bounds__(256) void attn_join(AttnArgs a) {
     __shared__ int s_count[4], s_most[4];
     __shared__ float s_acc[4][D + 1];
     const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6);
+    const auto slot = [&](const Item& x, int p) {
+        return a.part + (int64_t)(2 * (x.w + p) + (p == 0)) * PART;
+    };
+    const auto store = [&](const Item& x, int r, fe acc, float l) {
+        const int t = r / a.G;
+        fe v = 0.0f;
+        if (l != 0.0f) v = acc * (1.0f / l);
+        if (E * lane < D)
+            *(fe*)(a.out + ((int64_t)(x.t0 + t) * a.hq + x.h * a.G + r % a.G) * D + E * lane) = v;
+    };
+    // Two rows of an item of few parts, rl the first one's place among its RT.
+    constexpr int R = 2;
+    const auto two_rows = [&](const Item& x, int rl) {
+        const int r0 = x.rt * RT + rl;
+        if (r0 >= x.nt * a.G) return;
+        float mp[R], lp[R];
+        fe o[R][NARROW];
+#pragma unroll
+        for (int k = 0; k < R; ++k) {
+            mp[k] = LOWEST, lp[k] = 0.0f;
+            const bool on = r0 + k < x.nt * a.G;
+            if (on && lane < x.parts) {
+                const float* s = slot(x, lane) + RT * D + rl + k;
+                mp[k] = s[0], lp[k] = s[RT];
+            }
+#pragma unroll
+            for (int p = 0; p < NARROW; ++p) {
+                o[k][p] = 0.0f;
+                if (on && p < x.parts && E * lane < D) o[k][p] = *(const fe*)(slot(x, p) + (rl + k) * D + E * lane);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < R; ++k) {
+            float m = mp[k];
+            for (int q = NARROW / 2; q; q >>= 1) m = fmaxf(m, __shfl_xor(m, q));
+            m = __shfl(m, 0);
+            const float f = __builtin_amdgcn_exp2f(mp[k] - m);
+            float l = lp[k] * f;
+            for (int q = NARROW / 2; q; q >>= 1) l += __shfl_xor(l, q);
+            l = __shfl(l, 0);
+            fe acc = 0.0f;
+#pragma unroll
+            for (int p = 0; p < NARROW; ++p)
+                if (p < x.parts) acc += __shfl(f, p) * o[k][p];
+            if (r0 + k < x.nt * a.G) store(x, r0 + k, acc, l);
+        }
+    };
+    if (NEAR && !a.desc[WIDE]) {
+        // No item has many parts: a work-group takes those of one work-group's, a share of its rows,
+        // and looks at no other's.
+        const int w = blockIdx.x % a.grid, c = blockIdx.x / a.grid, share = gridDim.x / a.grid;
+        if (c >= share) return;
+        const int parts = a.desc[w];
+        const int4 rec = ((const int4*)(a.desc + MAX_ITEMS))[w];
+        if (!parts) return;
+        const Item x{parts, w, rec.x, rec.y, rec.z, rec.w};
+        for (int job = c * 4 + wave; job < RT / R; job += share * 4) two_rows(x, job * R);
+        return;
+    }
     // the items, in the order of the work-groups that began them: thread i looks at
     // the K next to each other from K i on
     constexpr int K = MAX_ITEMS / 256;
@@ -193,54 +253,9 @@ __global__ __launch_bounds__(256) void attn_join(AttnArgs a) {
     for (int k = 0; k < K; ++k)
         if (parts[k]) s_item[at++] = {parts[k], tid * K + k, rec[k].x, rec[k].y, rec[k].z, rec[k].w};
     __syncthreads();
-    const auto slot = [&](const Item& x, int p) {
-        return a.part + (int64_t)(2 * (x.w + p) + (p == 0)) * PART;
-    };
-    const auto store = [&](const Item& x, int r, fe acc, float l) {
-        const int t = r / a.G;
-        fe v = 0.0f;
-        if (l != 0.0f) v = acc * (1.0f / l);
-        if (E * lane < D)
-            *(fe*)(a.out + ((int64_t)(x.t0 + t) * a.hq + x.h * a.G + r % a.G) * D + E * lane) = v;
-    };
     if (most <= NARROW) {
-        constexpr int R = 2;
-        for (int job = blockIdx.x * 4 + wave; job < items * (RT / R); job += gridDim.x * 4) {
-            const Item x = s_item[job / (RT / R)];
-            const int rl = job % (RT / R) * R, r0 = x.rt * RT + rl;
-            if (r0 >= x.nt * a.G) continue;
-            float mp[R], lp[R];
-            fe o[R][NARROW];
-#pragma unroll
-            for (int k = 0; k < R; ++k) {
-                mp[k] = LOWEST, lp[k] = 0.0f;
-                const bool on = r0 + k < x.nt * a.G;
-                if (on && lane < x.parts) {
-                    const float* s = slot(x, lane) + RT * D + rl + k;
-                    mp[k] = s[0], lp[k] = s[RT];
-                }
-#pragma unroll
-                for (int p = 0; p < NARROW; ++p) {
-                    o[k][p] = 0.0f;
-                    if (on && p < x.parts && E * lane < D) o[k][p] = *(const fe*)(slot(x, p) + (rl + k) * D + E * lane);
-                }
-            }
-#pragma unroll
-            for (int k = 0; k < R; ++k) {
-                float m = mp[k];
-                for (int q = NARROW / 2; q; q >>= 1) m = fmaxf(m, __shfl_xor(m, q));
-                m = __shfl(m, 0);
-                const float f = __builtin_amdgcn_exp2f(mp[k] - m);
-                float l = lp[k] * f;
-                for (int q = NARROW / 2; q; q >>= 1) l += __shfl_xor(l, q);
-                l = __shfl(l, 0);
-                fe acc = 0.0f;
-#pragma unroll
-                for (int p = 0; p < NARROW; ++p)
-                    if (p < x.parts) acc += __shfl(f, p) * o[k][p];
-                if (r0 + k < x.nt * a.G) store(x, r0 + k, acc, l);
-            }
-        }
+        for (int job = blockIdx.x * 4 + wave; job < items * (RT / R); job += gridDim.x * 4)
+            two_rows(s_item[job / (RT / R)], job % (RT / R) * R);
         return;
     }
     for (int job = blockIdx.x; job < items * RT; job += gridDim.x) {
@@ -292,7 +307,7 @@ __global__ __launch_bounds__(256) void attn_join(AttnArgs a) {
     }
 }
 
-constexpr size_t DESC_BYTES = (size_t)MAX_ITEMS * (DESC + 1) * 4;
+constexpr size_t DESC_BYTES = (size_t)MAX_ITEMS * (DESC + 1) * 4 + 16;
 
 }  // namespace
 }  // namespace fq

@@ -124,9 +124,12 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
     {
         const int first = lane * per;
         int64_t mine = 0;
+        int longest = 0;
         for (int i = first; i < min(first + per, a.B); ++i) {
             cu0 = a.cu[i], cu1 = a.cu[i + 1], cached = a.lengths[i];
-            mine += request<RT, KU, OV, true>(a, cu0, cu1, cached).units;
+            const Request rq = request<RT, KU, OV, true>(a, cu0, cu1, cached);
+            mine += rq.units;
+            if (rq.units) longest = max(longest, rq.cost);
         }
         int64_t upto = mine;
         for (int o = 1; o < 64; o <<= 1) {
@@ -135,6 +138,11 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
         }
         total = uni64(__shfl(upto, 63));
         span = divided(total + gridDim.x - 1, gridDim.x);
+        // (an item of `longest` units lies on that many work-groups and one at most)
+        if (wg == 0) {
+            const bool wide = __any(longest > (NARROW - 2) * span);
+            if (tid == 0) a.desc[WIDE] = wide;
+        }
         const int64_t u0 = wg * span;
         const uint64_t past = __ballot(upto > u0);
         const int at = past ? __builtin_ctzll(past) : 0;
@@ -721,7 +729,7 @@ hipError_t go(AttnArgs a, int max_new, int cus, uint8_t* ws, hipStream_t st) {
     a.part = (float*)(ws + DESC_BYTES);
     a.whole = uncut<S>(a, max_new);
     hipLaunchKernelGGL(attn8_kernel<S>, dim3(a.grid), dim3(64 * S::WAVES), S::LDS, st, a);
-    if (!a.whole) hipLaunchKernelGGL((attn_join<S::D, S::RT>), dim3(JOIN_WGS * cus), dim3(256), 0, st, a);
+    if (!a.whole) hipLaunchKernelGGL((attn_join<S::D, S::RT, true>), dim3(std::max(JOIN_WGS * cus, a.grid)), dim3(256), 0, st, a);
     return hipGetLastError();
 }
 
