@@ -356,6 +356,8 @@ __global__ __launch_bounds__(256) void walk_kernel(VerifyArgs a, Space w) {
     if (tid < 64) walk<TYPE>(a, w, b, c == 0, s_left);
     if (b == a.B - 1 && c == 0)  // padding
         for (int64_t i = std::max(a.cu[a.B], 0) + tid; i < a.N; i += 256) a.path[i] = -1;
+    if (b == 0 && c == 0)  // (cu begins with 0; what lay before it would be nobody's)
+        for (int i = tid; i < std::min(a.cu[0], a.N); i += 256) a.path[i] = -1;
     __syncthreads();
     const Left& l = s_left;
     if (c == 0) {
