@@ -367,7 +367,7 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
                 const bool on = t < nt;
                 // (a chain: how many of the new tokens the row sees)
                 mask[c] = !on ? 0 : a.masks ? a.masks[t0 + t] : (uint64_t)t + 1;
-                from[c] = 0;
+                from[c] = 0x7FFFFFFF;  // (a row of nobody's sees none of what the others do not)
                 if (WIN && on) {
                     const Reach r = reach(a, len, t, mask[c]);
                     mask[c] = r.mask, from[c] = r.from;
@@ -510,13 +510,16 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
                     const uint32_t in = holes ? there(i) : ~0u;
 #pragma unroll
                     for (int c = 0; c < NR; ++c) {
-                        mul[c] = 1.0f;
+                        // (with a window a tile seen in part has the bits of one seen whole, whichever it is:
+                        // but for factors of 0 and NaN, which would make NaN of the infinity)
+                        const bool later = WIN && rs[c] > 0.0f;
+                        mul[c] = later ? rs[c] : 1.0f;
                         const uint32_t see = (seen<WIN>(a, mask[c], from[c], key0, old, all) & in) >> (4 * g);
 #pragma unroll
                         for (int sub = 0; sub < 2; ++sub)
 #pragma unroll
                             for (int r = 0; r < 4; ++r)
-                                sc[sub][c][r] = see >> (16 * sub + r) & 1 ? sc[sub][c][r] * rs[c]
+                                sc[sub][c][r] = see >> (16 * sub + r) & 1 ? (later ? sc[sub][c][r] : sc[sub][c][r] * rs[c])
                                                                           : -__builtin_inff();
                     }
                     // values that are not finite: zeros, and noted where they are the request's.
@@ -754,9 +757,8 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
     if (!cut && tid == 0) a.desc[wg] = 0;
 }
 
-
 template <class S>
-hipError_t go(AttnArgs a, int cus, uint8_t* ws, hipStream_t st) {
+hipError_t go(AttnArgs a, int max_new, int cus, uint8_t* ws, hipStream_t st) {
     a.grid = S::PC * cus;
     a.desc = (int*)ws;
     a.part = (float*)(ws + DESC_BYTES);
@@ -764,9 +766,10 @@ hipError_t go(AttnArgs a, int cus, uint8_t* ws, hipStream_t st) {
     // cut, and there is nothing to join: six units take about as long as a second launch
     // (one of 333 keys, D = 64: 12.4 us, cut 10.0 + 6.1; 64 of 370, one token: 23.1, cut
     // 25.8 + 6.6; 8 of 340, 8 tokens: 21.1, cut 15.3 + 6.2).  In a wider table the same
-    // requests are cut: nothing on the host knows the lengths.
-    a.whole = (int64_t)a.max_blocks << a.c.bs_log2 <= 6 * std::max(S::KU, 64);
+    // requests are cut: nothing on the host knows the lengths.  A window bounds them also:
+    // 64 requests under one of 1000, one token, 48.6, cut 57 (with the launches).
     a.grid = std::min(a.grid, MAX_ITEMS);
+    a.whole = S::WIN ? uncut<S>(a, max_new) : (int64_t)a.max_blocks << a.c.bs_log2 <= 6 * std::max(S::KU, 64);
     hipLaunchKernelGGL(attn_kernel<S>, dim3(a.grid), dim3(64 * S::WAVES), S::LDS, st, a);
     if (!a.whole) hipLaunchKernelGGL((attn_join<S::D, S::RT>), dim3(JOIN_WGS * cus), dim3(256), 0, st, a);
     return hipGetLastError();
@@ -793,16 +796,16 @@ hipError_t rows(const AttnArgs& a, int max_new, int cus, uint8_t* ws, hipStream_
     // 19.5, <2, 1, 4, 2, 1> 15.0.
     const int64_t r = (int64_t)max_new * a.G;
     if constexpr (D == 256) {
-        if (r <= 16) return go<Shape<BF16, WIN, D, 1, 1, 2, 2, 1>>(a, cus, ws, st);
-        return go<Shape<BF16, WIN, D, 1, 4, 1, 4, 1>>(a, cus, ws, st);
+        if (r <= 16) return go<Shape<BF16, WIN, D, 1, 1, 2, 2, 1>>(a, max_new, cus, ws, st);
+        return go<Shape<BF16, WIN, D, 1, 4, 1, 4, 1>>(a, max_new, cus, ws, st);
     } else {
-        if (r <= 16) return go<Shape<BF16, WIN, D, 1, 1, 2, 2, 2>>(a, cus, ws, st);
+        if (r <= 16) return go<Shape<BF16, WIN, D, 1, 1, 2, 2, 2>>(a, max_new, cus, ws, st);
         if constexpr (D == 64) {
-            if (r <= 32) return go<Shape<BF16, WIN, D, 1, 2, 2, 4, 2>>(a, cus, ws, st);
+            if (r <= 32) return go<Shape<BF16, WIN, D, 1, 2, 2, 4, 2>>(a, max_new, cus, ws, st);
         } else {
-            if (r <= 32) return go<Shape<BF16, WIN, D, 2, 1, 2, 2, 2>>(a, cus, ws, st);
+            if (r <= 32) return go<Shape<BF16, WIN, D, 2, 1, 2, 2, 2>>(a, max_new, cus, ws, st);
         }
-        return go<Shape<BF16, WIN, D, 1, 4, 1, 3, 3>>(a, cus, ws, st);
+        return go<Shape<BF16, WIN, D, 1, 4, 1, 3, 3>>(a, max_new, cus, ws, st);
     }
 }
 

@@ -12,8 +12,6 @@
 // Values: O = sum p s_v c.  Codes become fp16 (exactly: a byte beside 0x64 is 1024 and itself) and
 // p s_v two fp16 parts as in fq_attn.hip.  The references are of the scores plus log2 s_v, so that
 // p s_v stays in fp16's range whatever the groups' scales; the sums are of p.
-#include <type_traits>
-
 #include "fq_attn.h"
 #include "fq_group8.h"
 
@@ -34,11 +32,6 @@ constexpr float LAG = 4.0f;
 constexpr float UP = 2048.0f;
 constexpr float MOST = 8355711.0f;  // 127 (1 + 256 + 65536): the largest that three signed bytes hold
 constexpr int LIMBS = 3;
-
-// a / b, in 32 bits where that does (a 64-bit division takes a third of a microsecond).
-__device__ __forceinline__ int64_t divided(int64_t a, int64_t b) {
-    return (uint64_t)(a | b) >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
-}
 
 // The largest of three.  (Written out: the compiler makes numbers that may be signalling NaN quiet first.)
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -342,7 +335,7 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
                 const bool on = t < nt;
                 // (a chain: how many of the new tokens the row sees)
                 mask[c] = !on ? 0 : a.masks ? a.masks[t0 + t] : (uint64_t)t + 1;
-                from[c] = 0;
+                from[c] = 0x7FFFFFFF;
                 if (on) {
                     const Reach reached = reach(a, len, t, mask[c]);
                     mask[c] = reached.mask, from[c] = reached.from;
@@ -711,33 +704,6 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
     if (!cut && tid == 0) a.desc[wg] = 0;
 }
 
-// The most keys that an item walks, by the table's columns and the window.  (A request may have more new
-// tokens than it was said: its items only take longer.)
-template <class S>
-int64_t most_keys(const AttnArgs& a, int max_new) {
-    const int64_t keys = (int64_t)a.max_blocks << a.c.bs_log2;
-    if (!a.window) return keys;
-    return std::min<int64_t>(keys, (int64_t)a.window + max_new + (a.sinks ? S::KU + std::min<int64_t>(a.sinks, keys) : 0));
-}
-
-// Whether items are left whole, so that nothing is to be joined: where they have 6 units at most, by
-// the table's columns and the window, and up to 12, or any number under a window, where they take no longer one
-// after the other on the work-groups than cut into even shares, with the begin of a second part and the
-// second launch (about JOIN units).  Without a window the longest item counts against three
-// quarters of it on average.  D = 128, 8 x 4 heads, one token, us: 64 requests of 760 keys 21.6, cut 30;
-// 64 of 20001 under a window of 1023 37, cut 46 + 8; one of 630 13.1, cut 14.5.
-template <class S>
-bool uncut(const AttnArgs& a, int max_new) {
-    constexpr int JOIN = 2 + 256 / S::KU, MOST_UNITS = 12;
-    const int64_t keys = most_keys<S>(a, max_new);
-    if (keys <= 6 * std::max(S::KU, 64)) return true;
-    if (!a.window && keys > MOST_UNITS * S::KU) return false;
-    const int64_t units = keys / S::KU + 2, even = a.window ? units : units * 3 / 4;
-    const int64_t items = (int64_t)a.B * a.hkv * (((int64_t)max_new * a.G + S::RT - 1) / S::RT);
-    const int64_t turns = (items + a.grid - 1) / a.grid;
-    return turns * (units + S::OV) <= items * (even + 2 * S::OV) / a.grid + JOIN;
-}
-
 template <class S>
 hipError_t go(AttnArgs a, int max_new, int cus, uint8_t* ws, hipStream_t st) {
     a.grid = std::min(S::PC * cus, MAX_ITEMS);
@@ -752,7 +718,7 @@ hipError_t go(AttnArgs a, int max_new, int cus, uint8_t* ws, hipStream_t st) {
 template <int D>
 hipError_t rows(const AttnArgs& a, int max_new, int cus, uint8_t* ws, hipStream_t st) {
     const int64_t r = (int64_t)max_new * a.G;
-    using Few = std::conditional_t<D == 256, Shape<D, 1, 1, 2, 2, 2>, Shape<D, 1, 1, 4, 2, 2>>;
+    using Few = Shape<D, 1, 1, 4, 2, D == 256 ? 1 : 2>;
     const int64_t tiles = (int64_t)a.B * a.hkv * ((r + 15) / 16), units = most_keys<Few>(a, max_new) / Few::KU + 1;
     if (r <= 32 || tiles * units <= 16 * (int64_t)Few::PC * cus) return go<Few>(a, max_new, cus, ws, st);
     if constexpr (D == 256) {
