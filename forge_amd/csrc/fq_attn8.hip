@@ -11,7 +11,8 @@
 //
 // Values: O = sum p s_v c.  Codes become fp16 (exactly: a byte beside 0x64 is 1024 and itself) and
 // p s_v two fp16 parts as in fq_attn.hip.  The references are of the scores plus log2 s_v, so that
-// p s_v stays in fp16's range whatever the groups' scales; the sums are of p.
+// p s_v stays in fp16's range whatever the groups' scales; the sums are of p.  (Where s_v is below
+// 2^-80 the parts lose bits: an element is then off by up to 2^-109.)
 #include "fq_attn.h"
 #include "fq_group8.h"
 
@@ -30,6 +31,10 @@ constexpr int SUBS = KT / GROUP;
 // parts are raised by: together they stay below fp16's largest.
 constexpr float LAG = 4.0f;
 constexpr float UP = 2048.0f;
+// The references lie this much (log2) below that sum, and this far below the scores at most, so that p has
+// room on both sides: for scales up to 2^121 (of the largest values) above, for groups of zeros below.
+constexpr float BELOW = 20.0f, MOST_BELOW = -100.0f;
+constexpr float UP_SCALE = UP / 1048576.0f;  // UP 2^-BELOW
 constexpr float MOST = 8355711.0f;  // 127 (1 + 256 + 65536): the largest that three signed bytes hold
 constexpr int LIMBS = 3;
 
@@ -500,7 +505,7 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
                     const float sk = held_scale(__uint_as_float(ts[sub]));
                     sv[sub] = held_scale(__uint_as_float(ts[SUBS + sub]));
                     // (any number near log2 sv; a group of zeros still has its part in the sums)
-                    lift[sub] = fmaxf(__builtin_amdgcn_logf(sv[sub]), -80.0f);
+                    lift[sub] = fmaxf(__builtin_amdgcn_logf(sv[sub]) - BELOW, MOST_BELOW);
 #pragma unroll
                     for (int c = 0; c < NR; ++c) mul[sub][c] = rs[c] * sk;
                 }
@@ -552,7 +557,7 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
                     for (int r = 0; r < 4; ++r) {
                         p[r] = __builtin_amdgcn_exp2f(fmaf(sc[sub][c][r], mul[sub][c], -mrow[c]));
                         sum[c] += p[r];
-                        p[r] *= UP * sv[sub];
+                        p[r] *= UP_SCALE * sv[sub];
                     }
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
@@ -651,7 +656,7 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
 #pragma unroll
                 for (int w = 0; w < WK; ++w)
                     lsum[c] += s_ml[1][w][rl] * __builtin_amdgcn_exp2f(s_ml[0][w][rl] - m);
-                const float f = __builtin_amdgcn_exp2f(mrow[c] - m) * (1.0f / UP);
+                const float f = __builtin_amdgcn_exp2f(mrow[c] - m) * (1.0f / UP_SCALE);
                 mrow[c] = m;
 #pragma unroll
                 for (int d = 0; d < DT; ++d) {

@@ -51,7 +51,8 @@
  *
  * fq_tree_attention, fq_window_attention, fq_token_logprobs and fq_verify_draft keep partial results in the
  * library's per-stream workspace; fq_reserve_step sizes it for calls under
- * HIP-graph capture (fq_release_workspace frees it).
+ * HIP-graph capture (fq_release_workspace frees it).  A graph uses the workspace of the stream
+ * that it was captured on: such graphs and that stream's calls run one after the other.
  */
 #ifndef FORGE_STEP_H
 #define FORGE_STEP_H
