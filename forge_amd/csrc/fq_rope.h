@@ -89,7 +89,7 @@ __device__ __forceinline__ HeadRuns head_runs(const RopeArgs& a, int n, int h, i
                 if (INTER) {  // pairs (0, 1) (2, 3) of y0, then of y1
                     const f4 y = i < 2 ? y0 : y1;
                     const float u = y[2 * (i & 1)], v = y[2 * (i & 1) + 1];
-                    const float t0 = u * c[i] - v * s[i], t1 = v * c[i] + u * s[i];
+                    const float t0 = fmaf(u, c[i], -(v * s[i])), t1 = fmaf(u, s[i], v * c[i]);
                     if (i < 2) {
                         x0[2 * i] = t0, x0[2 * i + 1] = t1;
                     } else {
