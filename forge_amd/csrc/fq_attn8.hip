@@ -12,7 +12,20 @@
 // Values: O = sum p s_v c.  Codes become fp16 (exactly: a byte beside 0x64 is 1024 and itself) and
 // p s_v two fp16 parts as in fq_attn.hip.  The references are of the scores plus log2 s_v, so that
 // p s_v stays in fp16's range whatever the groups' scales; the sums are of p.  (Where s_v is below
-// 2^-80 the parts lose bits: an element is then off by up to 2^-109.)
+// 2^-80 the parts lose bits: an element is then off by up to 2^-109.)  The transposing read gives a lane
+// its column's 8 keys; it is asked for a tile ahead of its use.
+//
+// Bound: for one token a request the bytes of codes, half of those of 16 bits, and what a tile costs to
+// begin; with more rows the vector instructions beside the matrix ones: 16 codes become fp16 with 20 (of
+// 32 keys x 128 columns for each 32 rows), a score its probability's parts with ten.  Kernel + join, us, D = 128:
+// 48 requests of up to 5001 keys, one token, 4 kv heads x 7 (184 MB) 44 + 5.4; one of 131000, 13 tokens, 4 x 7
+// (135 MB, matrix work 37) 81 + 10; 32 of up to 8190, 1 to 32 tokens, 8 x 4 (410 MB at least,
+// 634 asked for; matrix work 79) 175 + 15; 64 of up to 20001 under a window of 1023, 8 x 4 (135 MB),
+// items whole, 38; one of 333 keys 9.  There vector instructions are issued in 52 % of the cycles,
+// matrix ones busy in 25 %, and a wave waits for 34 % of its time.  Steps (131000 keys / full batch):
+// one wave's tiles without copies ahead 73500 / 13964; copies to LDS with the scales among them, eight waves
+// a CU 107 / 219; values read a tile ahead, conversions between the matrix instructions 94 / 186; waves
+// of 32 rows on their own, four work-groups a CU 80 / 175.
 #include "fq_attn.h"
 #include "fq_group8.h"
 
@@ -722,6 +735,25 @@ hipError_t go(AttnArgs a, int max_new, int cus, uint8_t* ws, hipStream_t st) {
 
 template <int D>
 hipError_t rows(const AttnArgs& a, int max_new, int cus, uint8_t* ws, hipStream_t st) {
+    // By the rows of an item.  Up to 32, and wherever there are too few tiles of rows and keys to fill
+    // the work-groups: waves of 16 rows with keys of their own, four groups of keys side by side, which share
+    // a short item's units best.  More rows: waves of 32, so that codes are converted half as often, then two
+    // that share a tile.  D = 256: 16 rows, whose sums fill the registers.  With the launches, us, the shape taken
+    // first:
+    //   D = 128, 8 kv heads x 4       <1, 1, 4, 2, 2>  <2, 1, 2, 2, 4>  <2, 2, 2, 3, 2>
+    //   32 x 8190 keys, 16 rows             90.0            101              118
+    //   16 x 4090, 32 rows                  40.7             46.3             53.0
+    //   32 x 8190, 28 rows                 108              106              123
+    //   the same, 48 rows                  139              118              128
+    //   8 x 8190, 256 rows                 145              105               95.4
+    //   32 x 8190, 160 rows                352              219              211
+    //   D = 64, 16 x 8000, 32 rows          29.1             34.9             39.7
+    //   the same, 96 rows                   42.9             42.2             50.0
+    //   8 trees of 25 over 760 keys, 4 x 7 (175 rows, few tiles): 16.5, by rows alone 32
+    //   D = 256, 16 x 8000, 2 x 5     <1, 1, 4, 2, 1>  <1, 1, 2, 2, 2>  <1, 2, 1, 3, 2>
+    //   5 rows                              34.5             36.0             43.0
+    //   30 rows                             44.0             42.4             45.8
+    //   80 rows                             72.7             63.6             60.6
     const int64_t r = (int64_t)max_new * a.G;
     using Few = Shape<D, 1, 1, 4, 2, D == 256 ? 1 : 2>;
     const int64_t tiles = (int64_t)a.B * a.hkv * ((r + 15) / 16), units = most_keys<Few>(a, max_new) / Few::KU + 1;

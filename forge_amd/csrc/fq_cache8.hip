@@ -45,7 +45,8 @@ __device__ __forceinline__ void store16(void* out, int64_t at, u4 w, float s) {
 constexpr int ROWS = 16;  // of a work-group at most
 
 // Rows of keys and values, a lane 16 codes at a time.  Bound by the bytes, one in, two or four
-// out, and for few rows by three loads one behind the other (requests, table, codes).
+// out, and for few rows by three loads one behind the other (requests, table, codes).  3946 tokens, 8 heads
+// of 128 to fp16 (25 MB): 8.6 us; four pieces of 16 codes a lane are on their way at a time.  42 tokens 3.9.
 template <int TYPE>
 __global__ __launch_bounds__(256) void read_kernel(ReadArgs a, int most) {
     __shared__ int s_slot[ROWS], s_request[ROWS];
@@ -108,7 +109,8 @@ __global__ __launch_bounds__(256) void read_kernel(ReadArgs a, int most) {
 constexpr int MOST = 64;  // accepted tokens that move
 
 // One request's accepted tokens, one kv head's keys or values: all that move are in LDS before
-// any is written.  A handful of tokens: bound by latency (path, table, rows).
+// any is written.  A handful of tokens: bound by latency (path, table, rows).  7 trees of up to 25 tokens, 4 heads of
+// 128, 16 bits: 3.4 us; 96 of up to 48, 8 heads, 8 bits: 9.6.
 template <bool CODES>
 __global__ __launch_bounds__(256) void keep_kernel(KeepArgs a) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];

@@ -11,7 +11,10 @@
 // whole sum first, another launch sums what is left.  Pick: the chunk in which the sum passes the random number, then
 // the token in it.
 //
-// Bound: the bytes of the logits, read once; a row of each request is read again.
+// Bound: the bytes of the logits, read once; a row of each request is read again.  32 trees of up to 25 tokens,
+// 152064 fp32 logits (400 rows, 243 MB): 44 us for the statistics, 5.6 TB/s, 14 for the walk, 8 for the pick.  One
+// chain of 6 x 32000 with draft probabilities: 3.6, 7.7, 5.8 and 7.4, each a launch's latency and loads that follow
+// one another.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
