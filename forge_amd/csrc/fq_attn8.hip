@@ -13,19 +13,20 @@
 // p s_v two fp16 parts as in fq_attn.hip.  The references are of the scores plus log2 s_v, so that
 // p s_v stays in fp16's range whatever the groups' scales; the sums are of p.  (Where s_v is below
 // 2^-80 the parts lose bits: an element is then off by up to 2^-109.)  The transposing read gives a lane
-// its column's 8 keys; it is asked for a tile ahead of its use.
+// its column's 8 keys; it is asked for before the softmax.
 //
 // Bound: for one token a request the bytes of codes, half of those of 16 bits, and what a tile costs to
 // begin; with more rows the vector instructions beside the matrix ones: 16 codes become fp16 with 20 (of
-// 32 keys x 128 columns for each 32 rows), a score its probability's parts with ten.  Kernel + join, us, D = 128:
+// 32 keys x 128 columns for each 32 rows), a score its probability's parts with thirteen.  Kernel + join, us, D = 128:
 // 48 requests of up to 5001 keys, one token, 4 kv heads x 7 (184 MB) 44 + 5.4; one of 131000, 13 tokens, 4 x 7
-// (135 MB, matrix work 37) 81 + 10; 32 of up to 8190, 1 to 32 tokens, 8 x 4 (410 MB at least,
-// 634 asked for; matrix work 79) 175 + 15; 64 of up to 20001 under a window of 1023, 8 x 4 (135 MB),
-// items whole, 38; one of 333 keys 9.  There vector instructions are issued in 52 % of the cycles,
-// matrix ones busy in 25 %, and a wave waits for 34 % of its time.  Steps (131000 keys / full batch):
+// (135 MB, matrix work 37) 78 + 10; 32 of up to 8190, 1 to 32 tokens, 8 x 4 (410 MB at least,
+// 1160 asked of the L2s, 525 of memory; matrix work 79) 169 + 15; 64 of up to 20001 under a window of 1023, 8 x 4 (135 MB),
+// items whole, 38; one of 333 keys 9.  There vector instructions are issued in 55 % of the cycles,
+// matrix units busy in 28 %, with two waves a SIMD.  Steps (131000 keys / full batch):
 // one wave's tiles without copies ahead 73500 / 13964; copies to LDS with the scales among them, eight waves
-// a CU 107 / 219; values read a tile ahead, conversions between the matrix instructions 94 / 186; waves
-// of 32 rows on their own, four work-groups a CU 80 / 175.
+// a CU 107 / 219; values asked for before the softmax, conversions between the matrix instructions 94 / 186; waves
+// of 32 rows on their own, four work-groups a CU 80 / 175; the next scores' conversion held there (the
+// compiler moved it behind) 78 / 169.
 #include "fq_attn.h"
 #include "fq_group8.h"
 
@@ -628,7 +629,9 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
 #pragma unroll
                         for (int e = s0 + m * (s1 - s0) / RUN; e < s0 + (m + 1) * (s1 - s0) / RUN; ++e) {
                             const int sub = e / 4 / NR, k = e / 4 % NR, r = e % 4;
-                            sc[sub][k][r] = (float)((high[sub][k][r] << 8) + low[sub][k][r]);
+                            float next = (float)((high[sub][k][r] << 8) + low[sub][k][r]);
+                            asm volatile("" : "+v"(next));  // (here, and not behind the matrix instructions)
+                            sc[sub][k][r] = next;
                         }
                         __builtin_amdgcn_sched_barrier(0);
                     }
