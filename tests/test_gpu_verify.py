@@ -291,6 +291,77 @@ def test_a_sampled_step_on_another_stream_and_in_a_graph(window):
             assert torch.equal(a, b), r
 
 
+def test_steps_on_two_streams_at_once():
+    states = [state_of(1, None), state_of(2, None)]
+    want = [[t.clone() for t in step_of([t.clone() for t in s], w)] for s, w in zip(states, (None, 128))]
+    copies = [[[t.clone() for t in s] for s in states] for _ in range(6)]
+    sides = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for c in copies:
+        for i, w in enumerate((None, 128)):
+            with torch.cuda.stream(sides[i]):
+                got[i].append(step_of(c[i], w))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for g in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(want[i], g))
+
+
+def test_graphs_of_two_streams_at_once():
+    states, sides, graphs, kept = [state_of(1, None), state_of(2, None)], [torch.cuda.Stream(), torch.cuda.Stream()], [], []
+    want = [[t.clone() for t in step_of([t.clone() for t in s], w)] for s, w in zip(states, (None, 128))]
+    for s, side, w in zip(states, sides, (None, 128)):
+        with torch.cuda.stream(side):
+            step.reserve()
+        torch.cuda.synchronize()
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=side):
+            kept.append(step_of(s, w))
+    fresh = [[t.clone() for t in s] for s in (state_of(1, None), state_of(2, None))]
+    for _ in range(4):
+        for s, f in zip(states, fresh):
+            for a, b in zip(s, f):
+                a.copy_(b)
+        torch.cuda.synchronize()
+        for g, side in zip(graphs, sides):
+            with torch.cuda.stream(side):
+                g.replay()
+        torch.cuda.synchronize()
+        for k, x in zip(kept, want):
+            assert all(torch.equal(a, b) for a, b in zip(k, x))
+
+
+def test_a_padded_step():
+    # buffers longer than the step: rows behind the last request change nothing and come out empty
+    state = state_of(3, None)
+    lengths, new, table, free, parents, x, rope, kc, ks, vc, vs, logits, tokens, u = state
+    want = [t.clone() for t in step_of([t.clone() for t in state], 128)]
+    N, more = x.shape[0], 5
+
+    def longer(t, value):
+        return torch.cat([t, torch.full((more, *t.shape[1:]), value, dtype=t.dtype, device="cuda")])
+
+    padded = [lengths, new, table, free, longer(parents, -1), longer(x, math.nan), rope, kc, ks, vc, vs,
+              longer(logits, math.nan), longer(tokens, 7), longer(u, 0.5)]
+    o, accepted, path, following, k, v = step_of(padded, 128)
+    for a, b in zip((o[:N], accepted, path[:N], following, k[:N], v[:N]), want):
+        assert torch.equal(a, b)
+    assert not o[N:].any() and bool((path[N:] == -1).all()) and not k[N:].any() and not v[N:].any()
+
+
+def test_no_tokens_at_all():
+    k, v = step.paged_cache(4, 16, 2, 64, torch.int8)
+    table, none, cu = ints([[0, 1], [2, 3]]), ints([]), ints([0, 0, 0])
+    q = step.qk_norm_rope(torch.zeros((0, 8 * 64), device="cuda"), none, none, step.rope_table(8, 64), k, v)
+    assert tuple(q.shape) == (0, 4, 64)
+    for window in (None, 8):
+        assert step.tree_attention(q, k, v, table, ints([5, 0]), cu, window=window).numel() == 0
+    step.keep_accepted(k, v, table, ints([5, 0]), cu, none, ints([0, 0]))
+    kk, vv = step.read_cache(k, v, table, cu, 0)
+    assert kk.numel() == 0 and vv.numel() == 0
+
+
 def test_capture_without_a_workspace_is_refused():
     from forge_amd import _lib
     side = torch.cuda.Stream()
