@@ -18,9 +18,9 @@
 // Bound: for one token a request the bytes of codes, half of those of 16 bits, and what a tile costs to
 // begin; with more rows the vector instructions beside the matrix ones: 16 codes become fp16 with 20 (of
 // 32 keys x 128 columns for each 32 rows), a score its probability's parts with thirteen.  Kernel + join, us, D = 128:
-// 48 requests of up to 5001 keys, one token, 4 kv heads x 7 (184 MB) 44 + 5.4; one of 131000, 13 tokens, 4 x 7
-// (135 MB, matrix work 37) 78 + 10; 32 of up to 8190, 1 to 32 tokens, 8 x 4 (410 MB at least,
-// 1160 asked of the L2s, 525 of memory; matrix work 79) 169 + 15; 64 of up to 20001 under a window of 1023, 8 x 4 (135 MB),
+// 48 requests of up to 5001 keys, one token, 4 kv heads x 7 (184 MB) 45 + 5.4; one of 131000, 13 tokens, 4 x 7
+// (135 MB, matrix work 37) 80 + 10; 32 of up to 8190, 1 to 32 tokens, 8 x 4 (410 MB at least,
+// 1160 asked of the L2s, 525 of memory; matrix work 79) 171 + 15; 64 of up to 20001 under a window of 1023, 8 x 4 (135 MB),
 // items whole, 38; one of 333 keys 9.  There vector instructions are issued in 55 % of the cycles,
 // matrix units busy in 28 %, with two waves a SIMD.  Steps (131000 keys / full batch):
 // one wave's tiles without copies ahead 73500 / 13964; copies to LDS with the scales among them, eight waves
@@ -45,10 +45,12 @@ constexpr int SUBS = KT / GROUP;
 // parts are raised by: together they stay below fp16's largest.
 constexpr float LAG = 4.0f;
 constexpr float UP = 2048.0f;
-// The references lie this much (log2) below that sum, and this far below the scores at most, so that p has
-// room on both sides: for scales up to 2^121 (of the largest values) above, for groups of zeros below.
-constexpr float BELOW = 20.0f, MOST_BELOW = -100.0f;
-constexpr float UP_SCALE = UP / 1048576.0f;  // UP 2^-BELOW
+// The references are MOST_BELOW under the scores at most (groups of zeros have their part in the sums).
+// From the first scale above LARGE on they are BELOW lower (log2), and p that much larger, so that p does not
+// vanish at scales up to 2^121, those of the largest values.  (Not from the start: exponents of small
+// magnitude are rounded less; 333 keys 4.9e-7 off, else 5.5e-7.)
+constexpr float MOST_BELOW = -80.0f, LARGE = 1.152921504606846976e18f;  // 2^60
+constexpr float BELOW = 20.0f, BELOW_TIMES = 1048576.0f;
 constexpr float MOST = 8355711.0f;  // 127 (1 + 256 + 65536): the largest that three signed bytes hold
 constexpr int LIMBS = 3;
 
@@ -409,6 +411,7 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
             const bool busy = WR == 1 || rt * RT + wr * 16 * NR < nt * a.G;
             f4 o[DT][NR];
             float mrow[NR], lrow[NR];
+            float below = 0.0f, up_by = UP;  // (o is in units of up_by, whichever that is)
 #pragma unroll
             for (int c = 0; c < NR; ++c) {
                 mrow[c] = LOWEST;
@@ -519,10 +522,18 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
                     const float sk = held_scale(__uint_as_float(ts[sub]));
                     sv[sub] = held_scale(__uint_as_float(ts[SUBS + sub]));
                     // (any number near log2 sv; a group of zeros still has its part in the sums)
-                    lift[sub] = fmaxf(__builtin_amdgcn_logf(sv[sub]) - BELOW, MOST_BELOW);
+                    lift[sub] = fmaxf(__builtin_amdgcn_logf(sv[sub]), MOST_BELOW);
 #pragma unroll
                     for (int c = 0; c < NR; ++c) mul[sub][c] = rs[c] * sk;
                 }
+                if (__any(fmaxf(sv[0], sv[1]) > LARGE) && below == 0.0f) {
+                    below = BELOW;
+                    up_by = UP / BELOW_TIMES;
+#pragma unroll
+                    for (int c = 0; c < NR; ++c) mrow[c] -= BELOW, lrow[c] *= BELOW_TIMES;
+                }
+#pragma unroll
+                for (int sub = 0; sub < SUBS; ++sub) lift[sub] -= below;
                 if (tail) {
                     const int old = len - key0, all = keys - key0;
                     const uint32_t in = holes ? there(i) : ~0u;
@@ -571,7 +582,7 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
                     for (int r = 0; r < 4; ++r) {
                         p[r] = __builtin_amdgcn_exp2f(fmaf(sc[sub][c][r], mul[sub][c], -mrow[c]));
                         sum[c] += p[r];
-                        p[r] *= UP_SCALE * sv[sub];
+                        p[r] *= up_by * sv[sub];
                     }
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
@@ -672,7 +683,7 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
 #pragma unroll
                 for (int w = 0; w < WK; ++w)
                     lsum[c] += s_ml[1][w][rl] * __builtin_amdgcn_exp2f(s_ml[0][w][rl] - m);
-                const float f = __builtin_amdgcn_exp2f(mrow[c] - m) * (1.0f / UP_SCALE);
+                const float f = __builtin_amdgcn_exp2f(mrow[c] - m) * (1.0f / up_by);
                 mrow[c] = m;
 #pragma unroll
                 for (int d = 0; d < DT; ++d) {

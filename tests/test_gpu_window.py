@@ -286,6 +286,25 @@ def test_codes_values_of_any_size(log, D, new):
     c.check(window=300, sinks=4)
 
 
+@pytest.mark.parametrize("log", [61, 90, 118])
+@pytest.mark.parametrize("hq, D, new", [(4, 64, 64), (4, 128, 64), (1, 128, 33), (4, 256, 50)])
+def test_codes_large_values_behind_small_ones(log, hq, D, new):
+    # rows that see small ones alone keep their bits, before and after the first large one
+    c = Case([0], [new], hq, 1, D, tree=True, seed=25)
+    pages = c.table[0, :-(-new // 16)].tolist()
+    for i, p in enumerate(pages):
+        c.caches[1].scales[p] = 2.0 ** (log if i == 2 else -6)
+    c.masks = torch.tensor([1 << i if i < 63 else -2 ** 63 for i in range(new)], dtype=torch.int64)  # each its own key alone
+    out, v = c.run(max_new=new).double().cpu(), c.values()[1]
+    for i in range(new):
+        want = v[pages[i // 16], i % 16, 0]
+        assert float((out[i] - want).abs().max()) <= 40 * U * float(want.abs().max())
+    c = Case([100 * 16], [3], hq, 1, D, seed=26)
+    for i in (0, 55, 99):  # (what is small vanishes beside it)
+        c.caches[1].scales[int(c.table[0, i])] = 2.0 ** log
+        c.check()
+
+
 def test_codes_scores_far_apart():
     for at in (0, 35, 199, 203):
         c = Case([200], [4], 4, 1, 64, seed=15)
