@@ -39,7 +39,8 @@ __device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)"
 
 // What a request brings.
 struct Request {
-    int t0, nt, len;  // its first new token, how many, its cached tokens
+    int t0, nt, len;  // its first new token, how many, its cached tokens (of those the table can hold)
+    int pos;          // its first new token's position
     int keys, nu;     // keys and units of them that are walked
     int su, skip;     // with a window: units that hold the sinks, units left out behind them
     int rts;          // tiles of RT rows
@@ -55,13 +56,15 @@ __device__ __forceinline__ Request request(const AttnArgs& a, int c0, int c1, in
     const int64_t most = (int64_t)a.max_blocks << a.c.bs_log2;
     r.keys = (int)min((int64_t)max(len, 0) + r.nt, min(most, (int64_t)INT32_MAX - 4096));
     r.len = min(max(len, 0), r.keys);
+    r.pos = max(len, 0);
     r.nu = (r.keys + KU - 1) / KU;
     r.su = r.skip = 0;
     if constexpr (WIN) {
-        // No new token lies before position len, so none sees a cached one before this, but for sinks.
-        const int from = a.window ? max(r.len + 1 - a.window, 0) : 0;
+        // No new token lies before position pos, so none sees a cached one before this, but for sinks.
+        // (Which may be behind all keys there are: a unit stays, masked, so that zeros are written.)
+        const int from = a.window ? max(r.pos - a.window + 1, 0) : 0;
         r.su = (min(a.sinks, r.keys) + KU - 1) / KU;
-        r.skip = max(from / KU - r.su, 0);
+        r.skip = max(min(from / KU - r.su, r.nu - max(r.su, 1)), 0);
         r.nu -= r.skip;
     }
     r.rts = (int)(((int64_t)r.nt * a.G + RT - 1) / RT);
@@ -107,20 +110,21 @@ __device__ __forceinline__ uint32_t shifted(uint64_t m, int n) {
 }
 
 // What a row of a call with a window sees of the context: the sinks and from `from` on; and a
-// draft's bits without those the window has left.  t: its number among the new tokens.
+// draft's bits without those the window has left.  pos: the request's first new token's position, t: the
+// row's number among the new tokens.
 struct Reach {
     int from;
     uint64_t mask;
 };
-__device__ __forceinline__ Reach reach(const AttnArgs& a, int len, int t, uint64_t mask) {
+__device__ __forceinline__ Reach reach(const AttnArgs& a, int pos, int t, uint64_t mask) {
     const int depth = a.masks ? max(__builtin_popcountll(mask) - 1, 0) : t;
-    Reach r{a.window ? (int)min(max((int64_t)len + depth + 1 - a.window, (int64_t)0), (int64_t)INT32_MAX) : 0, mask};
+    Reach r{a.window ? (int)min(max((int64_t)pos + depth + 1 - a.window, (int64_t)0), (int64_t)INT32_MAX) : 0, mask};
     if (a.masks && a.window && depth >= a.window) {
-        // a bit's position is len and how many are below it
+        // a bit's position is pos and how many are below it
         uint64_t rest = mask;
         r.mask = 0;
         for (int at = 0; rest; rest &= rest - 1, ++at)
-            if (depth - at < a.window || len + at < a.sinks) r.mask |= rest & -rest;
+            if (depth - at < a.window || (int64_t)pos + at < a.sinks) r.mask |= rest & -rest;
     }
     return r;
 }

@@ -258,7 +258,7 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
             const uint8_t* vb = a.v + (int64_t)h * a.c.sh * 2;
             const int* table = a.table + b * a.table_stride;
             // The first key that all of the item's rows see, and all from there on to the context's end.
-            const int clear = WIN && a.window ? (int)min((int64_t)len + (a.masks ? 63 : min(nt - 1, (rt * RT + RT - 1) / a.G)) + 1 - a.window,
+            const int clear = WIN && a.window ? (int)min((int64_t)rq.pos + (a.masks ? 63 : min(nt - 1, (rt * RT + RT - 1) / a.G)) + 1 - a.window,
                                                          (int64_t)INT32_MAX) : 0;
             // A tile's pages, read ahead; the places of its 16s of keys in a cache;
             // its copies.  (Past the last key: its page again.)
@@ -369,7 +369,7 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
                 mask[c] = !on ? 0 : a.masks ? a.masks[t0 + t] : (uint64_t)t + 1;
                 from[c] = 0x7FFFFFFF;  // (a row of nobody's sees none of what the others do not)
                 if (WIN && on) {
-                    const Reach r = reach(a, len, t, mask[c]);
+                    const Reach r = reach(a, rq.pos, t, mask[c]);
                     mask[c] = r.mask, from[c] = r.from;
                 }
                 const float* q = a.q + (int64_t)(t0 + (on ? t : 0)) * a.ldq + (int64_t)(on ? hh : 0) * D;

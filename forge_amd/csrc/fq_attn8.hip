@@ -248,7 +248,7 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
             const uint8_t* vb = a.v + (int64_t)h * a.c.sh;
             const int* table = a.table + b * a.table_stride;
             // The first key that all of the item's rows see, and all from there on to the context's end.
-            const int clear = a.window ? (int)min((int64_t)len + (a.masks ? 63 : min(nt - 1, (rt * RT + RT - 1) / a.G)) + 1 - a.window,
+            const int clear = a.window ? (int)min((int64_t)rq.pos + (a.masks ? 63 : min(nt - 1, (rt * RT + RT - 1) / a.G)) + 1 - a.window,
                                                   (int64_t)INT32_MAX) : 0;
             // A tile's pages, read ahead; where its two groups lie in a cache, and their scales; its
             // copies.  (Past the last tile: it again.)  In blocks of 32 tokens and more both are in one.
@@ -358,7 +358,7 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
                 mask[c] = !on ? 0 : a.masks ? a.masks[t0 + t] : (uint64_t)t + 1;
                 from[c] = 0x7FFFFFFF;
                 if (on) {
-                    const Reach reached = reach(a, len, t, mask[c]);
+                    const Reach reached = reach(a, rq.pos, t, mask[c]);
                     mask[c] = reached.mask, from[c] = reached.from;
                 }
                 const float* q = a.q + (int64_t)(t0 + (on ? t : 0)) * a.ldq + (int64_t)(on ? hh : 0) * D;
