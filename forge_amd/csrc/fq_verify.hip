@@ -3,8 +3,11 @@
 // Three or four launches.  Statistics: every row's largest logit m and s = sum e^((x - m) / T)
 // (at temperatures of 0 or below its first largest), one pass over the logits in 32 bits, rows cut into parts
 // where there are few.  Walk: what is accepted.  Whether a token is, were it tried, depends on
-// its earlier siblings alone: u (1 - sum of their p) < p, so that all tests are made at
-// once, a lane a token, and the walk goes over bits.  The same launch sums e^((x - m) / T) of
+// its earlier siblings alone: u (s - sum of their e) < e, e = e^((x - m) / T) of the token's logit, so that all
+// tests are made at once, a lane a token, and the walk goes over bits.  s is the statistics', in 32 bits:
+// a test on the walk's way whose two sides are nearer to each other than s is exact is made again with
+// the row's sum in 64 bits (one in 2^14 or so at 152064 tokens, at random numbers; one wave
+// sums them alone).  The same launch sums e of
 // each request's last accepted row, without the refused tokens, over chunks in 64 bits (a random number within
 // 1e-7 of a border of the cumulated sum would find another token in 32: at 150000
 // tokens one number in a hundred).  With draft probabilities, whose subtraction needs the
@@ -35,6 +38,8 @@ constexpr int STEP = 256 * E;     // of a work-group
 constexpr int MAX_STATS = 1 << 20;
 constexpr int MAX_SUMS = 1 << 18;  // chunks of all requests
 constexpr int LANES = 64;          // tokens of a request whose parents count
+// Temperatures between which the statistics' exponents, in 32 bits, neither overflow nor lose bits: 2^-100, 2^100.
+constexpr float FAR_LOW = 7.8886091e-31f, FAR_HIGH = 1.2676506e30f;
 
 struct Stat {
     float m, s;  // s: NaN for a row with NaN or +inf, 0 for one of -inf alone; > 0 otherwise
@@ -55,6 +60,7 @@ struct Space {
     Left* left;
     double *whole, *rest;  // [B][chunks]
     int chunks, chunk;
+    float unsure;  // what part of itself a row's sum of the statistics is off by at most
 };
 
 __device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
@@ -217,6 +223,24 @@ __device__ __forceinline__ Stat joined(const VerifyArgs& a, const Space& w, int 
 }
 __device__ __forceinline__ bool usable(const Stat& s) { return s.s > 0.0f && s.s < __builtin_inff(); }
 
+// A row's sum of e^((x - m) / T) in 64 bits, by the wave.
+template <int TYPE>
+__device__ __forceinline__ double row_sum(const VerifyArgs& a, int row, float m, double inv) {
+    constexpr int AHEAD = 8;
+    const int lane = threadIdx.x & 63;
+    const int64_t begin = (int64_t)row * a.ld;
+    double sum = 0.0;
+    for (int64_t at = lane; at < a.V; at += 64 * AHEAD) {
+        float v[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) v[i] = at + 64 * i < a.V ? load1<TYPE>(a.x, begin + at + 64 * i) : -__builtin_inff();
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) sum += exp_of(((double)v[i] - (double)m) * inv);
+    }
+    for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o);
+    return sum;
+}
+
 __device__ __forceinline__ double lane_of(double v, int i) {
     const uint64_t b = __builtin_bit_cast(uint64_t, v);
     const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)b, i), hi = __builtin_amdgcn_readlane((uint32_t)(b >> 32), i);
@@ -255,29 +279,57 @@ __device__ __forceinline__ void walk(const VerifyArgs& a, const Space& w, int b,
     float m = 0.0f;
     int accepted = 0, last = 0;
     if (nt > 0) {
-        // p of token i of the request after token `up`
+        // What token i of the request has after token `up`: e of the row's sum s, which is off by off * s at most.
+        struct Chance {
+            double e = 0.0, s = 0.0, off = 0.0;
+            float m = 0.0f;
+        };
+        const double off = T >= FAR_LOW && T <= FAR_HIGH ? w.unsure : __builtin_inf();
         const auto chance = [&](int i, int up) {
+            Chance p;
             const int token = a.tokens[t0 + i];
-            if (up < 0 || token < 0 || token >= a.V) return 0.0;
+            if (up < 0 || token < 0 || token >= a.V) return p;
             const Stat s = joined(a, w, t0 + up, T);
-            if (!usable(s)) return 0.0;
-            if (!(T > 0.0f)) return s.first == token ? 1.0 : 0.0;
-            const float x = load1<TYPE>(a.x, (int64_t)(t0 + up) * a.ld + token);
-            return exp(((double)x - (double)s.m) * inv) / (double)s.s;
+            if (!usable(s)) return p;
+            if (T > 0.0f) {
+                const float x = load1<TYPE>(a.x, (int64_t)(t0 + up) * a.ld + token);
+                p.e = exp_of(((double)x - (double)s.m) * inv), p.s = s.s, p.off = off, p.m = s.m;
+            } else {
+                p.e = s.first == token ? 1.0 : 0.0, p.s = 1.0;
+            }
+            return p;
+        };
+        // Whether s leaves open if u (s - taken) < e.  (Never where u is 0 or NaN, nor of a sum in 64 bits, off 0.)
+        const auto in_doubt = [](const Chance& p, double u, double taken) {
+            return fabs(u * (p.s - taken) - p.e) < u * p.s * p.off;
+        };
+        // The row's sum in 64 bits that lane k's test is about.
+        const auto exact = [&](const Chance& p, int up, int k) {
+            return row_sum<TYPE>(a, t0 + up, __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(p.m), k)), inv);
         };
         if (!a.parents) {
             accepted = 1;
             for (int base = 1; base < nt; base += 64) {
                 const int i = base + lane;
-                bool good = false;
+                Chance p;
+                double u = 0.0;
                 if (i < nt) {
-                    const double p = chance(i, i - 1);
+                    p = chance(i, i - 1);
                     const int token = a.tokens[t0 + i];
                     const bool known = token >= 0 && token < a.V;
                     const double q = a.q && known ? (double)a.q[(int64_t)(t0 + i) * a.ldq + token] : 1.0;
-                    good = (double)a.u[t0 + i] * q < p;
+                    u = (double)a.u[t0 + i] * q;
                 }
-                const uint64_t no = __ballot(!good);
+                uint64_t no;
+                for (;;) {  // until nothing is in doubt before the first that is refused
+                    const bool doubt = in_doubt(p, u, 0.0);
+                    no = __ballot(!doubt && !(u * p.s < p.e));
+                    const uint64_t open = __ballot(doubt) & (no ? (no & -no) - 1 : ~0ull);
+                    if (__builtin_expect(!open, 1)) break;
+                    const int k = __builtin_ctzll(open);
+                    const double s = exact(p, base + k - 1, k);
+                    if (lane == k) p.s = s, p.off = 0.0;
+                }
                 accepted += no ? __builtin_ctzll(no) : 64;
                 if (no) break;
             }
@@ -295,7 +347,8 @@ __device__ __forceinline__ void walk(const VerifyArgs& a, const Space& w, int b,
         } else {
             const int n = min(nt, LANES);
             int par = -9, token = -1;
-            double p = 0.0, u = 0.0;
+            Chance p;
+            double u = 0.0;
             if (lane < n) {
                 par = a.parents[t0 + lane];
                 if (par < 0 || par >= lane) par = -9;
@@ -312,18 +365,33 @@ __device__ __forceinline__ void walk(const VerifyArgs& a, const Space& w, int b,
                 refused_before |= is && __builtin_amdgcn_readlane(token, j) == token;
             }
             if (par < 0) siblings = 0;
-            if (refused_before) p = 0.0;
-            double mass = 1.0;
+            if (refused_before) p.e = 0.0;
+            double taken = 0.0;
             for (uint64_t rest = siblings; __any(rest != 0); rest &= rest - 1) {
-                const double v = __shfl(p, rest ? __builtin_ctzll(rest) : 0);
-                if (rest) mass -= v;
+                const double v = __shfl(p.e, rest ? __builtin_ctzll(rest) : 0);
+                if (rest) taken += v;
             }
-            const uint64_t good = __ballot(par >= 0 && u * mass < p);
-            const uint64_t pass = __ballot((good >> lane & 1) && !(siblings & good));
-            uint64_t acc = 1;
-            for (uint64_t more = 1; more;) {  // a level of the branch at a time
-                more = __ballot((pass >> lane & 1) && (acc >> (par & 63) & 1)) & ~acc;
-                acc |= more;
+            uint64_t acc;
+            for (;;) {  // until nothing is in doubt on the walk's way
+                const bool doubt = par >= 0 && in_doubt(p, u, taken);
+                const uint64_t good = __ballot(par >= 0 && !doubt && u * (p.s - taken) < p.e);
+                const uint64_t pass = __ballot((good >> lane & 1) && !(siblings & good));
+                acc = 1;
+                for (uint64_t more = 1; more;) {  // a level of the branch at a time
+                    more = __ballot((pass >> lane & 1) && (acc >> (par & 63) & 1)) & ~acc;
+                    acc |= more;
+                }
+                // Those behind an accepted token with no sibling before them that is sure to be taken.  The
+                // earliest such token's row settles all of its children.
+                uint64_t open = __ballot(doubt && (acc >> (par & 63) & 1) && !(siblings & good));
+                if (__builtin_expect(!open, 1)) break;
+                int up = LANES, k = 0;
+                for (; open; open &= open - 1) {
+                    const int at = __builtin_ctzll(open), v = __builtin_amdgcn_readlane(par, at);
+                    if (v < up) up = v, k = at;
+                }
+                const double s = exact(p, up, k);
+                if (par == up && p.s > 0.0) p.s = s, p.off = 0.0;
             }
             accepted = __builtin_popcountll(acc);
             last = 63 - __builtin_clzll(acc);
@@ -567,6 +635,12 @@ hipError_t launch_verify(const VerifyArgs& a0, int type, int cus, hipStream_t st
     a.seg = (most + a.parts - 1) / a.parts * STEP;
     a.parts = (a.V + a.seg - 1) / a.seg;
     Space w;
+    // In units of 2^-24.  A term's exponent y (to base 2, from the row's largest; the rescalings on its way
+    // add up to no more) is a product of rounded numbers, 6 |y| off, the term 6 ln 2 |y|; over the terms
+    // that is 4.2 log2 V on average at most, 126 (the average of -y is the entropy less that of the largest
+    // term).  Exponentials are 2 off, a lane's step 13 (ten sums, a rescaling), the lanes' and
+    // waves' sums 12, the join of a part 4.
+    w.unsure = (140.0f + 13.0f * (float)(a.seg / STEP) + 4.0f * (float)a.parts) / 16777216.0f;
     const int per = std::max(1, (int)(((int64_t)a.B * most + MAX_SUMS - 1) / MAX_SUMS));
     w.chunk = per * STEP;
     w.chunks = (a.V + w.chunk - 1) / w.chunk;

@@ -187,8 +187,8 @@ int fq_window_attention(const float* q, int64_t ldq, const int32_t* lengths, con
  *   path [N]         path[cu[b] + d]: the number of the d-th accepted token; -1 behind
  *   next_tokens [B]  the next token; -1 for a request without tokens and after a row that
  *                    has a NaN or +inf logit or nothing but -inf: nothing is accepted behind it
- * A drafted token outside 0 .. V-1 is refused.  Uniforms are in [0, 1).  Sums that random numbers are compared with are in
- * 64 bits.  With parents, tokens from the 65th of a request on are reached by nothing.  N at most 2^20. */
+ * A drafted token outside 0 .. V-1 is refused.  Uniforms are in [0, 1).  Acceptance and the next token
+ * are those of sums in 64 bits.  With parents, tokens from the 65th of a request on are reached by nothing.  N at most 2^20. */
 int fq_verify_draft(const void* logits, uint32_t type, int64_t ld, int V, const int32_t* tokens,
                     const int32_t* cu, int B, int N, const int32_t* parents,
                     const float* uniforms, const float* draft_probs, int64_t ldp,
