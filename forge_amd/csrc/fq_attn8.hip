@@ -110,7 +110,7 @@ struct Shape {
     static constexpr int PART = RT * (D + 2);  // floats of a partial result
     // What an item costs beside its units, in units.
     static constexpr int OV = 256 / KU;
-    static_assert(2 * NI % WR == 0 && (WR == 1 ? NS >= 2 : NS >= 3), "copies");
+    static_assert(2 * NI % WR == 0 && (WR == 1 ? NS == 2 : NS >= 3), "copies");
     static_assert(NI + (NS - 1) * (2 * NI + 1) < 64, "vmcnt");
     static_assert(PC * (LDS + 8 * WK * RT + 64) <= 160 * 1024, "LDS");
     static_assert(PC <= MAX_GRID && (size_t)PC * PART <= MAX_PART, "workspace");
@@ -492,9 +492,6 @@ __global__ __launch_bounds__(64 * S::WAVES, (S::WAVES * S::PC + 3) / 4) void att
                         read_pages(i + NS + 1);
                         copy_k(stage);
                         wait_vm<(NS - 1) * (2 * NI + 1)>();
-                    } else if (NS > 2 && i + 2 < n) {
-                        if (NS > 3 && i + 3 < n) wait_vm<5 * NI + 2>();
-                        else wait_vm<3 * NI + 1>();
                     } else if (i + 1 < n) {
                         wait_vm<NI>();
                     } else {
