@@ -222,10 +222,15 @@ __global__ __launch_bounds__(256) void keep_kernel(KeepArgs a) {
 
 }  // namespace
 
-hipError_t launch_read8(const ReadArgs& a, int type, hipStream_t st) {
+int read8_rows(const Cache8& c) {
     // (about four pieces a lane)
     int rows = ROWS;
-    while (rows > 1 && 2 * rows * (a.c.hkv * a.c.D / 16) > 4 * 256) rows /= 2;
+    while (rows > 1 && 2 * rows * (c.hkv * c.D / 16) > 4 * 256) rows /= 2;
+    return rows;
+}
+
+hipError_t launch_read8(const ReadArgs& a, int type, hipStream_t st) {
+    const int rows = read8_rows(a.c);
     const dim3 g((unsigned)(((int64_t)a.N + rows - 1) / rows)), t(256);
     if (type == 0) hipLaunchKernelGGL(read_kernel<0>, g, t, 0, st, a, rows);
     else if (type == 1) hipLaunchKernelGGL(read_kernel<1>, g, t, 0, st, a, rows);

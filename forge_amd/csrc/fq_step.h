@@ -105,6 +105,7 @@ struct ReadArgs {
     int B, N;
     void *k, *v;
 };
+int read8_rows(const Cache8& c);  // rows of a work-group of 256 lanes
 hipError_t launch_read8(const ReadArgs& a, int type, hipStream_t st);
 
 struct KeepArgs {

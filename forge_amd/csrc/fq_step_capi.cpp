@@ -187,14 +187,16 @@ int fq_read_cache8(const int8_t* k_cache, const int8_t* v_cache, const float* k_
     if (rc != FQ_OK) return rc;
     if (type != FQ_TYPE_F32 && type != FQ_TYPE_F16 && type != FQ_TYPE_BF16) return FQ_ERR_DTYPE;
     if (!heads_ok(hkv, D, 16) || B < 1 || N < 0 || max_blocks < 1 || table_stride < max_blocks) return FQ_ERR_SHAPE;
-    if (N == 0) return FQ_OK;
-    if (!block_table || !starts || !k_out || !v_out) return FQ_ERR_NULL;
-    if (!aligned16(k_out) || !aligned16(v_out)) return FQ_ERR_ALIGN;
     fq::ReadArgs a{};
     // (the kernel reads them)
     a.c = {const_cast<int8_t*>(k_cache), const_cast<int8_t*>(v_cache), const_cast<float*>(k_scales),
            const_cast<float*>(v_scales), {num_blocks, log2_of(block_size), stride_block, stride_token, stride_head},
            hkv, D};
+    // (the grid's lanes, 256 for some rows, are 32 bits)
+    if (((int64_t)N - 1) / fq::read8_rows(a.c) + 1 >= (1 << 24)) return FQ_ERR_SHAPE;
+    if (N == 0) return FQ_OK;
+    if (!block_table || !starts || !k_out || !v_out) return FQ_ERR_NULL;
+    if (!aligned16(k_out) || !aligned16(v_out)) return FQ_ERR_ALIGN;
     a.table = {block_table, max_blocks, table_stride};
     a.starts = starts;
     a.first = first;
@@ -219,7 +221,7 @@ int fq_keep_accepted(uint32_t cache_type, void* k_cache, void* v_cache, float* k
                                        stride_token, stride_head);
     if (rc != FQ_OK) return rc;
     if (!heads_ok(hkv, D, codes ? 16 : 8) || B < 1 || N < 0 || max_blocks < 1 || table_stride < max_blocks ||
-        (int64_t)B * hkv >= (1 << 24))
+        (int64_t)B * hkv >= (1 << 23))  // (512 lanes each, the grid's lanes are 32 bits)
         return FQ_ERR_SHAPE;
     if (N == 0) return FQ_OK;
     if (!block_table || !lengths || !cu || !path || !accepted) return FQ_ERR_NULL;

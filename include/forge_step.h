@@ -149,7 +149,8 @@ int fq_qk_norm_rope8(const float* qkv, int64_t ld, int N, int hq, int hkv, int D
 /* Keys and values of a cache of 8 bits as [N][hkv][D] of type F32, F16 or BF16: rows
  * starts[b] .. starts[b+1]-1 are request b's tokens from number first[b] on (first
  * NULL: from 0), zeros where the table has no block, and for rows past starts[B].  starts
- * [B+1] rises from 0.  D: a multiple of 16, at most 512. */
+ * [B+1] rises from 0.  D: a multiple of 16, at most 512.  N: below 2^24 (2^28 where hkv * D is 512 at
+ * most). */
 int fq_read_cache8(const int8_t* k_cache, const int8_t* v_cache, const float* k_scales,
                    const float* v_scales, int num_blocks, int block_size, int hkv, int D,
                    int64_t stride_block, int64_t stride_token, int64_t stride_head,
@@ -200,7 +201,7 @@ int fq_verify_draft(const void* logits, uint32_t type, int64_t ld, int V, const 
  * and values of caches of any type, all read before any is written.  Of the first 64 only; those whose path is d,
  * or no new token, or whose slot is no block's, stay.  Caches of 8 bits: what is moved enters
  * its groups as in fq_qk_norm_rope8, with y / 127 = its scale * (its largest code / 127).  D: a multiple of
- * 8 (8 bits: 16), at most 512. */
+ * 8 (8 bits: 16), at most 512.  B * hkv: below 2^23. */
 int fq_keep_accepted(uint32_t cache_type, void* k_cache, void* v_cache, float* k_scales,
                      float* v_scales, int num_blocks, int block_size, int hkv, int D,
                      int64_t stride_block, int64_t stride_token, int64_t stride_head,

@@ -115,3 +115,10 @@ def test_host_tensors_are_refused():
                  lambda: step.verify_draft(torch.zeros(2, 9), i, i, torch.zeros(2))):
         with pytest.raises(RuntimeError, match="device tensor"):
             call()
+
+
+@pytest.mark.parametrize("call", [
+    lambda: keep(B=2 ** 22, hkv=2), lambda: keep(B=2 ** 23, hkv=1), lambda: keep(type=F16, ks=None, vs=None, B=2 ** 23, hkv=1),
+    lambda: read(hkv=1, D=16, N=2 ** 28), lambda: read(hkv=1, D=16, N=2 ** 31 - 1), lambda: read(hkv=64, D=512, N=2 ** 24)])
+def test_grids_of_more_lanes_than_32_bits_are_refused(call):
+    assert call() == SHAPE
