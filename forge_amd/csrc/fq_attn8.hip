@@ -4,10 +4,16 @@
 // next tile's products beside this one's softmax, and lagging references are those of fq_attn.hip.  What
 // differs: tiles are int8 codes, 32 keys in two groups of 16 that have a scale each.
 //
-// Scores: the fp32 queries, 16 to 23 bits of their row's largest element, are three signed bytes
+// Scores: the fp32 queries, rounded to 24 bits of their row's largest element, are three signed bytes
 // to the power-of-two base 256, so that all products with the codes are int8 matrix instructions
 // with exact sums: no key is converted, and three of them take as long as one and a half of fp16's
-// (two parts).  A score is its integer times the row's and the group's scale.
+// (two parts).  A score is its integer times the row's and the group's scale.  With m the row's largest element
+// an element is off by 2^-23 m at most and a score by m (2^-23 sum |c| + 2^-14) of the key's scale (the lowest
+// bytes' sums lose their fraction of 256): at most 2^-8 m of it for D = 128, where the cache's own rounding, half a
+// code an element, is m / 2 of it in that element alone.  Against 64 bits on the same codes (4096 keys, D = 128, L1
+// norm of the probabilities) that is 1e-7 for elements alike, 1.4e-6, 5.5e-6 and 3.3e-4 where one is 16, 64 and
+// 4096 times the others and the codes there are 0; products in fp32 stay at 6e-8.  A fourth byte, of 16
+// registers a lane and as many for its sums, does not fit: waves of 32 rows at D = 128, and all at 256, hold 256.
 //
 // Values: O = sum p s_v c.  Codes become fp16 (exactly: a byte beside 0x64 is 1024 and itself) and
 // p s_v two fp16 parts as in fq_attn.hip.  The references are of the scores plus log2 s_v, so that
@@ -20,13 +26,18 @@
 // 32 keys x 128 columns for each 32 rows), a score its probability's parts with thirteen.  Kernel + join, us, D = 128:
 // 48 requests of up to 5001 keys, one token, 4 kv heads x 7 (184 MB) 45 + 5.4; one of 131000, 13 tokens, 4 x 7
 // (135 MB, matrix work 37) 80 + 10; 32 of up to 8190, 1 to 32 tokens, 8 x 4 (410 MB at least,
-// 1160 asked of the L2s, 525 of memory; matrix work 79) 171 + 15; 64 of up to 20001 under a window of 1023, 8 x 4 (135 MB),
-// items whole, 38; one of 333 keys 9.  There vector instructions are issued in 55 % of the cycles,
+// 1160 asked of the L2s, 524 of memory; matrix work 79) 173 + 15; 64 of up to 20001 under a window of 1023,
+// 8 x 4 (135 MB), items whole, 38; one of 333 keys 9.  There vector instructions are issued in 55 % of the cycles,
 // matrix units busy in 28 %, with two waves a SIMD.  Steps (131000 keys / full batch):
 // one wave's tiles without copies ahead 73500 / 13964; copies to LDS with the scales among them, eight waves
 // a CU 107 / 219; values asked for before the softmax, conversions between the matrix instructions 94 / 186; waves
 // of 32 rows on their own, four work-groups a CU 80 / 175; the next scores' conversion held there (the
-// compiler moved it behind) 78 / 169.
+// compiler moved it behind) 78 / 169; references lowered only where a scale above 2^60 is met, for bits (333 keys
+// 5.5e-7 -> 4.9e-7 off), 80 / 173.
+//
+// A chain's tiles of rows all walk the keys from the first that any of the request's tokens sees to its last
+// token's: a prompt of 2731 tokens, 8 x 4, takes 400 + 15 us where products up to each row's own token would take 96,
+// and as long under a window of 1023 (58).
 #include "fq_attn.h"
 #include "fq_group8.h"
 

@@ -145,7 +145,8 @@ def qk_norm_rope(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor
     Into a Cache8 the tokens of a request go as plan_step's slots have them, next to each other.  16
     tokens and a kv head share a scale, the largest magnitude over 127; a token that
     needs a larger one than its group has gives the group that, and the codes held are
-    rounded again.  Infinite elements are held to the largest finite one of the group, NaN is 0."""
+    rounded again.  (A drafted token that is refused later has its part in that scale, until the
+    group's first slot is written again.)  Infinite elements are held to the largest finite one of the group, NaN is 0."""
     return _native().rope(qkv, positions, slots, table, k_cache, v_cache, bias, q_weight, k_weight, eps,
                           interleaved, _stream(qkv))
 
@@ -167,7 +168,9 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
 
     window: of the keys above, a token sees those of the window positions up to its own and
     those of the request's first sinks positions (a drafted token's position is that of plan_step);
-    what no token of the call sees is not read."""
+    what no token of the call sees is not read.
+
+    Over a Cache8 a query's elements count to 24 bits of the largest of its head's."""
     return _native().attention(q, k_cache, v_cache, block_table, lengths, cu, masks, max_new, scale,
                                window, sinks, _stream(q))
 

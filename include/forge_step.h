@@ -137,7 +137,9 @@ int fq_tree_attention(const float* q, int64_t ldq, const int32_t* lengths, const
  *                          rint(code * (old s * (1 / s)))
  * and an element's code is rint(x * (1 / s)), held to -127 .. 127, 0 for NaN and where s is
  * below 2^-126.  Codes behind the group's last new token stay as they are.  Where
- * tokens of a group come otherwise, its codes and scale are unspecified.  D: a multiple of 16. */
+ * tokens of a group come otherwise, its codes and scale are unspecified.  The old s counts all that was written
+ * since the group's first slot was, drafted tokens that were refused and are overwritten among it: a large
+ * one leaves its group a coarser scale until that slot is written again.  D: a multiple of 16. */
 int fq_qk_norm_rope8(const float* qkv, int64_t ld, int N, int hq, int hkv, int D, int rot,
                      int interleaved, const float* bias, const float* q_weight,
                      const float* k_weight, float eps, const int32_t* positions,
@@ -149,8 +151,8 @@ int fq_qk_norm_rope8(const float* qkv, int64_t ld, int N, int hq, int hkv, int D
 /* Keys and values of a cache of 8 bits as [N][hkv][D] of type F32, F16 or BF16: rows
  * starts[b] .. starts[b+1]-1 are request b's tokens from number first[b] on (first
  * NULL: from 0), zeros where the table has no block, and for rows past starts[B].  starts
- * [B+1] rises from 0.  D: a multiple of 16, at most 512.  N: below 2^24 (2^28 where hkv * D is 512 at
- * most). */
+ * [B+1] rises from 0.  D: a multiple of 16, at most 512.  N: at most 2^24 - 1 (2^28 - 16 where hkv * D is
+ * 512 or less). */
 int fq_read_cache8(const int8_t* k_cache, const int8_t* v_cache, const float* k_scales,
                    const float* v_scales, int num_blocks, int block_size, int hkv, int D,
                    int64_t stride_block, int64_t stride_token, int64_t stride_head,
@@ -162,7 +164,12 @@ int fq_read_cache8(const int8_t* k_cache, const int8_t* v_cache, const float* k_
  * token at position p sees of these keys the ones at positions j with p - j < window or j <
  * sinks; a cached token's position is its number, a new one's lengths[b] + its depth, which
  * is, with masks, the number of its mask's bits less one (each of them a token that is
- * the parent of the next; 0 for a mask of none).  window 0: no window. */
+ * the parent of the next; 0 for a mask of none).  window 0: no window.  That holds for lengths past the
+ * table's columns too, whose missing keys are not there.
+ * I8: a query's elements are rounded to 24 bits of the largest of its token and head, m, which puts a score
+ * off by |scale| m s (2^-23 (sum of |codes|) + 2^-14) at most, s the key's scale, beside fp32's roundings:
+ * below a hundredth of what the codes' own rounding may do, but more than products in fp32 where a few
+ * elements are far above the others. */
 int fq_window_attention(const float* q, int64_t ldq, const int32_t* lengths, const int32_t* cu,
                         const uint64_t* masks, int B, int N, int max_new, int hq, int hkv, int D,
                         float scale, int window, int sinks, uint32_t cache_type,
@@ -189,7 +196,8 @@ int fq_window_attention(const float* q, int64_t ldq, const int32_t* lengths, con
  *   next_tokens [B]  the next token; -1 for a request without tokens and after a row that
  *                    has a NaN or +inf logit or nothing but -inf: nothing is accepted behind it
  * A drafted token outside 0 .. V-1 is refused.  Uniforms are in [0, 1).  Acceptance and the next token
- * are those of sums in 64 bits.  With parents, tokens from the 65th of a request on are reached by nothing.  N at most 2^20. */
+ * are those of sums in 64 bits.
+ * With parents, tokens from the 65th of a request on are reached by nothing.  N at most 2^20. */
 int fq_verify_draft(const void* logits, uint32_t type, int64_t ld, int V, const int32_t* tokens,
                     const int32_t* cu, int B, int N, const int32_t* parents,
                     const float* uniforms, const float* draft_probs, int64_t ldp,
