@@ -128,6 +128,24 @@ def test_a_deep_branch_of_borders():
     assert done.path.tolist()[n - 1] == last
 
 
+@pytest.mark.parametrize("n", [64, 65, 140])
+def test_long_chains_of_borders(n):
+    """Two chains, each token next to its border: one accepted to its end, one but for its last token."""
+    V, T = 700, 1.1
+    rng = np.random.default_rng(n)
+    x = torch.from_numpy(1.5 * rng.standard_normal((2 * n, V))).float()
+    tokens, u = np.zeros(2 * n, dtype=np.int32), np.full(2 * n, 0.5, dtype=np.float32)
+    for i in range(2 * n):
+        if i % n:
+            p = softmax(x[i - 1].double().numpy(), T)
+            tokens[i] = t = next(int(t) for t in np.argsort(-p) if clear(p[t]))
+            u[i] = around(p[t])[i == 2 * n - 1]
+    done = step.verify_draft(x.cuda(), ints(tokens), ints([0, n, 2 * n]), torch.from_numpy(u).cuda(),
+                             temperature=torch.full((2,), T, device="cuda"))
+    assert done.accepted.tolist() == [n, n - 1]
+    assert done.path.tolist() == list(range(n)) + list(range(n - 1)) + [-1]
+
+
 @pytest.mark.parametrize("T", [2.0 ** -130, 2.0 ** -120, 2.0 ** 110, 2.0 ** 126])
 def test_temperatures_far_out(T):
     """Temperatures whose inverse, or whose logits' differences, leave fp32's range."""
